@@ -314,8 +314,97 @@ int kvc_decode_plan_run(const void* plan, size_t plan_bytes, int64_t t0, int64_t
  */
 int kvc_set_kernel_policy(int policy);
 
+/*
+ * Paged KV cache held in 4 bits: no counterpart in the reference, whose int4
+ * compressor (quantization_only.py:56-198) only decodes back to dense tensors.
+ *
+ * A layer's pool is n_pages pages of kvc_kv4_page_bytes() bytes (16-byte
+ * aligned); a page holds page_size (16, 32, 64, 128 or 256) tokens of every KV
+ * head.  Each token's head (head_dim 64 or 128) is quantised in groups of
+ * group_size (32, 64 or 128, dividing head_dim) elements:
+ *   x = zero + scale * q,  q = clamp(rint((x - zero) / scale), -8, 7),
+ *   scale = (max - min) / 15,  zero = min + 8 * scale,
+ * scale and zero rounded to float16, q exactly rounded (half to even).
+ * Magnitudes above 65024 are held as 65024; a NaN makes its whole group NaN.
+ * The order of the bytes inside a page is the library's own.
+ *
+ * `table` holds the page ids of each sequence, (rows, table_stride) int32 on
+ * the device: token t of row r is in page table[r][t / page_size].  An entry
+ * that is no page sets the device error word (401) and is skipped.
+ */
+typedef struct {
+  const int32_t* table;
+  int64_t table_stride;
+  int64_t n_pages;
+  int32_t n_kv, head_dim, page_size, group_size;
+} kvc_kv4_layout;
+
+/*
+ * The new tokens (or queries) of one step, device arrays of int32:
+ * rows[i] is sequence i's table row, kv_len[i] its cached tokens with the
+ * step's own among them (they are the last ones), q_start (n_seqs + 1) the
+ * prefix sums of the step's tokens.  For kvc_kv4_write, half_start (n_seqs + 1)
+ * counts the aligned 8-token halves of units that each sequence's new tokens
+ * touch, half_seq[j] is the sequence of half j, n_halves their number.
+ */
+typedef struct {
+  const int32_t *rows, *kv_len, *q_start, *half_seq, *half_start;
+  int64_t n_halves;
+  int32_t n_seqs, max_new; /* max_new: most tokens of one sequence */
+  int64_t n_tokens;        /* q_start[n_seqs] */
+} kvc_kv4_step;
+
+/*
+ * Split of the cached tokens into items of `chunk` tokens (a multiple of 32)
+ * for kvc_kv4_attend, device arrays of int32: item j covers tokens
+ * [item_first[j], item_first[j] + chunk) of sequence item_seq[j]; the items of
+ * sequence i are item_start[i] .. item_start[i + 1] - 1, at least one.
+ * max_items: most items of one sequence.
+ */
+typedef struct {
+  const int32_t *item_seq, *item_first, *item_start;
+  int64_t n_items;
+  int32_t chunk, max_items;
+} kvc_kv4_split;
+
+int64_t kvc_kv4_page_bytes(int n_kv, int head_dim, int page_size, int group_size);
+
+/* Quantise the step's K and V (dtype KVC_F32 / F16 / BF16; element strides of
+ * a sequence, a token and a head, features contiguous) into their pages.
+ * packed: the tokens of all sequences lie in one row of tokens (seq_stride is
+ * not used).  Only the step's own tokens' bytes are written; the pages they lie
+ * in must not be shared with another sequence. */
+int kvc_kv4_write(const kvc_kv4_layout* layout, const kvc_kv4_step* step, void* pool, const void* k, const void* v,
+                  int dtype, int64_t seq_stride, int64_t token_stride, int64_t head_stride, int packed,
+                  void* stream);
+
+/* Tokens [t0, t1) of table row `row` as dense (n_layers, n_kv, t1 - t0,
+ * head_dim) K and V; the layers' pools are layer_bytes apart. */
+int kvc_kv4_read(const kvc_kv4_layout* layout, const void* pool, int64_t layer_bytes, int n_layers, int row,
+                 int64_t t0, int64_t t1, int dtype, void* k_out, void* v_out, void* stream);
+
+/* softmax(scale q k^T) v of the step's queries (n_q heads, a multiple of n_kv)
+ * over their sequences' pages.  causal: query i of a sequence's n sees the
+ * first kv_len - n + 1 + i tokens, otherwise all kv_len.  A query that sees
+ * nothing gets zeros.  Strides in elements, as for kvc_kv4_write. */
+size_t kvc_kv4_attend_workspace_bytes(const kvc_kv4_layout* layout, const kvc_kv4_step* step,
+                                      const kvc_kv4_split* split, int n_q);
+int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* step, const kvc_kv4_split* split,
+                   const void* pool, int n_q, const void* q, int64_t q_seq_stride, int64_t q_token_stride,
+                   int64_t q_head_stride, void* out, int64_t o_seq_stride, int64_t o_token_stride,
+                   int64_t o_head_stride, int packed, int dtype, int causal, float scale, void* workspace,
+                   size_t ws_bytes, void* stream);
+
+/* Copy page src[i] to page dst[i] in each of up to KVC_MAX_CELLS pools of
+ * n_pages pages of page_bytes bytes (any element type).  src and dst are HOST
+ * arrays, read before the call returns.  No page may be written twice, or read
+ * and written, by one call. */
+int kvc_copy_pages(int n_pools, void* const* pools, int64_t n_pages, int64_t page_bytes, int64_t n_pairs,
+                   const int32_t* src, const int32_t* dst, void* stream);
+
 /* Reads and clears the device-side error word (an mbarrier wait in a
- * tensor-core kernel that gave up records a nonzero code).  Synchronises
+ * tensor-core kernel that gave up, or a page table entry out of range, records
+ * a nonzero code).  Synchronises
  * the device: a diagnostic, not for the hot path. */
 int kvc_device_error(int* code);
 

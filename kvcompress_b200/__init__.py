@@ -6,7 +6,7 @@ schema, cache); the arithmetic runs in the hand-written CUDA kernels of
 """
 
 from kvcompress_b200.api import CompressionHandle, CompressionStats, disable_compression, enable_compression
-from kvcompress_b200.cache import CacheManager, CompressedKVCache, CompressionMetadata
+from kvcompress_b200.cache import CacheManager, CompressedKVCache, CompressionMetadata, PagedKVCache
 from kvcompress_b200.compressor import (CompressedPayload, CompressorStats, DecodeStream, FlashJoLTCompressor,
                                         IdentityCompressor, IntQuantOnlyCompressor, JoLTCompressor,
                                         JointAllocator, KVCompressor, build_compressor, flashjolt_cap,
@@ -15,5 +15,5 @@ from kvcompress_b200.compressor import (CompressedPayload, CompressorStats, Deco
 __all__ = ["CacheManager", "CompressedKVCache", "CompressedPayload", "CompressionHandle", "CompressionMetadata",
            "CompressionStats", "disable_compression", "enable_compression",
            "CompressorStats", "DecodeStream", "FlashJoLTCompressor", "IdentityCompressor", "IntQuantOnlyCompressor",
-           "JoLTCompressor", "JointAllocator", "KVCompressor", "build_compressor", "flashjolt_cap",
+           "JoLTCompressor", "JointAllocator", "KVCompressor", "PagedKVCache", "build_compressor", "flashjolt_cap",
            "supported_methods"]

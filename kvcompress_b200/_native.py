@@ -13,7 +13,7 @@ import threading
 
 from kvcompress_b200 import _build
 
-__all__ = ["lib", "check", "KVC", "ptr_array"]
+__all__ = ["lib", "check", "KVC", "Kv4Layout", "Kv4Split", "Kv4Step", "ptr_array"]
 
 _LOCK = threading.Lock()
 _LIB = None
@@ -40,6 +40,29 @@ class KVC:
     ERR_WORKSPACE = -5
     ERR_UNSUPPORTED = -8
 
+
+class Kv4Layout(ctypes.Structure):
+    """``kvc_kv4_layout``."""
+
+    _fields_ = [("table", P), ("table_stride", I64), ("n_pages", I64), ("n_kv", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("page_size", ctypes.c_int32), ("group_size", ctypes.c_int32)]
+
+
+class Kv4Step(ctypes.Structure):
+    """``kvc_kv4_step``."""
+
+    _fields_ = [("rows", P), ("kv_len", P), ("q_start", P), ("half_seq", P), ("half_start", P), ("n_halves", I64),
+                ("n_seqs", ctypes.c_int32), ("max_new", ctypes.c_int32), ("n_tokens", I64)]
+
+
+class Kv4Split(ctypes.Structure):
+    """``kvc_kv4_split``."""
+
+    _fields_ = [("item_seq", P), ("item_first", P), ("item_start", P), ("n_items", I64),
+                ("chunk", ctypes.c_int32), ("max_items", ctypes.c_int32)]
+
+
+_LAYOUT, _STEP, _SPLIT = (ctypes.POINTER(t) for t in (Kv4Layout, Kv4Step, Kv4Split))
 
 _SIGNATURES = {
     "kvc_last_error": (ctypes.c_char_p, []),
@@ -75,6 +98,13 @@ _SIGNATURES = {
     "kvc_set_kernel_policy": (I, [I]),
     "kvc_device_error": (I, [ctypes.POINTER(I)]),
     "kvc_cast": (I, [I64, P, I, P, I, P]),
+    "kvc_kv4_page_bytes": (I64, [I, I, I, I]),
+    "kvc_kv4_write": (I, [_LAYOUT, _STEP, P, P, P, I, I64, I64, I64, I, P]),
+    "kvc_kv4_read": (I, [_LAYOUT, P, I64, I, I, I64, I64, I, P, P, P]),
+    "kvc_kv4_attend_workspace_bytes": (SZ, [_LAYOUT, _STEP, _SPLIT, I]),
+    "kvc_kv4_attend": (I, [_LAYOUT, _STEP, _SPLIT, P, I, P, I64, I64, I64, P, I64, I64, I64, I, I, I,
+                           ctypes.c_float, P, SZ, P]),
+    "kvc_copy_pages": (I, [I, PP, I64, I64, I64, P, P, P]),
 }
 
 

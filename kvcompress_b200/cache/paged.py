@@ -1,0 +1,310 @@
+"""Paged KV cache held in 4 bits, and the attention that reads it.
+
+No counterpart in the reference, whose int4 compressor
+(kvcompress/compressor/quantization_only.py:56-198) only decodes back to dense
+tensors: here queries attend the packed codes, sequences of any length share
+one pool of pages, and pages are forked, compacted and freed.
+
+Each token's head is quantised in groups of ``group_size`` elements as ``x =
+zero + scale * q`` with ``q`` in [-8, 7], ``scale = (max - min) / 15`` and ``zero =
+min + 8 * scale`` rounded to float16, ``q`` rounded half to even; a token of a
+head costs ``head_dim / 2 + 4 * head_dim / group_size`` bytes each for K and V.
+Magnitudes above 65024 are held as 65024; a NaN makes its group NaN.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass, field
+from typing import Any, Sequence
+
+import numpy as np
+import torch
+
+from kvcompress_b200 import ops
+from kvcompress_b200._native import Kv4Layout, Kv4Split, Kv4Step
+from kvcompress_b200.cache.pages import PageTable
+
+__all__ = ["CacheStep", "PagedKVCache"]
+
+_CHUNK = 256  # tokens of the smallest item of the attention's split
+
+
+@dataclass
+class CacheStep:
+    """The new tokens, or the queries, of some sequences: made by
+    ``PagedKVCache.extend`` / ``view``, used by every layer's ``write`` / ``attend``.
+
+    ``counts[i]`` tokens belong to ``seqs[i]``, the last ones of its
+    ``lengths[i]`` cached tokens.  A step is good until a fork, free, truncate
+    or compact changes the cache."""
+
+    seqs: list[int]
+    counts: list[int]
+    lengths: list[int]
+    writable: bool
+    epoch: int
+    cache: Any = field(repr=False)
+    meta: torch.Tensor = field(repr=False)  # device arrays that ``desc`` points into
+    desc: Kv4Step = field(repr=False)
+    splits: dict[int, tuple[Kv4Split, torch.Tensor]] = field(default_factory=dict, repr=False)
+
+    @property
+    def tokens(self) -> int:
+        return int(self.desc.n_tokens)
+
+
+def _upload(arrays: Sequence[np.ndarray], device: torch.device) -> tuple[torch.Tensor, list[int]]:
+    """int32 arrays in one device buffer (one asynchronous copy from pinned
+    memory, which torch keeps until the copy is done) and their addresses."""
+    host = torch.empty(max(1, sum(a.size for a in arrays)), dtype=torch.int32, pin_memory=True)
+    view, at, offsets = host.numpy(), 0, []
+    for a in arrays:
+        view[at:at + a.size] = a
+        offsets.append(at)
+        at += a.size
+    buf = host.to(device, non_blocking=True)
+    return buf, [buf.data_ptr() + 4 * o for o in offsets]
+
+
+def _prefix(counts: np.ndarray) -> np.ndarray:
+    out = np.zeros(counts.size + 1, dtype=np.int64)
+    np.cumsum(counts, out=out[1:])
+    return out
+
+
+def split_chunk(lengths: np.ndarray, copies: int, slots: int) -> int:
+    """Tokens of an item so that ``copies`` CTAs an item fill ``slots`` resident
+    CTAs evenly: of one to four full waves (or no split at all) the choice with
+    the least waves x (tokens + a CTA's fixed cost in tokens)."""
+    longest = int(lengths.max(initial=1))
+    total = max(1, int(lengths.sum()))
+    best, cost = 0, float("inf")
+    for waves in (1, 2, 3, 4, 0):
+        chunk = _CHUNK
+        if waves == 0:
+            chunk = longest
+        else:
+            chunk = max(_CHUNK, -(-total * copies // (waves * slots)))
+        chunk = -(-chunk // 32) * 32
+        while waves and chunk < longest:
+            items = int(np.maximum(1, -(-lengths // chunk)).sum()) * copies
+            if items <= waves * slots:
+                break
+            chunk += max(32, chunk // 64 // 32 * 32)
+        items = int(np.maximum(1, -(-lengths // chunk)).sum()) * copies
+        c = -(-items // slots) * (min(chunk, longest) + 192)
+        if c < cost:
+            best, cost = chunk, c
+    return best
+
+
+class PagedKVCache:
+    """K and V of ``n_layers`` layers in 4 bits, in pages of ``page_size`` tokens.
+
+    ``page_size`` is 16, 32, 64, 128 or 256, ``head_dim`` 64 or 128, ``group_size``
+    32, 64 or 128 (default ``head_dim``).  ``max_sequences`` sequences of up to
+    ``max_tokens`` tokens can live at once (their page table is ``max_sequences *
+    max_tokens / page_size`` int32).
+
+    A step of a model::
+
+        step = cache.extend(seqs, [1] * len(seqs))      # room for the new tokens
+        for layer in range(n_layers):
+            cache.write(layer, k, v, step)
+            out = cache.attend(layer, q, step)
+
+    Launches go to the current stream; use a cache from one stream at a time.
+    ``write`` and ``attend`` may be captured into a CUDA graph (not ``extend``,
+    ``view``, ``fork``, ``compact``), which then repeats that step.  There is no
+    gradient through a cache in 4 bits.
+    """
+
+    def __init__(self, *, n_layers: int, n_pages: int, n_kv_heads: int, head_dim: int, page_size: int = 64,
+                 group_size: int | None = None, max_sequences: int = 256, max_tokens: int | None = None,
+                 device: torch.device | str = "cuda") -> None:
+        self.n_layers, self.n_kv_heads, self.head_dim = int(n_layers), int(n_kv_heads), int(head_dim)
+        self.page_size = int(page_size)
+        self.group_size = self.head_dim if group_size is None else int(group_size)
+        if self.n_layers < 1 or self.n_kv_heads < 1:
+            raise ValueError("PagedKVCache: n_layers and n_kv_heads must be positive")
+        if self.head_dim not in (64, 128):
+            raise ValueError(f"PagedKVCache: head_dim must be 64 or 128, got {head_dim}")
+        if self.page_size not in (16, 32, 64, 128, 256):
+            raise ValueError(f"PagedKVCache: page_size must be 16, 32, 64, 128 or 256, got {page_size}")
+        if self.group_size not in (32, 64, 128) or self.head_dim % self.group_size:
+            raise ValueError(f"PagedKVCache: group_size must be 32, 64 or 128 and divide head_dim, got {group_size}")
+        self.pages = PageTable(n_pages, page_size, max_sequences,
+                               int(n_pages) * self.page_size if max_tokens is None else max_tokens)
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise RuntimeError(f"PagedKVCache: kvcompress_b200 runs on CUDA tensors only (got {device})")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.device = device
+        self.page_bytes = ops.kv4_page_bytes(self.n_kv_heads, self.head_dim, self.page_size, self.group_size)
+        # zeros: a page's bytes are defined before its first tokens are written
+        self.pool = torch.zeros(self.n_layers, self.pages.n_pages, self.page_bytes, dtype=torch.uint8, device=device)
+        self.table = torch.zeros(self.pages.table.shape, dtype=torch.int32, device=device)
+        self._layers = [self.pool.data_ptr() + i * self.pool.stride(0) for i in range(self.n_layers)]
+        self._layout = Kv4Layout(self.table.data_ptr(), self.table.stride(0), self.pages.n_pages, self.n_kv_heads,
+                                 self.head_dim, self.page_size, self.group_size)
+        self._slots = 2 * torch.cuda.get_device_properties(device).multi_processor_count
+
+    # ---- sequences ---------------------------------------------------------
+
+    def add(self) -> int:
+        """A new empty sequence's id."""
+        return self.pages.add()
+
+    def length(self, seq: int) -> int:
+        """Tokens of ``seq`` in the cache."""
+        return self.pages.length(seq)
+
+    def free(self, seq: int) -> None:
+        """Forget ``seq``; pages that no fork shares become free."""
+        self.pages.free(seq)
+
+    def truncate(self, seq: int, length: int) -> None:
+        """Drop ``seq``'s tokens from ``length`` on (drafts that were rejected)."""
+        self.pages.truncate(seq, length)
+
+    def fork(self, seq: int) -> int:
+        """A new sequence that continues ``seq``: it shares the pages, and whichever
+        of the two is extended first takes a copy of a partly filled last page."""
+        return self.pages.fork(seq)
+
+    def compact(self) -> int:
+        """Move the used pages to the pool's start; returns the number of moved pages."""
+        moves = self.pages.compact()
+        self._copy(moves)
+        self._sync()
+        return len(moves)
+
+    def memory_used(self) -> int:
+        """Bytes of the pages in use, all layers."""
+        return (self.pages.n_pages - self.pages.free_pages) * self.page_bytes * self.n_layers
+
+    # ---- steps -----------------------------------------------------------
+
+    def extend(self, seqs: Sequence[int], counts: Sequence[int]) -> CacheStep:
+        """Room for ``counts[i]`` new tokens of ``seqs[i]`` (``RuntimeError`` without
+        enough free pages, nothing changed then); the step to write and attend them with."""
+        seqs, counts = [int(s) for s in seqs], [int(n) for n in counts]
+        self._copy(self.pages.extend(seqs, counts))
+        return self._step(seqs, counts, True)
+
+    def view(self, seqs: Sequence[int], counts: Sequence[int]) -> CacheStep:
+        """A step that adds nothing: ``counts[i]`` queries over ``seqs[i]`` as it is.
+        Under a causal mask they stand at its last ``counts[i]`` positions (queries
+        before its first token see nothing).  A sequence may be named twice."""
+        seqs, counts = [int(s) for s in seqs], [int(n) for n in counts]
+        if len(seqs) != len(counts):
+            raise ValueError(f"PagedKVCache.view: {len(seqs)} sequences but {len(counts)} query counts")
+        if any(n < 0 for n in counts):
+            raise ValueError("PagedKVCache.view: query counts must not be negative")
+        return self._step(seqs, counts, False)
+
+    def _step(self, seqs: list[int], counts: list[int], writable: bool) -> CacheStep:
+        self._sync()
+        n = np.array(counts, dtype=np.int64)
+        lengths = np.array([self.pages.length(s) for s in seqs], dtype=np.int64)
+        rows = np.array([self.pages.row(s) for s in seqs], dtype=np.int64)
+        if int(n.sum()) > 2 ** 31 - 1:
+            raise ValueError("PagedKVCache: too many tokens in one step")
+        halves = np.zeros_like(n)
+        if writable:  # aligned runs of 8 tokens that the new ones touch
+            halves = np.where(n > 0, (lengths - 1) // 8 - (lengths - n) // 8 + 1, 0)
+        q_start, half_start = _prefix(n), _prefix(halves)
+        half_seq = np.repeat(np.arange(len(seqs)), halves)
+        meta, at = _upload((rows, lengths, q_start, half_seq, half_start), self.device)
+        desc = Kv4Step(at[0], at[1], at[2], at[3], at[4], int(half_start[-1]), len(seqs), int(n.max(initial=0)),
+                       int(q_start[-1]))
+        return CacheStep(seqs, counts, lengths.tolist(), writable, self.pages.epoch, self, meta, desc)
+
+    def _split(self, step: CacheStep, copies: int) -> Kv4Split:
+        got = step.splits.get(copies)
+        if got is None:
+            lengths = np.array(step.lengths, dtype=np.int64)
+            chunk = split_chunk(lengths, copies, self._slots)
+            items = np.maximum(1, -(-lengths // chunk))
+            start = _prefix(items)
+            seq = np.repeat(np.arange(len(step.seqs)), items)
+            first = (np.arange(int(start[-1])) - start[seq]) * chunk
+            buf, at = _upload((seq, first, start), self.device)
+            got = step.splits[copies] = (Kv4Split(at[0], at[1], at[2], int(start[-1]), chunk,
+                                                  int(items.max(initial=1))), buf)
+        return got[0]
+
+    def _check(self, what: str, layer: int, step: CacheStep) -> int:
+        if step.cache is not self:
+            raise ValueError(f"PagedKVCache.{what}: the step belongs to another cache")
+        if step.epoch != self.pages.epoch:
+            raise RuntimeError(f"PagedKVCache.{what}: sequences were forked, freed, truncated or compacted since the "
+                               "step was made; make it again")
+        if not 0 <= layer < self.n_layers:
+            raise IndexError(f"PagedKVCache.{what}: layer {layer} of {self.n_layers}")
+        return self._layers[layer]
+
+    # ---- data ---------------------------------------------------------------
+
+    def write(self, layer: int, key: torch.Tensor, value: torch.Tensor, step: CacheStep) -> None:
+        """Quantise the step's new K and V of ``layer`` into the pages.
+
+        ``key`` / ``value``: ``(tokens, n_kv_heads, head_dim)``, the sequences' tokens
+        one after the other, or ``(B, n_kv_heads, T, head_dim)`` when every sequence
+        has T new tokens; float32, float16 or bfloat16, any strides with contiguous
+        features."""
+        pool = self._check("write", layer, step)
+        if not step.writable:
+            raise ValueError("PagedKVCache.write: a view adds no tokens; use a step from extend()")
+        ops.kv4_write(self._layout, step.desc, pool, key, value, self.device)
+
+    def attend(self, layer: int, query: torch.Tensor, step: CacheStep, *, causal: bool = True,
+               scale: float | None = None) -> torch.Tensor:
+        """Attention of the step's queries over their sequences' cached tokens.
+
+        ``query``: ``(tokens, n_heads, head_dim)`` or ``(B, n_heads, T, head_dim)``,
+        ``n_heads`` a multiple of ``n_kv_heads`` (consecutive query heads share a KV
+        head); the result has its shape and dtype.  ``causal``: a query sees the
+        tokens up to its own position, otherwise all cached tokens of its sequence;
+        one that sees none gets zeros.  ``scale`` defaults to ``head_dim ** -0.5``."""
+        pool = self._check("attend", layer, step)
+        return ops.kv4_attend(self._layout, step.desc, lambda copies: self._split(step, copies), pool, query,
+                              causal=causal, scale=self.head_dim ** -0.5 if scale is None else float(scale),
+                              device=self.device)
+
+    def read(self, seq: int, *, layers: Sequence[int] | None = None, t0: int = 0, t1: int | None = None,
+             dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+        """Tokens ``[t0, t1)`` of ``seq`` decoded: K and V, each ``(layers, n_kv_heads,
+        t1 - t0, head_dim)``.  ``k[i]``, ``v[i]`` are the cells a ``KVCompressor`` takes.
+        ``layers`` (default all) is a range of consecutive layers."""
+        n = self.pages.length(seq)
+        t0, t1 = int(t0), n if t1 is None else int(t1)
+        if not 0 <= t0 <= t1 <= n:
+            raise ValueError(f"PagedKVCache.read: bad token range [{t0}, {t1}) of {n}")
+        pick = list(range(self.n_layers)) if layers is None else [int(i) for i in layers]
+        if pick and (pick != list(range(pick[0], pick[0] + len(pick))) or pick[0] < 0 or pick[-1] >= self.n_layers):
+            raise ValueError(f"PagedKVCache.read: layers must be consecutive and within {self.n_layers}, got {pick}")
+        self._sync()
+        return ops.kv4_read(self._layout, self._layers[pick[0]] if pick else self._layers[0], self.pool.stride(0),
+                            len(pick), self.pages.row(seq), t0, t1, dtype, self.device)
+
+    # ---- internals ---------------------------------------------------------
+
+    def _copy(self, pairs: list[tuple[int, int]]) -> None:
+        if pairs:
+            ops.copy_pages(self.pool, [s for s, _ in pairs], [d for _, d in pairs])
+
+    def _sync(self) -> None:
+        """Bring the device's page table up to the host's."""
+        dirty = self.pages.dirty
+        if not dirty:
+            return
+        width = self.pages.max_pages
+        at = np.unique(np.concatenate([np.arange(r * width + a, r * width + b) for r, a, b in dirty]))
+        host = torch.empty(2, at.size, dtype=torch.int64, pin_memory=True)
+        host[0] = torch.from_numpy(at)
+        host[1] = torch.from_numpy(self.pages.table.reshape(-1)[at].astype(np.int64))
+        dev = host.to(self.device, non_blocking=True)
+        self.table.view(-1).index_copy_(0, dev[0], dev[1].to(torch.int32))
+        dirty.clear()

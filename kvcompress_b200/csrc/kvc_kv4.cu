@@ -1,0 +1,407 @@
+// Writing, reading and moving the pages of the 4-bit KV cache.
+//
+// All three are bound by memory.  A warp of the write and read kernels takes
+// 8 tokens of one head's K or V, 4 lanes a token: lane c of a token holds the
+// features 32 w + 8 c + 0..7, which is both a 16-byte load of a 16-bit input
+// (4 lanes: 64 contiguous bytes) and word w of K's chunk c, so K's codes need
+// no exchange at all and V's one shuffle a word with the neighbouring token.
+#include <algorithm>
+
+#include "kvc_kv4.cuh"
+#include "kvc_tc.cuh"
+
+namespace kvc {
+
+int kv4_read_device_error(int* out) {
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, tc::g_kvc_device_error, sizeof(int));
+  if (e != cudaSuccess) return fail(KVC_ERR_LAUNCH, std::string("device error read: ") + cudaGetErrorString(e));
+  *out = v;
+  int zero = 0;
+  cudaMemcpyToSymbol(tc::g_kvc_device_error, &zero, sizeof(int));
+  return KVC_OK;
+}
+
+namespace kv4 {
+namespace {
+
+// ---- element access ---------------------------------------------------------
+
+// Eight consecutive elements as float32.  vec: 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool vec, float (&x)[8]) {
+  if (!vec) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = Elt<T>::to_f32(p[i]);
+    return;
+  }
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      T e[2];
+      memcpy(e, &w[i], 4);
+      x[2 * i] = Elt<T>::to_f32(e[0]);
+      x[2 * i + 1] = Elt<T>::to_f32(e[1]);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const T e[2] = {Elt<T>::from(x[2 * i]), Elt<T>::from(x[2 * i + 1])};
+      memcpy(&w[i], e, 4);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// ---- the quantiser ------------------------------------------------------------
+
+// scale = (hi - lo) / 15 and zero = lo + 8 scale, each to float32 and then to
+// float16; the quotient and the sum are formed in 64 bits so that a float16
+// step is never decided by an earlier rounding.  A NaN in the group makes both
+// NaN.
+__device__ __forceinline__ __half2 params_of(float lo, float hi, bool nan) {
+  if (nan) return __half2half2(__ushort_as_half(0x7FFF));
+  const __half s = __float2half_rn((float)(((double)hi - (double)lo) / 15.0));
+  const __half z = __float2half_rn((float)((double)lo + 8.0 * (double)__half2float(s)));
+  return __halves2half2(s, z);
+}
+
+// clamp(rint((x - z) / s), -8, 7) of the exact quotient.  (x - z) * (1 / s) in
+// float32 is within 1.5e-6 of it (|quotient| <= 8.5, three roundings), so only
+// a result that close to a half needs more: there the sign of
+// (x - z) - (n + 1/2) s decides, which is exact: (n + 1/2) s has 16 bits, the
+// rounded x - z is next to it (their difference is exact by Sterbenz' lemma),
+// and the rounding error of x - z is itself a float32 (Knuth's two-sum).
+// NaN gives -8.
+__device__ __forceinline__ float level_of(float x, float s, float z, float inv) {
+  const float a = x - z;
+  const float t = fminf(fmaxf(a * inv, -8.0f), 7.0f);
+  float n = rintf(t);
+  if (fabsf(t - n) > 0.499996f) {
+    const float f = floorf(t), h = (f + 0.5f) * s;
+    const float bb = a - x;
+    const float err = (x - (a - bb)) + (-z - bb);
+    const float res = (a - h) + err;
+    const bool odd = (((int)f) & 1) != 0;
+    n = res > 0.0f || (res == 0.0f && odd) ? f + 1.0f : f;
+  }
+  return n;
+}
+
+struct KvIn {
+  const void *k, *v;
+  int64_t sb, st, sh;  // strides of a sequence, a token and a head, in elements
+  int packed;          // tokens of all sequences in one row of tokens (sb unused)
+  int vec;             // 16-byte loads are aligned
+};
+
+// W = D / 32 words a lane; WPG words a quantisation group.
+template <typename T, int D, int WPG>
+__global__ void __launch_bounds__(128) kv4_write_kernel(Layout L, Step S, uint8_t* pool, KvIn in, int64_t n_halves,
+                                                        const int32_t* __restrict__ half_seq,
+                                                        const int32_t* __restrict__ half_start) {
+  constexpr int W = D / 32, NG = W / WPG;
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int64_t id = blockIdx.x * 4LL + (threadIdx.x >> 5);
+  if (id >= n_halves * L.n_kv * 2) return;
+  const int is_v = (int)(id & 1), h = (int)((id >> 1) % L.n_kv);
+  const int64_t half = (id >> 1) / L.n_kv;
+  const int b = half_seq[half];
+  const int len = S.kv_len[b], q0 = S.q_start[b], n = S.q_start[b + 1] - q0, first = len - n;
+  const int tok0 = (first / 8 + (int)(half - half_start[b])) * 8, pos = tok0 + r;
+  const bool valid = pos >= first && pos < len;
+  const int64_t page = page_of(L, S.rows[b], tok0, &tc::g_kvc_device_error);
+  if (page < 0) return;
+
+  float x[W][8];
+  if (valid) {
+    const int64_t row = (int64_t)(pos - first) + (in.packed ? q0 : 0);
+    const T* src = static_cast<const T*>(is_v ? in.v : in.k) + (in.packed ? 0 : b * in.sb) + row * in.st + h * in.sh;
+#pragma unroll
+    for (int w = 0; w < W; ++w) load8(src + 32 * w + 8 * c, in.vec != 0, x[w]);
+  } else {
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[w][e] = 0.0f;
+  }
+
+  uint8_t* unit = pool + unit_off<D>(L, page, h, tok0);
+  const int t = pos & 15, p = (tok0 >> 3) & 1;
+  uint32_t word[W];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    float lo = 3.0e38f, hi = -3.0e38f;
+    bool nan = false;
+#pragma unroll
+    for (int w = g * WPG; w < (g + 1) * WPG; ++w)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        nan |= x[w][e] != x[w][e];
+        x[w][e] = fminf(fmaxf(x[w][e], -kLimit), kLimit);
+        lo = fminf(lo, x[w][e]);
+        hi = fmaxf(hi, x[w][e]);
+      }
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      nan |= __shfl_xor_sync(0xffffffffu, (int)nan, o) != 0;
+    }
+    const __half2 sz = params_of(lo, hi, nan);
+    const float s = __low2float(sz), z = __high2float(sz), inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
+#pragma unroll
+    for (int w = g * WPG; w < (g + 1) * WPG; ++w) {
+      uint32_t bits = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bits |= (uint32_t)((int)level_of(x[w][e], s, z, inv) + 8) << (4 * (e ^ 1));
+      word[w] = bits;
+    }
+    if (valid && c == 0)
+      reinterpret_cast<__half2*>(unit + (is_v ? vp_base(D, NG) : kp_base(D)))[t * NG + g] = sz;
+  }
+
+  if (!is_v) {
+    if (!valid) return;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(unit + k_chunk<D>(t, c));
+    if constexpr (W == 4) *reinterpret_cast<uint4*>(dst) = make_uint4(word[0], word[1], word[2], word[3]);
+    else *reinterpret_cast<uint2*>(dst) = make_uint2(word[0], word[1]);
+    return;
+  }
+  const int cc = r >> 1, odd = r & 1;
+  if (tok0 >= first && tok0 + 8 <= len) {
+    // token pairs are neighbouring lanes (lane ^ 4): the even token's lane
+    // takes features 4 (2 c) .. of both, the odd one's the next four
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? word[w] & 0xFFFFu : word[w] >> 16, 4);
+      word[w] = odd ? got | (word[w] & 0xFFFF0000u) : (word[w] & 0xFFFFu) | got << 16;
+    }
+    uint32_t* dst = reinterpret_cast<uint32_t*>(unit + v_chunk<D>(p, (2 * c + odd) * 4 + cc));
+    if constexpr (W == 4) *reinterpret_cast<uint4*>(dst) = make_uint4(word[0], word[1], word[2], word[3]);
+    else *reinterpret_cast<uint2*>(dst) = make_uint2(word[0], word[1]);
+  } else if (valid) {
+    // other tokens of the half keep their codes: two bytes hold four features
+    // of one token
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        *reinterpret_cast<uint16_t*>(unit + v_chunk<D>(p, (2 * c + j) * 4 + cc) + w * 4 + odd * 2) =
+            (uint16_t)(word[w] >> (16 * j));
+  }
+}
+
+// Dense (layers, n_kv, t1 - t0, D) K and V of tokens [t0, t1) of one sequence.
+template <typename T, int D, int WPG>
+__global__ void __launch_bounds__(128) kv4_read_kernel(Layout L, const uint8_t* pool, int64_t layer_bytes, int row,
+                                                       int t0, int t1, int64_t n_halves, int64_t n_warps,
+                                                       T* __restrict__ ko, T* __restrict__ vo) {
+  constexpr int W = D / 32, NG = W / WPG;
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int64_t id = blockIdx.x * 4LL + (threadIdx.x >> 5);
+  if (id >= n_warps) return;
+  const int is_v = (int)(id & 1), h = (int)((id >> 1) % L.n_kv);
+  const int64_t half = ((id >> 1) / L.n_kv) % n_halves, layer = ((id >> 1) / L.n_kv) / n_halves;
+  const int tok0 = (int)(t0 / 8 + half) * 8, pos = tok0 + r, t = pos & 15;
+  const int64_t page = page_of(L, row, tok0, &tc::g_kvc_device_error);
+  if (page < 0) return;
+  const uint8_t* unit = pool + layer * layer_bytes + unit_off<D>(L, page, h, tok0);
+
+  const int odd = r & 1, p = (tok0 >> 3) & 1;
+  const uint32_t* src = reinterpret_cast<const uint32_t*>(
+      unit + (is_v ? v_chunk<D>(p, (2 * c + odd) * 4 + (r >> 1)) : k_chunk<D>(t, c)));
+  uint32_t word[W];
+  if constexpr (W == 4) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(src));
+    word[0] = a.x, word[1] = a.y, word[2] = a.z, word[3] = a.w;
+  } else {
+    const uint2 a = __ldg(reinterpret_cast<const uint2*>(src));
+    word[0] = a.x, word[1] = a.y;
+  }
+  if (is_v) {  // the write's exchange again: it is its own inverse
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? word[w] & 0xFFFFu : word[w] >> 16, 4);
+      word[w] = odd ? got | (word[w] & 0xFFFF0000u) : (word[w] & 0xFFFFu) | got << 16;
+    }
+  }
+  if (pos < t0 || pos >= t1) return;
+  const __half2* par = reinterpret_cast<const __half2*>(unit + (is_v ? vp_base(D, NG) : kp_base(D))) + t * NG;
+  T* dst = (is_v ? vo : ko) + ((layer * L.n_kv + h) * (int64_t)(t1 - t0) + (pos - t0)) * D + 8 * c;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const __half2 sz = par[w / WPG];
+    const float s = __low2float(sz), z = __high2float(sz);
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      // 2^23 + code as a float's bits; the subtraction leaves code - 8 exactly
+      const float q = __uint_as_float(0x4B000000u | ((word[w] >> (4 * (e ^ 1))) & 15u)) - 8388616.0f;
+      x[e] = fmaf(q, s, z);
+    }
+    store8(dst + 32 * w, x);
+  }
+}
+
+// ---- page copies ------------------------------------------------------------
+
+constexpr int kPairs = 1024;  // page pairs of a launch, by value: no staging buffer to keep alive
+constexpr int kCopyBytes = 16384;
+
+struct CopyPairs {
+  int32_t src[kPairs], dst[kPairs];
+};
+
+template <typename V>
+__global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CellPtrsMut pools,
+                                                         const __grid_constant__ CopyPairs pairs, int64_t page_bytes,
+                                                         int parts) {
+  const int pair = blockIdx.x / parts, part = blockIdx.x % parts;
+  uint8_t* base = static_cast<uint8_t*>(pools.p[blockIdx.y]);
+  const int64_t off = (int64_t)part * kCopyBytes;
+  const int n = (int)((page_bytes - off < kCopyBytes ? page_bytes - off : kCopyBytes) / (int64_t)sizeof(V));
+  const V* src = reinterpret_cast<const V*>(base + pairs.src[pair] * page_bytes + off);
+  V* dst = reinterpret_cast<V*>(base + pairs.dst[pair] * page_bytes + off);
+  for (int i = threadIdx.x; i < n; i += 4 * 256) {
+    V v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j * 256 < n) v[j] = src[i + j * 256];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j * 256 < n) dst[i + j * 256] = v[j];
+  }
+}
+
+}  // namespace
+
+int check_layout(const kvc_kv4_layout* l, const char* what) {
+  const std::string w(what);
+  if (!l || !l->table) return fail(KVC_ERR_ARG, w + ": NULL layout or table");
+  if (l->head_dim != 64 && l->head_dim != 128) return fail(KVC_ERR_SHAPE, w + ": head_dim must be 64 or 128");
+  if (l->page_size < 16 || l->page_size > 256 || (l->page_size & (l->page_size - 1)))
+    return fail(KVC_ERR_SHAPE, w + ": page_size must be 16, 32, 64, 128 or 256");
+  const int g = l->group_size;
+  if ((g != 32 && g != 64 && g != 128) || l->head_dim % g)
+    return fail(KVC_ERR_SHAPE, w + ": group_size must be 32, 64 or 128 and divide head_dim");
+  if (l->n_kv < 1 || l->n_pages < 1 || l->n_pages > INT32_MAX || l->table_stride < 1)
+    return fail(KVC_ERR_SHAPE, w + ": bad layout sizes");
+  return KVC_OK;
+}
+
+Layout to_layout(const kvc_kv4_layout* l) {
+  int log2 = 4;
+  while ((1 << log2) < l->page_size) ++log2;
+  return Layout{l->n_pages, l->n_kv, log2, l->head_dim / l->group_size, l->table, l->table_stride};
+}
+
+}  // namespace kv4
+}  // namespace kvc
+
+using namespace kvc;
+using namespace kvc::kv4;
+
+extern "C" int64_t kvc_kv4_page_bytes(int n_kv, int head_dim, int page_size, int group_size) {
+  if (n_kv < 1 || head_dim < 1 || page_size < 16 || group_size < 1) return 0;
+  return (int64_t)n_kv * (page_size / kUnit) * unit_bytes(head_dim, head_dim / group_size);
+}
+
+extern "C" int kvc_kv4_write(const kvc_kv4_layout* layout, const kvc_kv4_step* step, void* pool, const void* k,
+                             const void* v, int dtype, int64_t seq_stride, int64_t token_stride, int64_t head_stride,
+                             int packed, void* stream) {
+  if (int rc = check_layout(layout, "kvc_kv4_write")) return rc;
+  if (!step || !pool) return fail(KVC_ERR_ARG, "kvc_kv4_write: NULL pointer");
+  if (!dtype_ok(dtype)) return fail(KVC_ERR_DTYPE, "kvc_kv4_write: bad dtype");
+  if (!aligned16(pool)) return fail(KVC_ERR_ALIGN, "kvc_kv4_write: pool not 16-byte aligned");
+  if (step->n_halves < 0 || step->n_seqs < 0) return fail(KVC_ERR_SHAPE, "kvc_kv4_write: negative size");
+  if (step->n_halves == 0) return KVC_OK;
+  if (!k || !v) return fail(KVC_ERR_ARG, "kvc_kv4_write: NULL pointer");
+  const int64_t warps = step->n_halves * layout->n_kv * 2, blocks = ceil_div(warps, 4);
+  if (blocks > INT32_MAX) return fail(KVC_ERR_SHAPE, "kvc_kv4_write: too many tokens in one call");
+  const int64_t e = (int64_t)dtype_size(dtype);
+  const bool vec = aligned16(k) && aligned16(v) && (seq_stride * e) % 16 == 0 && (token_stride * e) % 16 == 0 &&
+                   (head_stride * e) % 16 == 0;
+  const KvIn in{k, v, seq_stride, token_stride, head_stride, packed, vec};
+  const Step s{step->n_seqs, step->rows, step->kv_len, step->q_start};
+  const Layout L = to_layout(layout);
+#define KVC_F(D, WPG)                                                                                         \
+  KVC_DISPATCH_DTYPE(dtype, T,                                                                                \
+                     (kv4_write_kernel<T, D, WPG><<<(unsigned)blocks, 128, 0, static_cast<cudaStream_t>(stream)>>>( \
+                         L, s, static_cast<uint8_t*>(pool), in, step->n_halves, step->half_seq, step->half_start)))
+  KVC_KV4_DISPATCH(layout, KVC_F);
+#undef KVC_F
+  return check_launch("kv4_write_kernel");
+}
+
+extern "C" int kvc_kv4_read(const kvc_kv4_layout* layout, const void* pool, int64_t layer_bytes, int n_layers, int row,
+                            int64_t t0, int64_t t1, int dtype, void* k_out, void* v_out, void* stream) {
+  if (int rc = check_layout(layout, "kvc_kv4_read")) return rc;
+  if (!pool || !k_out || !v_out) return fail(KVC_ERR_ARG, "kvc_kv4_read: NULL pointer");
+  if (!dtype_ok(dtype)) return fail(KVC_ERR_DTYPE, "kvc_kv4_read: bad dtype");
+  if (!aligned16(pool) || !aligned16(k_out) || !aligned16(v_out) || layer_bytes % 16)
+    return fail(KVC_ERR_ALIGN, "kvc_kv4_read: pool, layers and outputs must be 16-byte aligned");
+  if (n_layers < 0 || row < 0 || t0 < 0 || t1 < t0 || t1 > layout->table_stride * layout->page_size || t1 > INT32_MAX)
+    return fail(KVC_ERR_SHAPE, "kvc_kv4_read: bad layers or token range");
+  if (t0 == t1 || n_layers == 0) return KVC_OK;
+  const int64_t halves = (t1 - 1) / 8 - t0 / 8 + 1, warps = halves * layout->n_kv * 2 * n_layers;
+  const int64_t blocks = ceil_div(warps, 4);
+  if (blocks > INT32_MAX) return fail(KVC_ERR_SHAPE, "kvc_kv4_read: too many tokens in one call");
+  const Layout L = to_layout(layout);
+#define KVC_F(D, WPG)                                                                                        \
+  KVC_DISPATCH_DTYPE(dtype, T,                                                                               \
+                     (kv4_read_kernel<T, D, WPG><<<(unsigned)blocks, 128, 0, static_cast<cudaStream_t>(stream)>>>( \
+                         L, static_cast<const uint8_t*>(pool), layer_bytes, row, (int)t0, (int)t1, halves, warps,  \
+                         static_cast<T*>(k_out), static_cast<T*>(v_out))))
+  KVC_KV4_DISPATCH(layout, KVC_F);
+#undef KVC_F
+  return check_launch("kv4_read_kernel");
+}
+
+extern "C" int kvc_copy_pages(int n_pools, void* const* pools, int64_t n_pages, int64_t page_bytes, int64_t n_pairs,
+                              const int32_t* src, const int32_t* dst, void* stream) {
+  if (n_pools < 0 || n_pools > KVC_MAX_CELLS || n_pages < 0 || page_bytes < 0 || n_pairs < 0)
+    return fail(KVC_ERR_SHAPE, "kvc_copy_pages: bad sizes");
+  if (n_pools == 0 || n_pairs == 0 || page_bytes == 0) return KVC_OK;
+  if (!pools || !src || !dst) return fail(KVC_ERR_ARG, "kvc_copy_pages: NULL pointer");
+  CellPtrsMut p{};
+  bool a16 = page_bytes % 16 == 0, a4 = page_bytes % 4 == 0;
+  for (int i = 0; i < n_pools; ++i) {
+    if (!pools[i]) return fail(KVC_ERR_ARG, "kvc_copy_pages: NULL pool");
+    p.p[i] = pools[i];
+    a16 = a16 && aligned16(pools[i]);
+    a4 = a4 && (reinterpret_cast<uintptr_t>(pools[i]) & 3u) == 0;
+  }
+  for (int64_t i = 0; i < n_pairs; ++i)
+    if (src[i] < 0 || src[i] >= n_pages || dst[i] < 0 || dst[i] >= n_pages)
+      return fail(KVC_ERR_SHAPE, "kvc_copy_pages: page out of range");
+  const int64_t parts = ceil_div(page_bytes, kCopyBytes);
+  if (parts > INT32_MAX / kPairs) return fail(KVC_ERR_SHAPE, "kvc_copy_pages: page too large");
+  for (int64_t at = 0; at < n_pairs; at += kPairs) {
+    const int n = (int)std::min<int64_t>(kPairs, n_pairs - at);
+    CopyPairs pr;
+    memcpy(pr.src, src + at, n * sizeof(int32_t));
+    memcpy(pr.dst, dst + at, n * sizeof(int32_t));
+    const dim3 grid((unsigned)(n * parts), (unsigned)n_pools);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a16) copy_pages_kernel<uint4><<<grid, 256, 0, st>>>(p, pr, page_bytes, (int)parts);
+    else if (a4) copy_pages_kernel<uint32_t><<<grid, 256, 0, st>>>(p, pr, page_bytes, (int)parts);
+    else copy_pages_kernel<uint8_t><<<grid, 256, 0, st>>>(p, pr, page_bytes, (int)parts);
+    if (int rc = check_launch("copy_pages_kernel")) return rc;
+  }
+  return KVC_OK;
+}

@@ -43,6 +43,8 @@ int tc_decompress_launch(int n_cells, const uint8_t* const* codes, const float* 
 void tc_reuse_tucker_rows(bool allow);
 int tc_read_device_error(int* out);
 int tc_gram_read_device_error(int* out);
+int kv4_read_device_error(int* out);
+int kv4_attend_read_device_error(int* out);
 
 // 0: tensor cores when eligible (the quantise pass in its fp16 two-term
 // mode where it applies), 1: SIMT kernels only, 2: as 0 with the stats pass
@@ -530,6 +532,10 @@ extern "C" int kvc_device_error(int* code) {
   int rc = tc_read_device_error(&a);
   if (rc) return rc;
   if ((rc = tc_gram_read_device_error(&b))) return rc;
+  a = a ? a : b;
+  if ((rc = kv4_read_device_error(&b))) return rc;
+  a = a ? a : b;
+  if ((rc = kv4_attend_read_device_error(&b))) return rc;
   *code = a ? a : b;
   return KVC_OK;
 }

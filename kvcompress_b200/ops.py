@@ -23,10 +23,15 @@ __all__ = [
     "cells",
     "compress",
     "cast",
+    "copy_pages",
     "core",
     "decompress",
     "decompress_noalloc",
     "gram",
+    "kv4_attend",
+    "kv4_page_bytes",
+    "kv4_read",
+    "kv4_write",
     "project_feature",
     "residual_quant",
     "residual_stats",
@@ -665,3 +670,148 @@ def cast(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
         check(lib().kvc_cast(x.numel(), x.data_ptr(), _code(x.dtype), out.data_ptr(), _code(dtype),
                              _stream()), "kvc_cast")
     return out
+
+
+# ---- paged 4-bit cache -----------------------------------------------------
+
+
+def kv4_page_bytes(n_kv: int, head_dim: int, page_size: int, group_size: int) -> int:
+    """Bytes of one page of one layer of a 4-bit cache."""
+    return int(lib().kvc_kv4_page_bytes(n_kv, head_dim, page_size, group_size))
+
+
+def _kv4_code(dtype: torch.dtype) -> int:
+    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f"unsupported dtype {dtype}: float32, float16 or bfloat16")
+    return DTYPE_CODE[dtype]
+
+
+def _kv4_tokens(x: torch.Tensor, step, what: str, n_heads: int | None, layout, device) -> tuple[int, int, int, int]:
+    """Check a step's per-token tensor; (sequence, token, head) strides and whether it is packed."""
+    if not x.is_cuda:
+        raise RuntimeError(f"{what}: kvcompress_b200 runs on CUDA tensors only (got {x.device})")
+    if x.device != device:
+        raise ValueError(f"{what}: tensor on {x.device}, cache on {device}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what}: there is no gradient through a cache in 4 bits; use torch.no_grad() or detach()")
+    d, shape, st = layout.head_dim, x.shape, x.stride()
+    if x.dim() == 3:
+        if shape[0] != step.n_tokens or shape[2] != d or (n_heads is not None and shape[1] != n_heads):
+            raise ValueError(f"{what}: expected ({step.n_tokens}, {n_heads or 'heads'}, {d}), got {tuple(shape)}")
+        out = (0, st[0], st[1], 1)
+    elif x.dim() == 4:
+        t = step.max_new
+        if (shape[0] != step.n_seqs or shape[2] != t or t * step.n_seqs != step.n_tokens or shape[3] != d
+                or (n_heads is not None and shape[1] != n_heads)):
+            raise ValueError(f"{what}: expected ({step.n_seqs}, {n_heads or 'heads'}, T, {d}) with T tokens of every "
+                             f"sequence, got {tuple(shape)}")
+        out = (st[0], st[2], st[1], 0)
+    else:
+        raise ValueError(f"{what}: expected 3 or 4 dimensions, got {x.dim()}")
+    if st[-1] != 1 and x.numel():
+        raise ValueError(f"{what}: features must be contiguous")
+    return out
+
+
+def kv4_write(layout, step, pool: int, key: torch.Tensor, value: torch.Tensor, device: torch.device) -> None:
+    """Quantise a step's K and V into the pages of the layer at address ``pool`` (``kvc_kv4_write``)."""
+    if key.shape != value.shape or key.dtype != value.dtype:
+        raise ValueError(f"kv4_write: K {tuple(key.shape)} {key.dtype} and V {tuple(value.shape)} {value.dtype} differ")
+    code = _kv4_code(key.dtype)
+    if key.stride() != value.stride():
+        key, value = key.contiguous(), value.contiguous()
+    strides = _kv4_tokens(key, step, "kv4_write", layout.n_kv, layout, device)
+    _kv4_tokens(value, step, "kv4_write", layout.n_kv, layout, device)
+    with _on(device), _Stage("kv4_write", 1, 2 * key.numel() * key.element_size()):
+        check(lib().kvc_kv4_write(layout, step, pool, key.data_ptr(), value.data_ptr(), code, *strides, _stream()),
+              "kvc_kv4_write")
+
+
+def kv4_attend(layout, step, split, pool: int, query: torch.Tensor, *, causal: bool, scale: float,
+               device: torch.device) -> torch.Tensor:
+    """Attention of a step's queries over the pages of the layer at address
+    ``pool`` (``kvc_kv4_attend``).  ``split(copies)`` gives the split of the cached
+    tokens when each item is worked on by ``copies`` CTAs."""
+    code = _kv4_code(query.dtype)
+    qs = _kv4_tokens(query, step, "kv4_attend", None, layout, device)
+    n_q = int(query.shape[1])
+    if n_q % layout.n_kv or n_q == 0:
+        raise ValueError(f"kv4_attend: {n_q} query heads are no multiple of {layout.n_kv} KV heads")
+    out = torch.empty(query.shape, dtype=query.dtype, device=device)
+    if step.n_tokens == 0:
+        return out
+    st = out.stride()
+    os_ = (0, st[0], st[1]) if qs[3] else (st[0], st[2], st[1])
+    sp = split(layout.n_kv)
+    L = lib()
+    ws_n = L.kvc_kv4_attend_workspace_bytes(layout, step, sp, n_q)
+    # a buffer of this call's own: a captured graph keeps the one it was captured
+    # with, and no other graph or stream writes to it
+    ws = torch.empty(ws_n, dtype=torch.uint8, device=device) if ws_n else None
+    with _on(device), _Stage("kv4_attend", 1, 2 * query.numel() * query.element_size()):
+        check(L.kvc_kv4_attend(layout, step, sp, pool, n_q, query.data_ptr(), *qs[:3], out.data_ptr(), *os_, qs[3],
+                               code, int(causal), scale, ws.data_ptr() if ws_n else None, ws_n, _stream()),
+              "kvc_kv4_attend")
+    return out
+
+
+def kv4_read(layout, pool: int, layer_bytes: int, n_layers: int, row: int, t0: int, t1: int, dtype: torch.dtype,
+             device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
+    """Dense K and V, ``(n_layers, n_kv, t1 - t0, d)``, of table row ``row`` (``kvc_kv4_read``)."""
+    code = _kv4_code(dtype)
+    shape = (n_layers, layout.n_kv, t1 - t0, layout.head_dim)
+    k = torch.empty(shape, dtype=dtype, device=device)
+    v = torch.empty(shape, dtype=dtype, device=device)
+    if k.numel():
+        with _on(device), _Stage("kv4_read", 1, 2 * k.numel() * k.element_size()):
+            check(lib().kvc_kv4_read(layout, pool, layer_bytes, n_layers, row, t0, t1, code, k.data_ptr(),
+                                     v.data_ptr(), _stream()), "kvc_kv4_read")
+    return k, v
+
+
+def copy_pages(pools, src: Sequence[int], dst: Sequence[int]) -> None:
+    """Copy page ``src[i]`` to page ``dst[i]`` in every pool, in place.
+
+    ``pools``: a list of same-shape contiguous CUDA tensors whose first dimension
+    is the page (a K or V cache of each layer, say), of any element type, or one
+    tensor whose first dimension indexes the pools.  ``src`` / ``dst``: page numbers
+    on the host.  A page may be copied to several places; no page may be written
+    twice, or be read and written (``ValueError``)."""
+    if isinstance(pools, torch.Tensor):
+        if pools.dim() < 2:
+            raise ValueError("copy_pages: expected (pools, pages, ...)")
+        if not pools.is_cuda:
+            raise RuntimeError(f"copy_pages: kvcompress_b200 runs on CUDA tensors only (got {pools.device})")
+        if not pools.is_contiguous():
+            raise ValueError("copy_pages: pools must be contiguous")
+        n, step = int(pools.shape[0]), pools.stride(0) * pools.element_size()
+        ptrs, first = [pools.data_ptr() + i * step for i in range(n)], pools
+        n_pages, elems = int(pools.shape[1]), pools[0].numel() if n else 0
+    else:
+        xs = list(pools)
+        for i in range(0, len(xs), KVC.MAX_CELLS):
+            _cells(xs[i:i + KVC.MAX_CELLS], "copy_pages")
+            if xs[i].dim() < 1 or xs[i].shape != xs[0].shape or xs[i].dtype != xs[0].dtype or xs[i].device != xs[0].device:
+                raise ValueError("copy_pages: pools must share shape, dtype and device")
+        ptrs, first = [x.data_ptr() for x in xs], xs[0] if xs else None
+        n_pages, elems = (int(first.shape[0]), first.numel()) if xs else (0, 0)
+    src, dst = [int(i) for i in src], [int(i) for i in dst]
+    if len(src) != len(dst):
+        raise ValueError(f"copy_pages: {len(src)} sources but {len(dst)} destinations")
+    if not src or not ptrs:
+        return
+    to = set(dst)
+    if len(to) != len(dst):
+        raise ValueError("copy_pages: a page is written twice")
+    if not to.isdisjoint(src):
+        raise ValueError("copy_pages: a page is both read and written")
+    if min(min(src), min(dst)) < 0 or max(max(src), max(dst)) >= n_pages:
+        raise ValueError(f"copy_pages: page out of range (pool of {n_pages})")
+    page_bytes = elems // n_pages * first.element_size()
+    n = len(src)
+    a, b = (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst)
+    with _on(first.device), _Stage("copy_pages", 1, 2 * n * page_bytes * len(ptrs)):
+        for i in range(0, len(ptrs), KVC.MAX_CELLS):
+            part = ptrs[i:i + KVC.MAX_CELLS]
+            check(lib().kvc_copy_pages(len(part), ptr_array(part), n_pages, page_bytes, n, a, b, _stream()),
+                  "kvc_copy_pages")

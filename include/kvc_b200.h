@@ -330,7 +330,8 @@ int kvc_set_kernel_policy(int policy);
  *
  * `table` holds the page ids of each sequence, (rows, table_stride) int32 on
  * the device: token t of row r is in page table[r][t / page_size].  An entry
- * that is no page sets the device error word (401) and is skipped.
+ * that is no page sets the device error word (401); it is never followed, and
+ * what stands for its tokens is not defined.
  */
 typedef struct {
   const int32_t* table;
@@ -355,7 +356,7 @@ typedef struct {
 } kvc_kv4_step;
 
 /*
- * Split of the cached tokens into items of `chunk` tokens (a multiple of 32)
+ * Split of the cached tokens into items of `chunk` tokens (a multiple of 64)
  * for kvc_kv4_attend, device arrays of int32: item j covers tokens
  * [item_first[j], item_first[j] + chunk) of sequence item_seq[j]; the items of
  * sequence i are item_start[i] .. item_start[i + 1] - 1, at least one.
@@ -387,6 +388,9 @@ int kvc_kv4_read(const kvc_kv4_layout* layout, const void* pool, int64_t layer_b
  * over their sequences' pages.  causal: query i of a sequence's n sees the
  * first kv_len - n + 1 + i tokens, otherwise all kv_len.  A query that sees
  * nothing gets zeros.  Strides in elements, as for kvc_kv4_write. */
+/* kvc_kv4_attend_tiles: blocks that work on one item of one KV head, for choosing
+ * the split. */
+int kvc_kv4_attend_tiles(const kvc_kv4_layout* layout, const kvc_kv4_step* step, int n_q, int dtype);
 size_t kvc_kv4_attend_workspace_bytes(const kvc_kv4_layout* layout, const kvc_kv4_step* step,
                                       const kvc_kv4_split* split, int n_q);
 int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* step, const kvc_kv4_split* split,

@@ -85,12 +85,12 @@ def split_chunk(lengths: np.ndarray, copies: int, slots: int) -> int:
             chunk = longest
         else:
             chunk = max(_CHUNK, -(-total * copies // (waves * slots)))
-        chunk = -(-chunk // 32) * 32
+        chunk = -(-chunk // 64) * 64
         while waves and chunk < longest:
             items = int(np.maximum(1, -(-lengths // chunk)).sum()) * copies
             if items <= waves * slots:
                 break
-            chunk += max(32, chunk // 64 // 32 * 32)
+            chunk += max(64, chunk // 64 // 64 * 64)
         items = int(np.maximum(1, -(-lengths // chunk)).sum()) * copies
         c = -(-items // slots) * (min(chunk, longest) + 192)
         if c < cost:

@@ -1,10 +1,43 @@
-// Attention over the pages of the 4-bit KV cache.
+// Attention over the pages of the 4-bit KV cache, for a few queries a KV head.
 //
-// softmax(scale q k^T) v with one pass over the tokens: running maximum m,
-// sum l and accumulator o, rescaled by exp(m_old - m_new) when m grows; all in
-// float32.  A warp per query and head; each lane holds D / 32 features.
+// For a query q and the tokens t of its sequence, o = sum_t p_t v_t / sum_t p_t
+// with p_t = exp(scale q.k_t - m).  K and V are never dequantised: with k_t =
+// z_t + s_t (c_t - 8) in each group,
+//   q.k_t = s_t (q.c_t) + (z_t - 8 s_t) sum(q),
+//   sum_t p_t v_t = sum_t (p_t s'_t) c'_t - 8 sum_t (p_t s'_t) + sum_t p_t z'_t,
+// so the products run on the codes 0..15 themselves, as float16 operands of
+// mma.sync m16n8k16 with float32 accumulators.  A nibble masked out of its word
+// IS a float16: the bits 0x000n are the denormal n 2^-24 and 0x00n0 are
+// n 2^-20, exactly, so a word of 8 codes becomes four operand registers with
+// four ANDs and one shift.  The powers of two are taken out of the queries
+// (every second operand register is met by q / 16) and out of the result.
+//
+// With float32 queries the codes are centred instead (c - 8 as float16 from
+// 1024 + c, one more instruction a register): 8 s sum(q) and 8 s' are large
+// against a logit and an average over many tokens, and the accumulators' own
+// rounding would show (7e-6 of the result instead of 1e-6).
+//
+// What the kernel rounds: queries of 16 bits not at all (float16 with a power
+// of two per row), float32 ones to two float16 terms (22 bits); p s' to
+// float16 under a power of two that keeps its maximum near the top of the
+// range (two terms for float32 queries).  The sum that the constant 8 s'
+// multiplies is formed from the rounded weights, so their rounding acts on
+// c' - 8 and not on c'.
+//
+// A block takes `chunk` tokens of one sequence and KV head and up to 8 NT
+// columns (a column is a query and a head of the KV head's group: all of them
+// read the same codes).  Each warp works alone on runs of 32 (64 for d = 64)
+// tokens through its own ring of bulk copies: tokens are the M rows of both
+// products, so softmax statistics stay in a lane until the end; S^T's
+// accumulators become the second product's B operand by movmatrix.  The
+// running maximum is raised only when a logit exceeds it by 2^4, which is
+// rare, so the loop holds one vote and no reductions.  The warps' partial
+// results are joined through shared memory, the blocks' of a sequence by
+// attend_join_kernel in a fixed order.
+#include <algorithm>
+
 #include "kvc_kv4.cuh"
-#include "kvc_tc.cuh"
+#include "kvc_tma.cuh"
 
 namespace kvc {
 
@@ -21,70 +54,598 @@ int kv4_attend_read_device_error(int* out) {
 namespace kv4 {
 namespace {
 
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRaise = 4.0f;   // log2 units a logit may exceed the running maximum by
+constexpr float kTop = 2048.0f;  // weights p s' are held as (p s' / cap) * kTop <= 2^4 * 2^11 < 65504
+
 struct Qkv {
   const void* q;
   void* out;
-  int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;
+  int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;  // element strides of a sequence, a token, a head
   int packed, dtype, n_q, causal;
   float scale;
 };
 
-// Code 0..15 of feature x of token t (0..15) in a unit.
-template <int D>
-__device__ __forceinline__ int k_code(const uint8_t* unit, int t, int x) {
-  const uint8_t b = unit[k_chunk<D>(t, (x & 31) >> 3) + (x >> 5) * 4 + ((x & 7) >> 1)];
-  return x & 1 ? b & 15 : b >> 4;
-}
-template <int D>
-__device__ __forceinline__ int v_code(const uint8_t* unit, int t, int x) {
-  const int r = (x & 31) >> 2, c = (t & 7) >> 1;
-  const uint8_t b = unit[v_chunk<D>(t >> 3, r * 4 + c) + (x >> 5) * 4 + (t & 1) * 2 + ((x & 3) >> 1)];
-  return x & 1 ? b & 15 : b >> 4;
+struct Split {
+  const int32_t *item_seq, *item_first, *item_start;
+  int chunk, max_items;
+};
+
+// Partial results of an item: o (unnormalised) and (m, l) of each of its
+// sequence's columns, [item][KV head][column].
+struct Partial {
+  float* o;
+  float2* ml;
+  int64_t cols;  // columns of an item and KV head
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-template <int D>
-__global__ void __launch_bounds__(128) attend_simple_kernel(Layout L, Step S, const uint8_t* pool, Qkv a) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31, head = blockIdx.y * 4 + (threadIdx.x >> 5), tok = blockIdx.x;
-  if (head >= a.n_q) return;
-  int b = 0;
-  while (b + 1 < S.n_seqs && S.q_start[b + 1] <= tok) ++b;
-  const int q0 = S.q_start[b], n = S.q_start[b + 1] - q0, j = tok - q0, len = S.kv_len[b];
-  const int seen = a.causal ? len - n + 1 + j : len, h = head / (a.n_q / L.n_kv), gw = 32 * E / L.groups;
-  const int64_t row = a.packed ? tok : j;
-  const int64_t qo = (a.packed ? 0 : b * a.q_sb) + row * a.q_st + head * a.q_sh;
-  float q[E], o[E], m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) q[e] = load_dt(a.q, qo + e * 32 + lane, a.dtype), o[e] = 0.0f;
-  for (int t = 0; t < seen; ++t) {
-    const int64_t page = page_of(L, S.rows[b], t, &tc::g_kvc_device_error);
-    if (page < 0) continue;
-    const uint8_t* unit = pool + unit_off<D>(L, page, h, t);
-    const __half2* kp = reinterpret_cast<const __half2*>(unit + kp_base(D)) + (t & 15) * L.groups;
-    const __half2* vp = reinterpret_cast<const __half2*>(unit + vp_base(D, L.groups)) + (t & 15) * L.groups;
-    float s = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int x = e * 32 + lane;
-      const float2 p = __half22float2(kp[x / gw]);
-      s += q[e] * fmaf((float)(k_code<D>(unit, t & 15, x) - 8), p.x, p.y);
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  uint32_t r;
+  memcpy(&r, &h, 4);
+  return r;
+}
+__device__ __forceinline__ float2 unpack_half2(uint32_t r) {
+  __half2 h;
+  memcpy(&h, &r, 4);
+  return __half22float2(h);
+}
+
+// Two codes of a word as a float16 operand: nibble 0 (lo) or 1 (hi, 16 fold) of
+// each half; plain codes are 2^-24 fold, centred ones c - 8.
+template <bool CENTRED>
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
+  if constexpr (!CENTRED) return w & 0x000F000Fu;
+  uint32_t y;  // 1024 + c less 1032
+  asm("sub.f16x2 %0, %1, %2;" : "=r"(y) : "r"((w & 0x000F000Fu) | 0x64006400u), "r"(0x64086408u));
+  return y;
+}
+template <bool CENTRED>
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
+  if constexpr (!CENTRED) return w & 0x00F000F0u;
+  uint32_t y;  // 1024 + 16 c less 1152
+  asm("sub.f16x2 %0, %1, %2;" : "=r"(y) : "r"((w & 0x00F000F0u) | 0x64006400u), "r"(0x64806480u));
+  return y;
+}
+
+template <int W>
+__device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[W]) {
+  if constexpr (W == 4)
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(addr));
+  else
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+}
+__device__ __forceinline__ float2 lds_half2(uint32_t addr) {
+  uint32_t r;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(addr));
+  return unpack_half2(r);
+}
+
+// The sequence of query token `tok` (the last one whose tokens start at or before it).
+__device__ __forceinline__ int seq_of(const Step& S, int tok) {
+  int lo = 0, hi = S.n_seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (S.q_start[mid] <= tok) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Tokens that query j of n sees of len.
+__device__ __forceinline__ int visible(int causal, int len, int n, int j) {
+  return causal ? max(0, len - n + 1 + j) : len;
+}
+
+// NT tiles of 8 columns; TERMS float16 terms a query and a weight.  The more
+// accumulators a thread holds (D / 4 * NT), the fewer warps an SM has: blocks
+// of 8 warps twice, 4 warps three times or 4 warps twice.
+template <int D, int NT, int TERMS>
+struct Shape {
+  static constexpr int load = NT * TERMS * D / 128 > 0 ? NT * TERMS * D / 128 : 1;
+  static constexpr int warps = load == 1 ? 8 : 4;
+  static constexpr int blocks = load == 2 ? 3 : 2;
+  static constexpr int units = 256 / D;  // of a stage
+  static constexpr int tokens = units * kUnit;
+};
+
+// Units whose logits a thread holds at once (4 NT + 4 NG registers each).
+constexpr int units_at_once(int nt, int ng) { return nt + ng <= 3 ? 2 : 1; }
+
+template <int D, int WPG, int NT, int TERMS>
+struct Smem {
+  using S = Shape<D, NT, TERMS>;
+  static constexpr int NG = D / 32 / WPG;
+  static constexpr int stage = S::units * unit_bytes(D, NG);
+  static constexpr int stages_fit = (227 * 1024 / S::blocks - 2048) / (S::warps * stage);
+  static constexpr int stages = stages_fit > 4 ? 4 : stages_fit;
+  static constexpr int ring = S::warps * stages * stage;
+  static constexpr int o_stride = D + 4;  // floats of a column: the lanes of a store meet different banks
+  static constexpr int join = S::warps * 8 * NT * (o_stride + 2) * 4;
+  static constexpr int bytes = ring > join ? ring : join;
+  static_assert(stages >= 2, "stages");
+};
+
+template <int D, int WPG, int NT, int TERMS>
+__global__ void __launch_bounds__(Shape<D, NT, TERMS>::warps * 32, Shape<D, NT, TERMS>::blocks)
+    attend_kernel(Layout L, Step S, Split P, const uint8_t* __restrict__ pool, Qkv a, Partial part) {
+  using Sh = Shape<D, NT, TERMS>;
+  using Sm = Smem<D, WPG, NT, TERMS>;
+  constexpr int W = D / 32, NG = W / WPG, UB = unit_bytes(D, NG), WARPS = Sh::warps, STAGES = Sm::stages;
+  constexpr int UNITS = Sh::units, TOKENS = Sh::tokens, COLS = 8 * NT, AHEAD = 32 / UNITS;
+  constexpr int SUB = units_at_once(NT, NG);
+  constexpr bool CENTRED = TERMS == 2;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t full[WARPS][STAGES];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int item = blockIdx.x, h = blockIdx.y, col0 = blockIdx.z * COLS;
+  const int b = P.item_seq[item], t_begin = P.item_first[item];
+  const int q0 = S.q_start[b], n = S.q_start[b + 1] - q0, len = S.kv_len[b], group = a.n_q / L.n_kv;
+  const int cols = n * group;
+  if (col0 >= cols) return;
+  const int last = min(col0 + COLS, cols) - 1;
+  const int t_end = min(t_begin + P.chunk, visible(a.causal, len, n, last / group));
+  if (t_begin > 0 && t_begin >= t_end) return;  // nothing of this item is seen: the join knows
+  const int t_free = visible(a.causal, len, n, col0 / group);  // below it no column masks anything
+
+  if (lane == 0)
+    for (int i = 0; i < STAGES; ++i) tc::mbar_init(&full[warp][i], UNITS);
+  tc::mbar_fence_init();
+  __syncwarp();
+
+  // The warp's runs of TOKENS tokens: t_begin + (warp + i WARPS) TOKENS.
+  // Lane (i % AHEAD) * UNITS + u looks up unit u's page of run i and issues its
+  // copy, AHEAD runs at a time, so that no copy waits for a page lookup.
+  const int runs = t_end > t_begin ? (t_end - t_begin + TOKENS - 1) / TOKENS : 0;
+  const int mine = runs > warp ? (runs - warp + WARPS - 1) / WARPS : 0;
+  const uint32_t ring = tc::smem_u32(smem) + warp * STAGES * Sm::stage;
+  int64_t src = -1;
+  bool dead = false;
+  auto look = [&](int i) {  // pages of runs i .. i + AHEAD - 1
+    const int t = t_begin + (warp + (i + lane / UNITS) * WARPS) * TOKENS + (lane % UNITS) * kUnit;
+    src = -1;
+    if (i + lane / UNITS < mine && t < t_end) {
+      const int64_t page = page_of(L, S.rows[b], t, &tc::g_kvc_device_error);
+      // a bad entry reads page 0: its place in the sum is wrong, but in range
+      src = unit_off<D>(L, page < 0 ? 0 : page, h, t);
     }
+  };
+  auto issue = [&](int i) {
+    if (i % AHEAD == 0) look(i);
+    if (lane / UNITS == i % AHEAD) {
+      uint64_t* bar = &full[warp][i % STAGES];
+      if (src >= 0) {
+        tc::mbar_expect_tx(bar, UB);
+        tc::bulk_load(ring + (i % STAGES) * Sm::stage + (lane % UNITS) * UB, pool + src, UB, bar);
+      } else {
+        tc::mbar_arrive(bar);
+      }
+    }
+  };
+  for (int i = 0; i < STAGES && i < mine; ++i) issue(i);
+
+  // ---- queries: lane (r, c) holds features 32 w + 8 c + 0..7 of column r of each tile
+  uint32_t qf[TERMS][NT][W][4];
+  float fac[NT][2], qs[NT][2][NG];
+  int vis[NT][2];
 #pragma unroll
-    for (int i = 16; i; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
-    s *= a.scale;
-    const float m2 = fmaxf(m, s), f = __expf(m - m2), w = __expf(s - m2);
-    l = l * f + w;
-    m = m2;
+  for (int nt = 0; nt < NT; ++nt) {
+    const int col = col0 + nt * 8 + r;
+    float x[W][8], top = 0.0f, sum[NG];
+    const bool valid = col < cols;
+    const int j = col / group;
+    const int64_t at = (a.packed ? (int64_t)(q0 + j) * a.q_st : b * a.q_sb + j * a.q_st) +
+                       (int64_t)(h * group + col % group) * a.q_sh + 8 * c;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int x = e * 32 + lane;
-      const float2 p = __half22float2(vp[x / gw]);
-      o[e] = o[e] * f + w * fmaf((float)(v_code<D>(unit, t & 15, x) - 8), p.x, p.y);
+    for (int g = 0; g < NG; ++g) sum[g] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[w][e] = valid ? load_dt(a.q, at + 32 * w + e, a.dtype) : 0.0f;
+        top = fmaxf(top, fabsf(x[w][e]));
+        sum[w / WPG] += x[w][e];
+      }
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+      for (int g = 0; g < NG; ++g) sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], o);
+    }
+    // 2^k with top 2^k in [2^13, 2^14): 16-bit queries are exact in float16 down
+    // to 2^-28 of the row's maximum.  k is kept to +-100, where the power and
+    // its inverse are normal numbers
+    const int k = min(100, max(-100, 13 + 127 - (int)(__float_as_uint(top) >> 23)));
+    const float up = __uint_as_float((uint32_t)(127 + k) << 23), down = __uint_as_float((uint32_t)(127 - k) << 23);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      // operand register i of word w meets the nibbles i and i + 4, of which
+      // element e lies in nibble e ^ 1; nibbles 1, 3 count 16 fold
+      constexpr int el[4][2] = {{1, 5}, {0, 4}, {3, 7}, {2, 6}};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float f = i & 1 ? up * 0.0625f : up;
+        const float v0 = x[w][el[i][0]] * f, v1 = x[w][el[i][1]] * f;
+        qf[0][nt][w][i] = pack_half2(v0, v1);
+        if constexpr (TERMS == 2) {
+          const float2 hi = unpack_half2(qf[0][nt][w][i]);
+          qf[1][nt][w][i] = pack_half2(v0 - hi.x, v1 - hi.y);
+        }
+      }
+    }
+    const float s2 = a.scale * kLog2e;
+#pragma unroll
+    for (int j2 = 0; j2 < 2; ++j2) {  // what the accumulators' columns 2 c, 2 c + 1 need
+      const int from = (2 * c + j2) * 4;
+      fac[nt][j2] = __shfl_sync(0xffffffffu, down, from) * (CENTRED ? s2 : 16777216.0f * s2);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) qs[nt][j2][g] = __shfl_sync(0xffffffffu, sum[g], from) * s2;
+      const int cj = col0 + nt * 8 + 2 * c + j2;
+      vis[nt][j2] = cj < cols ? visible(a.causal, len, n, cj / group) : 0;
     }
   }
-  const int64_t oo = (a.packed ? 0 : b * a.o_sb) + row * a.o_st + head * a.o_sh;
+
+  float o[NT][2 * W][4], m[NT][2], l[NT][2], z[NT][2][NG];
+  float cap = 0.0f, hold = 0.0f;  // value scales are at most cap; hold = kTop / cap
 #pragma unroll
-  for (int e = 0; e < E; ++e) store_dt(a.out, oo + e * 32 + lane, seen > 0 ? o[e] / l : 0.0f, a.dtype);
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int i = 0; i < 2 * W; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      m[nt][j] = -INFINITY;
+      l[nt][j] = 0.0f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) z[nt][j][g] = 0.0f;
+    }
+  }
+
+  for (int i = 0; i < mine; ++i) {
+    const int stage = i % STAGES, t0 = t_begin + (warp + i * WARPS) * TOKENS;
+    if (!dead && !tc::mbar_wait(&full[warp][stage], (i / STAGES) & 1, 402)) dead = true;
+    dead = __any_sync(0xffffffffu, dead);
+    if (dead) {  // give up: wait (bounded) for the copies still in flight, then return
+      for (int k = i + 1; k < i + STAGES && k < mine; ++k)
+        tc::mbar_wait(&full[warp][k % STAGES], (k / STAGES) & 1, 402);
+      break;
+    }
+    const uint32_t base = ring + stage * Sm::stage;
+    const bool masked = t0 + TOKENS > t_free;
+
+#pragma unroll
+    for (int u0 = 0; u0 < UNITS; u0 += SUB) {
+      const uint32_t sub = base + u0 * UB;
+      const int ts = t0 + u0 * kUnit;
+      // ---- S^T of the run's tokens (rows r and r + 8 of each unit), in log2 units
+      float s[SUB][NT][4], top[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        const uint32_t unit = sub + u * UB;
+        uint32_t k0[W], k1[W];
+        lds_words<W>(unit + k_chunk<D>(r, c), k0);
+        lds_words<W>(unit + k_chunk<D>(r + 8, c), k1);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[u][nt][e] = 0.0f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          float acc[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[nt][e] = 0.0f;
+#pragma unroll
+          for (int w = g * WPG; w < (g + 1) * WPG; ++w) {
+            uint32_t x0 = k0[w], x1 = k1[w];
+#pragma unroll
+            for (int i2 = 0; i2 < 4; i2 += 2) {
+              const uint32_t a0 = codes_lo<CENTRED>(x0), a1 = codes_lo<CENTRED>(x1), a2 = codes_hi<CENTRED>(x0),
+                             a3 = codes_hi<CENTRED>(x1);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int term = 0; term < TERMS; ++term)
+                  mma16816(acc[nt], a0, a1, a2, a3, qf[term][nt][w][i2], qf[term][nt][w][i2 + 1]);
+              x0 >>= 8;
+              x1 >>= 8;
+            }
+          }
+          const float2 p0 = lds_half2(unit + kp_base(D) + (r * NG + g) * 4);
+          const float2 p1 = lds_half2(unit + kp_base(D) + ((r + 8) * NG + g) * 4);
+          const float off0 = CENTRED ? p0.y : fmaf(-8.0f, p0.x, p0.y), off1 = CENTRED ? p1.y : fmaf(-8.0f, p1.x, p1.y);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s[u][nt][e] += fmaf(acc[nt][e] * fac[nt][e & 1], e < 2 ? p0.x : p1.x, qs[nt][e & 1][g] * (e < 2 ? off0 : off1));
+        }
+        if (masked) {
+          const int t = ts + u * kUnit + r;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (t + (e < 2 ? 0 : 8) >= vis[nt][e & 1]) s[u][nt][e] = -INFINITY;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          top[nt][0] = fmaxf(top[nt][0], fmaxf(s[u][nt][0], s[u][nt][2]));
+          top[nt][1] = fmaxf(top[nt][1], fmaxf(s[u][nt][1], s[u][nt][3]));
+        }
+      }
+
+      // ---- value parameters; raise the running maxima where they have to be
+      float2 vp[SUB][2][NG];
+      float vtop = 0.0f;
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int i2 = 0; i2 < 2; ++i2)
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            float2 p = lds_half2(sub + u * UB + vp_base(D, NG) + ((r + 8 * i2) * NG + g) * 4);
+            if (masked && ts + u * kUnit + r + 8 * i2 >= t_end) p = make_float2(0.0f, 0.0f);
+            vp[u][i2][g] = p;
+            vtop = fmaxf(vtop, p.x);
+          }
+      bool raise = vtop > cap;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) raise |= top[nt][0] > m[nt][0] + kRaise || top[nt][1] > m[nt][1] + kRaise;
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int k = 4; k <= 16; k <<= 1) {
+          vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, k));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) top[nt][j] = fmaxf(top[nt][j], __shfl_xor_sync(0xffffffffu, top[nt][j], k));
+        }
+        float fcap = 1.0f;
+        if (vtop > cap) {  // the next power of two above it
+          const float up = 2.0f * __uint_as_float(__float_as_uint(vtop) & 0x7F800000u);
+          fcap = cap / up;
+          cap = up;
+          hold = kTop / up;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float m2 = fmaxf(m[nt][j], top[nt][j]);
+            const float f = m2 == m[nt][j] ? 1.0f : ex2(m[nt][j] - m2);
+            m[nt][j] = m2;
+            l[nt][j] *= f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) z[nt][j][g] *= f;
+#pragma unroll
+            for (int i2 = 0; i2 < 2 * W; ++i2) o[nt][i2][j] *= f * fcap, o[nt][i2][j + 2] *= f * fcap;
+          }
+      }
+
+      // ---- weights and the second product
+      const float centre = cap * (-8.0f / kTop);
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        const uint32_t unit = sub + u * UB;
+        uint32_t v0[W], v1[W];
+        lds_words<W>(unit + v_chunk<D>(0, lane), v0);
+        lds_words<W>(unit + v_chunk<D>(1, lane), v1);
+        uint32_t pf[TERMS][NT][NG][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float ms = m[nt][e & 1];
+            p[e] = ex2(s[u][nt][e] - (ms == -INFINITY ? 0.0f : ms));
+            l[nt][e & 1] += p[e];
+          }
+#pragma unroll
+          for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int i2 = 0; i2 < 2; ++i2) {
+              const float2 vs = vp[u][i2][g];
+              float w0 = p[2 * i2] * (vs.x * hold), w1 = p[2 * i2 + 1] * (vs.x * hold);
+              float y0 = p[2 * i2] * vs.y, y1 = p[2 * i2 + 1] * vs.y;
+              if (masked) {  // a token that a column does not see may hold NaN
+                if (s[u][nt][2 * i2] == -INFINITY) w0 = y0 = 0.0f;
+                if (s[u][nt][2 * i2 + 1] == -INFINITY) w1 = y1 = 0.0f;
+              }
+              const uint32_t hi = pack_half2(w0, w1);
+              const float2 got = unpack_half2(hi);
+              pf[0][nt][g][i2] = transpose8x8(hi);
+              if constexpr (TERMS == 2) pf[1][nt][g][i2] = transpose8x8(pack_half2(w0 - got.x, w1 - got.y));
+              z[nt][0][g] += CENTRED ? y0 : fmaf(got.x, centre, y0);
+              z[nt][1][g] += CENTRED ? y1 : fmaf(got.y, centre, y1);
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          uint32_t y0 = v0[w], y1 = v1[w];
+#pragma unroll
+          for (int i2 = 0; i2 < 2; ++i2) {
+            const uint32_t a0 = codes_lo<CENTRED>(y0), a1 = codes_hi<CENTRED>(y0), a2 = codes_lo<CENTRED>(y1),
+                           a3 = codes_hi<CENTRED>(y1);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int term = 0; term < TERMS; ++term)
+                mma16816(o[nt][2 * w + i2], a0, a1, a2, a3, pf[term][nt][w / WPG][0], pf[term][nt][w / WPG][1]);
+            y0 >>= 8;
+            y1 >>= 8;
+          }
+        }
+      }
+    }
+    __syncwarp();  // every lane has read the stage
+    if (i + STAGES < mine) issue(i + STAGES);
+  }
+
+  // ---- join the warps' results through shared memory
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(smem);
+  float2* sml = reinterpret_cast<float2*>(so + WARPS * COLS * Sm::o_stride);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int col = nt * 8 + 2 * c + j;
+#pragma unroll
+      for (int k = 4; k <= 16; k <<= 1) {
+        l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], k);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) z[nt][j][g] += __shfl_xor_sync(0xffffffffu, z[nt][j][g], k);
+      }
+      const float unhold = cap * (1.0f / kTop), f0 = unhold * (CENTRED ? 1.0f : 16777216.0f), f1 = f0 * 0.0625f;
+      float* dst = so + (warp * COLS + col) * Sm::o_stride + 4 * r;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float zg = z[nt][j][w / WPG];
+        *reinterpret_cast<float4*>(dst + 32 * w) =
+            make_float4(fmaf(o[nt][2 * w][j + 2], f1, zg), fmaf(o[nt][2 * w][j], f0, zg),
+                        fmaf(o[nt][2 * w + 1][j + 2], f1, zg), fmaf(o[nt][2 * w + 1][j], f0, zg));
+      }
+      if (r == 0) sml[warp * COLS + col] = make_float2(m[nt][j], l[nt][j]);
+    }
+  }
+  __syncthreads();
+  const bool alone = P.item_start[b + 1] - P.item_start[b] == 1;
+  for (int i = threadIdx.x; i < COLS * (D / 4); i += WARPS * 32) {
+    const int col = i / (D / 4), x = i % (D / 4) * 4, cj = col0 + col;
+    if (cj >= cols) break;
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sml[w * COLS + col].x);
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float2 ml = sml[w * COLS + col];
+      if (ml.y == 0.0f) continue;  // saw nothing (a sum is at least 1, or NaN)
+      const float f = ex2(ml.x - top);
+      const float4 v = *reinterpret_cast<const float4*>(so + (w * COLS + col) * Sm::o_stride + x);
+      sum = fmaf(ml.y, f, sum);
+      acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y), acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
+    }
+    if (alone) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const int j = cj / group;
+      const int64_t at = (a.packed ? (int64_t)(q0 + j) * a.o_st : b * a.o_sb + j * a.o_st) +
+                         (int64_t)(h * group + cj % group) * a.o_sh + x;
+      store_dt(a.out, at, acc.x * inv, a.dtype);
+      store_dt(a.out, at + 1, acc.y * inv, a.dtype);
+      store_dt(a.out, at + 2, acc.z * inv, a.dtype);
+      store_dt(a.out, at + 3, acc.w * inv, a.dtype);
+    } else {
+      const int64_t at = ((int64_t)item * L.n_kv + h) * part.cols + cj;
+      *reinterpret_cast<float4*>(part.o + at * D + x) = acc;
+      if (x == 0) part.ml[at] = make_float2(top, sum);
+    }
+  }
+}
+
+// Joins the items of the sequences that have several: a warp per query and
+// head, items in their order.
+template <int D>
+__global__ void __launch_bounds__(128) attend_join_kernel(Layout L, Step S, Split P, Qkv a, Partial part) {
+  constexpr int E = D / 32;
+  const int lane = threadIdx.x & 31, tok = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5);
+  if (head >= a.n_q) return;
+  const int b = seq_of(S, tok), i0 = P.item_start[b], i1 = P.item_start[b + 1];
+  if (i1 - i0 == 1) return;
+  const int q0 = S.q_start[b], n = S.q_start[b + 1] - q0, j = tok - q0, group = a.n_q / L.n_kv;
+  const int vis = visible(a.causal, S.kv_len[b], n, j), h = head / group;
+  // items past what the query sees hold nothing of it; the first always holds something
+  const int items = max(1, min(i1 - i0, (vis + P.chunk - 1) / P.chunk));
+  const int64_t at0 = ((int64_t)i0 * L.n_kv + h) * part.cols + j * group + head % group, step = L.n_kv * part.cols;
+  float top = -INFINITY;
+  for (int i = lane; i < items; i += 32) top = fmaxf(top, part.ml[at0 + i * step].x);
+#pragma unroll
+  for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+  float acc[E], sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < items; ++i) {
+    const float2 ml = part.ml[at0 + i * step];
+    const float* o = part.o + (at0 + i * step) * D + lane * E;
+    float v[E];
+    if constexpr (E == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(o);
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else {
+      const float2 x = *reinterpret_cast<const float2*>(o);
+      v[0] = x.x, v[1] = x.y;
+    }
+    const bool none = ml.y == 0.0f;
+    const float f = none ? 0.0f : ex2(ml.x - top);
+    sum = fmaf(ml.y, f, sum);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = none ? acc[e] : fmaf(v[e], f, acc[e]);
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const int64_t at = (a.packed ? (int64_t)tok * a.o_st : b * a.o_sb + j * a.o_st) + (int64_t)head * a.o_sh + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) store_dt(a.out, at + e, acc[e] * inv, a.dtype);
+}
+
+// Tiles of 8 columns a block takes: as many as there are, up to what the
+// registers hold (4 with one float16 term and one group a head, else 2).
+int tiles_of(int cols, int terms, int groups) { return cols <= 8 ? 1 : cols <= 16 || terms == 2 || groups > 1 ? 2 : 4; }
+
+template <int D, int WPG, int NT, int TERMS>
+int launch(const Layout& L, const Step& S, const Split& P, const void* pool, const Qkv& a, const Partial& part,
+           int64_t n_items, int col_tiles, cudaStream_t st) {
+  using Sm = Smem<D, WPG, NT, TERMS>;
+  auto kernel = attend_kernel<D, WPG, NT, TERMS>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sm::bytes);
+  if (e != cudaSuccess) return fail(KVC_ERR_LAUNCH, std::string("attend_kernel: ") + cudaGetErrorString(e));
+  const dim3 grid((unsigned)n_items, (unsigned)L.n_kv, (unsigned)col_tiles);
+  kernel<<<grid, Shape<D, NT, TERMS>::warps * 32, Sm::bytes, st>>>(L, S, P, static_cast<const uint8_t*>(pool), a, part);
+  return check_launch("attend_kernel");
+}
+
+template <int D, int WPG>
+int launch_tiles(const Layout& L, const Step& S, const Split& P, const void* pool, const Qkv& a, const Partial& part,
+                 int64_t n_items, int cols, cudaStream_t st) {
+  const int terms = a.dtype == KVC_F32 ? 2 : 1, nt = tiles_of(cols, terms, D / 32 / WPG);
+  const int tiles = (int)ceil_div(cols, 8 * nt);
+  if (tiles > 65535 || L.n_kv > 65535) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: too many queries or KV heads");
+  if (terms == 2)
+    return nt == 1 ? launch<D, WPG, 1, 2>(L, S, P, pool, a, part, n_items, tiles, st)
+                   : launch<D, WPG, 2, 2>(L, S, P, pool, a, part, n_items, tiles, st);
+  if (nt == 1) return launch<D, WPG, 1, 1>(L, S, P, pool, a, part, n_items, tiles, st);
+  if constexpr (D / 32 == WPG) {
+    if (nt == 4) return launch<D, WPG, 4, 1>(L, S, P, pool, a, part, n_items, tiles, st);
+  }
+  return launch<D, WPG, 2, 1>(L, S, P, pool, a, part, n_items, tiles, st);
 }
 
 }  // namespace
@@ -94,8 +655,17 @@ __global__ void __launch_bounds__(128) attend_simple_kernel(Layout L, Step S, co
 using namespace kvc;
 using namespace kvc::kv4;
 
-extern "C" size_t kvc_kv4_attend_workspace_bytes(const kvc_kv4_layout*, const kvc_kv4_step*, const kvc_kv4_split*, int) {
-  return 0;
+extern "C" int kvc_kv4_attend_tiles(const kvc_kv4_layout* layout, const kvc_kv4_step* step, int n_q, int dtype) {
+  if (!layout || !step || layout->n_kv < 1 || layout->group_size < 1 || n_q < 1) return 0;
+  const int64_t cols = (int64_t)step->max_new * (n_q / layout->n_kv);
+  if (cols <= 0 || cols > INT32_MAX) return 0;
+  return (int)ceil_div(cols, 8 * tiles_of((int)cols, dtype == KVC_F32 ? 2 : 1, layout->head_dim / layout->group_size));
+}
+
+extern "C" size_t kvc_kv4_attend_workspace_bytes(const kvc_kv4_layout* layout, const kvc_kv4_step* step,
+                                                 const kvc_kv4_split* split, int n_q) {
+  if (!layout || !step || !split || split->max_items <= 1) return 0;
+  return (size_t)split->n_items * n_q * step->max_new * (layout->head_dim + 2) * sizeof(float);
 }
 
 extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* step, const kvc_kv4_split* split,
@@ -108,15 +678,30 @@ extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* 
   if (!dtype_ok(dtype)) return fail(KVC_ERR_DTYPE, "kvc_kv4_attend: bad dtype");
   if (!aligned16(pool)) return fail(KVC_ERR_ALIGN, "kvc_kv4_attend: pool not 16-byte aligned");
   if (n_q < 1 || n_q % layout->n_kv) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: n_q must be a multiple of n_kv");
-  if (step->n_tokens == 0) return KVC_OK;
+  if (step->n_tokens == 0 || split->n_items == 0) return KVC_OK;
+  if (step->n_tokens < 0 || step->n_tokens > INT32_MAX || step->max_new < 1 || split->n_items < 0 ||
+      split->n_items > INT32_MAX || split->chunk < 64 || split->chunk % 64)
+    return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: bad step or split sizes");
+  const int64_t cols = (int64_t)step->max_new * (n_q / layout->n_kv);
+  if (cols > INT32_MAX / 2) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: too many queries");
+  const size_t need = kvc_kv4_attend_workspace_bytes(layout, step, split, n_q);
+  if (need && (!workspace || ws_bytes < need || !aligned16(workspace)))
+    return fail(KVC_ERR_WORKSPACE, "kvc_kv4_attend: workspace too small or not 16-byte aligned");
   const Step s{step->n_seqs, step->rows, step->kv_len, step->q_start};
+  const Split p{split->item_seq, split->item_first, split->item_start, split->chunk, split->max_items};
   const Qkv a{q, out, q_seq_stride, q_token_stride, q_head_stride, o_seq_stride, o_token_stride, o_head_stride,
               packed, dtype, n_q, causal, scale};
-  const dim3 grid((unsigned)step->n_tokens, (unsigned)ceil_div(n_q, 4));
+  Partial part{static_cast<float*>(workspace), nullptr, cols};
+  if (need) part.ml = reinterpret_cast<float2*>(part.o + (size_t)split->n_items * n_q * step->max_new * layout->head_dim);
   const Layout L = to_layout(layout);
-  if (layout->head_dim == 64)
-    attend_simple_kernel<64><<<grid, 128, 0, static_cast<cudaStream_t>(stream)>>>(L, s, static_cast<const uint8_t*>(pool), a);
-  else
-    attend_simple_kernel<128><<<grid, 128, 0, static_cast<cudaStream_t>(stream)>>>(L, s, static_cast<const uint8_t*>(pool), a);
-  return check_launch("attend_simple_kernel");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int rc = KVC_OK;
+#define KVC_F(D, WPG) rc = launch_tiles<D, WPG>(L, s, p, pool, a, part, split->n_items, (int)cols, st)
+  KVC_KV4_DISPATCH(layout, KVC_F);
+#undef KVC_F
+  if (rc || split->max_items <= 1) return rc;
+  const dim3 grid((unsigned)step->n_tokens, (unsigned)ceil_div(n_q, 4));
+  if (layout->head_dim == 64) attend_join_kernel<64><<<grid, 128, 0, st>>>(L, s, p, a, part);
+  else attend_join_kernel<128><<<grid, 128, 0, st>>>(L, s, p, a, part);
+  return check_launch("attend_join_kernel");
 }

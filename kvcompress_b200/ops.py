@@ -742,8 +742,8 @@ def kv4_attend(layout, step, split, pool: int, query: torch.Tensor, *, causal: b
         return out
     st = out.stride()
     os_ = (0, st[0], st[1]) if qs[3] else (st[0], st[2], st[1])
-    sp = split(layout.n_kv)
     L = lib()
+    sp = split(layout.n_kv * L.kvc_kv4_attend_tiles(layout, step, n_q, code))
     ws_n = L.kvc_kv4_attend_workspace_bytes(layout, step, sp, n_q)
     # a buffer of this call's own: a captured graph keeps the one it was captured
     # with, and no other graph or stream writes to it

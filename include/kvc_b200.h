@@ -357,13 +357,13 @@ typedef struct {
 
 /*
  * Split of the cached tokens into items of `chunk` tokens (a multiple of 64)
- * for kvc_kv4_attend, device arrays of int32: item j covers tokens
- * [item_first[j], item_first[j] + chunk) of sequence item_seq[j]; the items of
- * sequence i are item_start[i] .. item_start[i + 1] - 1, at least one.
- * max_items: most items of one sequence.
+ * for kvc_kv4_attend, device arrays of int32: items[4 j ..] (16-byte aligned) are
+ * item j's sequence i, its first token, rows[i] and kv_len[i]; it covers `chunk`
+ * tokens from the first one on.  The items of sequence i are item_start[i] ..
+ * item_start[i + 1] - 1, at least one.  max_items: most items of one sequence.
  */
 typedef struct {
-  const int32_t *item_seq, *item_first, *item_start;
+  const int32_t *items, *item_start;
   int64_t n_items;
   int32_t chunk, max_items;
 } kvc_kv4_split;

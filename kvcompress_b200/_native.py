@@ -58,7 +58,7 @@ class Kv4Step(ctypes.Structure):
 class Kv4Split(ctypes.Structure):
     """``kvc_kv4_split``."""
 
-    _fields_ = [("item_seq", P), ("item_first", P), ("item_start", P), ("n_items", I64),
+    _fields_ = [("items", P), ("item_start", P), ("n_items", I64),
                 ("chunk", ctypes.c_int32), ("max_items", ctypes.c_int32)]
 
 

@@ -229,10 +229,10 @@ class PagedKVCache:
             items = np.maximum(1, -(-lengths // chunk))
             start = _prefix(items)
             seq = np.repeat(np.arange(len(step.seqs)), items)
-            first = (np.arange(int(start[-1])) - start[seq]) * chunk
-            buf, at = _upload((seq, first, start), self.device)
-            got = step.splits[copies] = (Kv4Split(at[0], at[1], at[2], int(start[-1]), chunk,
-                                                  int(items.max(initial=1))), buf)
+            rows = np.array([self.pages.row(s) for s in step.seqs], dtype=np.int64)
+            table = np.stack((seq, (np.arange(int(start[-1])) - start[seq]) * chunk, rows[seq], lengths[seq]), 1)
+            buf, at = _upload((table.reshape(-1), start), self.device)
+            got = step.splits[copies] = (Kv4Split(at[0], at[1], int(start[-1]), chunk, int(items.max(initial=1))), buf)
         return got[0]
 
     def _check(self, what: str, layer: int, step: CacheStep) -> int:

@@ -35,6 +35,7 @@
 // results are joined through shared memory, the blocks' of a sequence by
 // attend_join_kernel in a fixed order.
 #include <algorithm>
+#include <type_traits>
 
 #include "kvc_kv4.cuh"
 #include "kvc_tma.cuh"
@@ -67,7 +68,8 @@ struct Qkv {
 };
 
 struct Split {
-  const int32_t *item_seq, *item_first, *item_start;
+  const int4* items;  // sequence, first token, table row, cached tokens
+  const int32_t* item_start;
   int chunk, max_items;
 };
 
@@ -159,51 +161,61 @@ __device__ __forceinline__ int visible(int causal, int len, int n, int j) {
   return causal ? max(0, len - n + 1 + j) : len;
 }
 
-// NT tiles of 8 columns; TERMS float16 terms a query and a weight.  The more
-// accumulators a thread holds (D / 4 * NT), the fewer warps an SM has: blocks
-// of 8 warps twice, 4 warps three times or 4 warps twice.
-template <int D, int NT, int TERMS>
+// Units whose logits a thread holds at once: two give twice the independent
+// products, where the registers are there.
+constexpr int units_at_once(int nt, int ng) { return nt == 1 && ng <= 2 ? 2 : 1; }
+
+// NT tiles of 8 columns; TERMS float16 terms a query and a weight.
+template <int D, int WPG, int NT, int TERMS>
 struct Shape {
-  static constexpr int load = NT * TERMS * D / 128 > 0 ? NT * TERMS * D / 128 : 1;
-  static constexpr int warps = load == 1 ? 8 : 4;
-  static constexpr int blocks = load == 2 ? 3 : 2;
+  static constexpr int NG = D / 32 / WPG;
+  // Registers a thread needs, roughly (accumulators, queries, columns' and
+  // groups' statistics): with up to 128 an SM has 16 warps (2 blocks of 8),
+  // with up to 168 it has 12 (3 of 4), else 8 (2 of 4).
+  static constexpr int regs = 45 + D / 4 * NT + (NT * TERMS == 1 ? D / 8 : 0) + 10 * NT + 8 * NG * NT +
+                              units_at_once(NT, NG) * 4 * (NT + NG) + 35 * (TERMS - 1);
+  static constexpr int warps = regs < 145 ? 8 : 4;
+  static constexpr int blocks = regs < 145 ? 2 : regs < 180 ? 3 : 2;
   static constexpr int units = 256 / D;  // of a stage
   static constexpr int tokens = units * kUnit;
 };
 
-// Units whose logits a thread holds at once (4 NT + 4 NG registers each).
-constexpr int units_at_once(int nt, int ng) { return nt + ng <= 3 ? 2 : 1; }
-
 template <int D, int WPG, int NT, int TERMS>
 struct Smem {
-  using S = Shape<D, NT, TERMS>;
+  using S = Shape<D, WPG, NT, TERMS>;
   static constexpr int NG = D / 32 / WPG;
   static constexpr int stage = S::units * unit_bytes(D, NG);
-  static constexpr int stages_fit = (227 * 1024 / S::blocks - 2048) / (S::warps * stage);
+  // query operands: in registers where they are few, else in shared memory
+  static constexpr bool q_shared = NT * TERMS > 1;
+  static constexpr int q_bytes = q_shared ? TERMS * NT * (D / 32) * 512 : 0;
+  static constexpr int stages_fit = (227 * 1024 / S::blocks - 2048 - q_bytes) / (S::warps * stage);
   static constexpr int stages = stages_fit > 4 ? 4 : stages_fit;
   static constexpr int ring = S::warps * stages * stage;
   static constexpr int o_stride = D + 4;  // floats of a column: the lanes of a store meet different banks
   static constexpr int join = S::warps * 8 * NT * (o_stride + 2) * 4;
-  static constexpr int bytes = ring > join ? ring : join;
+  static constexpr int q_at = ring > join ? ring : join;
+  static constexpr int bytes = q_at + q_bytes;
   static_assert(stages >= 2, "stages");
 };
 
 template <int D, int WPG, int NT, int TERMS>
-__global__ void __launch_bounds__(Shape<D, NT, TERMS>::warps * 32, Shape<D, NT, TERMS>::blocks)
+__global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D, WPG, NT, TERMS>::blocks)
     attend_kernel(Layout L, Step S, Split P, const uint8_t* __restrict__ pool, Qkv a, Partial part) {
-  using Sh = Shape<D, NT, TERMS>;
+  using Sh = Shape<D, WPG, NT, TERMS>;
   using Sm = Smem<D, WPG, NT, TERMS>;
   constexpr int W = D / 32, NG = W / WPG, UB = unit_bytes(D, NG), WARPS = Sh::warps, STAGES = Sm::stages;
   constexpr int UNITS = Sh::units, TOKENS = Sh::tokens, COLS = 8 * NT, AHEAD = 32 / UNITS;
   constexpr int SUB = units_at_once(NT, NG);
   constexpr bool CENTRED = TERMS == 2;
+  constexpr float kCode = CENTRED ? 1.0f : 16777216.0f;  // an operand is a code / kCode
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[WARPS][STAGES];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int item = blockIdx.x, h = blockIdx.y, col0 = blockIdx.z * COLS;
-  const int b = P.item_seq[item], t_begin = P.item_first[item];
-  const int q0 = S.q_start[b], n = S.q_start[b + 1] - q0, len = S.kv_len[b], group = a.n_q / L.n_kv;
+  const int4 it = P.items[item];
+  const int b = it.x, t_begin = it.y, len = it.w;
+  const int q0 = S.q_start[b], n = S.q_start[b + 1] - q0, group = a.n_q / L.n_kv;
   const int cols = n * group;
   if (col0 >= cols) return;
   const int last = min(col0 + COLS, cols) - 1;
@@ -221,34 +233,34 @@ __global__ void __launch_bounds__(Shape<D, NT, TERMS>::warps * 32, Shape<D, NT, 
   // copy, AHEAD runs at a time, so that no copy waits for a page lookup.
   const int runs = t_end > t_begin ? (t_end - t_begin + TOKENS - 1) / TOKENS : 0;
   const int mine = runs > warp ? (runs - warp + WARPS - 1) / WARPS : 0;
-  const uint32_t ring = tc::smem_u32(smem) + warp * STAGES * Sm::stage;
-  int64_t src = -1;
-  bool dead = false;
-  auto look = [&](int i) {  // pages of runs i .. i + AHEAD - 1
-    const int t = t_begin + (warp + (i + lane / UNITS) * WARPS) * TOKENS + (lane % UNITS) * kUnit;
-    src = -1;
-    if (i + lane / UNITS < mine && t < t_end) {
-      const int64_t page = page_of(L, S.rows[b], t, &tc::g_kvc_device_error);
-      // a bad entry reads page 0: its place in the sum is wrong, but in range
-      src = unit_off<D>(L, page < 0 ? 0 : page, h, t);
+  const uint32_t ring = tc::smem_u32(smem) + warp * STAGES * Sm::stage + (lane % UNITS) * UB;
+  const uint8_t* src = nullptr;
+  auto issue = [&](int i, int stage) {
+    if (i % AHEAD == 0) {  // pages of runs i .. i + AHEAD - 1
+      const int t = t_begin + (warp + (i + lane / UNITS) * WARPS) * TOKENS + (lane % UNITS) * kUnit;
+      src = nullptr;
+      if (t < t_end) {
+        const int64_t page = page_of(L, it.z, t, &tc::g_kvc_device_error);
+        // a bad entry reads page 0: its place in the sum is wrong, but in range
+        src = pool + unit_off<D>(L, page < 0 ? 0 : page, h, t);
+      }
     }
-  };
-  auto issue = [&](int i) {
-    if (i % AHEAD == 0) look(i);
     if (lane / UNITS == i % AHEAD) {
-      uint64_t* bar = &full[warp][i % STAGES];
-      if (src >= 0) {
+      uint64_t* bar = &full[warp][stage];
+      if (src) {
         tc::mbar_expect_tx(bar, UB);
-        tc::bulk_load(ring + (i % STAGES) * Sm::stage + (lane % UNITS) * UB, pool + src, UB, bar);
+        tc::bulk_load(ring + stage * Sm::stage, src, UB, bar);
       } else {
         tc::mbar_arrive(bar);
       }
     }
   };
-  for (int i = 0; i < STAGES && i < mine; ++i) issue(i);
+  for (int i = 0; i < STAGES && i < mine; ++i) issue(i, i);
 
   // ---- queries: lane (r, c) holds features 32 w + 8 c + 0..7 of column r of each tile
-  uint32_t qf[TERMS][NT][W][4];
+  constexpr bool QS = Sm::q_shared;
+  uint32_t qf[TERMS][QS ? 1 : NT][W][4];
+  const uint32_t q_at = tc::smem_u32(smem) + Sm::q_at + lane * 16;
   float fac[NT][2], qs[NT][2][NG];
   int vis[NT][2];
 #pragma unroll
@@ -280,35 +292,50 @@ __global__ void __launch_bounds__(Shape<D, NT, TERMS>::warps * 32, Shape<D, NT, 
     // its inverse are normal numbers
     const int k = min(100, max(-100, 13 + 127 - (int)(__float_as_uint(top) >> 23)));
     const float up = __uint_as_float((uint32_t)(127 + k) << 23), down = __uint_as_float((uint32_t)(127 - k) << 23);
+    const float sign = a.scale < 0.0f ? -up : up;  // the logits' factor is kept positive
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       // operand register i of word w meets the nibbles i and i + 4, of which
       // element e lies in nibble e ^ 1; nibbles 1, 3 count 16 fold
       constexpr int el[4][2] = {{1, 5}, {0, 4}, {3, 7}, {2, 6}};
+      uint32_t f[TERMS][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float f = i & 1 ? up * 0.0625f : up;
-        const float v0 = x[w][el[i][0]] * f, v1 = x[w][el[i][1]] * f;
-        qf[0][nt][w][i] = pack_half2(v0, v1);
+        const float p2 = i & 1 ? sign * 0.0625f : sign;
+        const float v0 = x[w][el[i][0]] * p2, v1 = x[w][el[i][1]] * p2;
+        f[0][i] = pack_half2(v0, v1);
         if constexpr (TERMS == 2) {
-          const float2 hi = unpack_half2(qf[0][nt][w][i]);
-          qf[1][nt][w][i] = pack_half2(v0 - hi.x, v1 - hi.y);
+          const float2 hi = unpack_half2(f[0][i]);
+          f[1][i] = pack_half2(v0 - hi.x, v1 - hi.y);
         }
       }
+#pragma unroll
+      for (int term = 0; term < TERMS; ++term)
+        if constexpr (QS) {
+          if (warp == nt % WARPS)
+            *reinterpret_cast<uint4*>(smem + Sm::q_at + ((term * NT + nt) * W + w) * 512 + lane * 16) =
+                make_uint4(f[term][0], f[term][1], f[term][2], f[term][3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) qf[term][nt][w][i] = f[term][i];
+        }
     }
-    const float s2 = a.scale * kLog2e;
 #pragma unroll
     for (int j2 = 0; j2 < 2; ++j2) {  // what the accumulators' columns 2 c, 2 c + 1 need
       const int from = (2 * c + j2) * 4;
-      fac[nt][j2] = __shfl_sync(0xffffffffu, down, from) * (CENTRED ? s2 : 16777216.0f * s2);
+      fac[nt][j2] = __shfl_sync(0xffffffffu, down, from) * kCode * fabsf(a.scale) * kLog2e;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) qs[nt][j2][g] = __shfl_sync(0xffffffffu, sum[g], from) * s2;
+      for (int g = 0; g < NG; ++g) qs[nt][j2][g] = __shfl_sync(0xffffffffu, sum[g] * sign, from) * (1.0f / kCode);
       const int cj = col0 + nt * 8 + 2 * c + j2;
       vis[nt][j2] = cj < cols ? visible(a.causal, len, n, cj / group) : 0;
     }
   }
 
-  float o[NT][2 * W][4], m[NT][2], l[NT][2], z[NT][2][NG];
+  if constexpr (QS) __syncthreads();
+
+  // Logits are kept in raw units (fac times them is log2 units).  A column's
+  // reference mf (log2 units) is raised when a logit exceeds mt.
+  float o[NT][2 * W][4], mf[NT][2], mt[NT][2], l[NT][2], z[NT][2][NG], zc[NT][NG][4];
   float cap = 0.0f, hold = 0.0f;  // value scales are at most cap; hold = kTop / cap
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -318,195 +345,230 @@ __global__ void __launch_bounds__(Shape<D, NT, TERMS>::warps * 32, Shape<D, NT, 
       for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.0f;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      m[nt][j] = -INFINITY;
+      mf[nt][j] = mt[nt][j] = -INFINITY;
       l[nt][j] = 0.0f;
 #pragma unroll
       for (int g = 0; g < NG; ++g) z[nt][j][g] = 0.0f;
     }
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) zc[nt][g][e] = 0.0f;
   }
 
-  for (int i = 0; i < mine; ++i) {
-    const int stage = i % STAGES, t0 = t_begin + (warp + i * WARPS) * TOKENS;
-    if (!dead && !tc::mbar_wait(&full[warp][stage], (i / STAGES) & 1, 402)) dead = true;
-    dead = __any_sync(0xffffffffu, dead);
-    if (dead) {  // give up: wait (bounded) for the copies still in flight, then return
-      for (int k = i + 1; k < i + STAGES && k < mine; ++k)
-        tc::mbar_wait(&full[warp][k % STAGES], (k / STAGES) & 1, 402);
-      break;
-    }
-    const uint32_t base = ring + stage * Sm::stage;
-    const bool masked = t0 + TOKENS > t_free;
-
+  // SUB units at shared address `sub`, from token ts on.  MASKED: some column
+  // does not see some of the tokens.
+  auto absorb = [&](uint32_t sub, int ts, auto masked) {
+    constexpr bool MASKED = decltype(masked)::value;
+    // S^T: rows r and r + 8 of each unit, columns 2 c and 2 c + 1 of each tile
+    float s[SUB][NT][4], top[NT][2];
 #pragma unroll
-    for (int u0 = 0; u0 < UNITS; u0 += SUB) {
-      const uint32_t sub = base + u0 * UB;
-      const int ts = t0 + u0 * kUnit;
-      // ---- S^T of the run's tokens (rows r and r + 8 of each unit), in log2 units
-      float s[SUB][NT][4], top[NT][2];
+    for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
+    for (int u = 0; u < SUB; ++u) {
+      const uint32_t unit = sub + u * UB;
+      uint32_t k0[W], k1[W];
+      lds_words<W>(unit + k_chunk<D>(r, c), k0);
+      lds_words<W>(unit + k_chunk<D>(r + 8, c), k1);
 #pragma unroll
-      for (int u = 0; u < SUB; ++u) {
-        const uint32_t unit = sub + u * UB;
-        uint32_t k0[W], k1[W];
-        lds_words<W>(unit + k_chunk<D>(r, c), k0);
-        lds_words<W>(unit + k_chunk<D>(r + 8, c), k1);
+      for (int g = 0; g < NG; ++g) {
+        float acc[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[u][nt][e] = 0.0f;
+          for (int e = 0; e < 4; ++e) acc[nt][e] = 0.0f;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          float acc[NT][4];
+        for (int w = g * WPG; w < (g + 1) * WPG; ++w) {
+          uint32_t x0 = k0[w], x1 = k1[w], qw[TERMS][NT][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int term = 0; term < TERMS; ++term)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[nt][e] = 0.0f;
+            for (int nt = 0; nt < NT; ++nt)
+              if constexpr (QS) {
+                lds_words<4>(q_at + ((term * NT + nt) * W + w) * 512, qw[term][nt]);
+              } else {
 #pragma unroll
-          for (int w = g * WPG; w < (g + 1) * WPG; ++w) {
-            uint32_t x0 = k0[w], x1 = k1[w];
-#pragma unroll
-            for (int i2 = 0; i2 < 4; i2 += 2) {
-              const uint32_t a0 = codes_lo<CENTRED>(x0), a1 = codes_lo<CENTRED>(x1), a2 = codes_hi<CENTRED>(x0),
-                             a3 = codes_hi<CENTRED>(x1);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int term = 0; term < TERMS; ++term)
-                  mma16816(acc[nt], a0, a1, a2, a3, qf[term][nt][w][i2], qf[term][nt][w][i2 + 1]);
-              x0 >>= 8;
-              x1 >>= 8;
-            }
-          }
-          const float2 p0 = lds_half2(unit + kp_base(D) + (r * NG + g) * 4);
-          const float2 p1 = lds_half2(unit + kp_base(D) + ((r + 8) * NG + g) * 4);
-          const float off0 = CENTRED ? p0.y : fmaf(-8.0f, p0.x, p0.y), off1 = CENTRED ? p1.y : fmaf(-8.0f, p1.x, p1.y);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              s[u][nt][e] += fmaf(acc[nt][e] * fac[nt][e & 1], e < 2 ? p0.x : p1.x, qs[nt][e & 1][g] * (e < 2 ? off0 : off1));
-        }
-        if (masked) {
-          const int t = ts + u * kUnit + r;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (t + (e < 2 ? 0 : 8) >= vis[nt][e & 1]) s[u][nt][e] = -INFINITY;
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          top[nt][0] = fmaxf(top[nt][0], fmaxf(s[u][nt][0], s[u][nt][2]));
-          top[nt][1] = fmaxf(top[nt][1], fmaxf(s[u][nt][1], s[u][nt][3]));
-        }
-      }
-
-      // ---- value parameters; raise the running maxima where they have to be
-      float2 vp[SUB][2][NG];
-      float vtop = 0.0f;
-#pragma unroll
-      for (int u = 0; u < SUB; ++u)
-#pragma unroll
-        for (int i2 = 0; i2 < 2; ++i2)
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            float2 p = lds_half2(sub + u * UB + vp_base(D, NG) + ((r + 8 * i2) * NG + g) * 4);
-            if (masked && ts + u * kUnit + r + 8 * i2 >= t_end) p = make_float2(0.0f, 0.0f);
-            vp[u][i2][g] = p;
-            vtop = fmaxf(vtop, p.x);
-          }
-      bool raise = vtop > cap;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) raise |= top[nt][0] > m[nt][0] + kRaise || top[nt][1] > m[nt][1] + kRaise;
-      if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-        for (int k = 4; k <= 16; k <<= 1) {
-          vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, k));
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) top[nt][j] = fmaxf(top[nt][j], __shfl_xor_sync(0xffffffffu, top[nt][j], k));
-        }
-        float fcap = 1.0f;
-        if (vtop > cap) {  // the next power of two above it
-          const float up = 2.0f * __uint_as_float(__float_as_uint(vtop) & 0x7F800000u);
-          fcap = cap / up;
-          cap = up;
-          hold = kTop / up;
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float m2 = fmaxf(m[nt][j], top[nt][j]);
-            const float f = m2 == m[nt][j] ? 1.0f : ex2(m[nt][j] - m2);
-            m[nt][j] = m2;
-            l[nt][j] *= f;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) z[nt][j][g] *= f;
-#pragma unroll
-            for (int i2 = 0; i2 < 2 * W; ++i2) o[nt][i2][j] *= f * fcap, o[nt][i2][j + 2] *= f * fcap;
-          }
-      }
-
-      // ---- weights and the second product
-      const float centre = cap * (-8.0f / kTop);
-#pragma unroll
-      for (int u = 0; u < SUB; ++u) {
-        const uint32_t unit = sub + u * UB;
-        uint32_t v0[W], v1[W];
-        lds_words<W>(unit + v_chunk<D>(0, lane), v0);
-        lds_words<W>(unit + v_chunk<D>(1, lane), v1);
-        uint32_t pf[TERMS][NT][NG][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float p[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float ms = m[nt][e & 1];
-            p[e] = ex2(s[u][nt][e] - (ms == -INFINITY ? 0.0f : ms));
-            l[nt][e & 1] += p[e];
-          }
-#pragma unroll
-          for (int g = 0; g < NG; ++g)
-#pragma unroll
-            for (int i2 = 0; i2 < 2; ++i2) {
-              const float2 vs = vp[u][i2][g];
-              float w0 = p[2 * i2] * (vs.x * hold), w1 = p[2 * i2 + 1] * (vs.x * hold);
-              float y0 = p[2 * i2] * vs.y, y1 = p[2 * i2 + 1] * vs.y;
-              if (masked) {  // a token that a column does not see may hold NaN
-                if (s[u][nt][2 * i2] == -INFINITY) w0 = y0 = 0.0f;
-                if (s[u][nt][2 * i2 + 1] == -INFINITY) w1 = y1 = 0.0f;
+                for (int i = 0; i < 4; ++i) qw[term][nt][i] = qf[term][nt][w][i];
               }
-              const uint32_t hi = pack_half2(w0, w1);
-              const float2 got = unpack_half2(hi);
-              pf[0][nt][g][i2] = transpose8x8(hi);
-              if constexpr (TERMS == 2) pf[1][nt][g][i2] = transpose8x8(pack_half2(w0 - got.x, w1 - got.y));
-              z[nt][0][g] += CENTRED ? y0 : fmaf(got.x, centre, y0);
-              z[nt][1][g] += CENTRED ? y1 : fmaf(got.y, centre, y1);
-            }
-        }
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-          uint32_t y0 = v0[w], y1 = v1[w];
-#pragma unroll
-          for (int i2 = 0; i2 < 2; ++i2) {
-            const uint32_t a0 = codes_lo<CENTRED>(y0), a1 = codes_hi<CENTRED>(y0), a2 = codes_lo<CENTRED>(y1),
-                           a3 = codes_hi<CENTRED>(y1);
+          for (int i2 = 0; i2 < 4; i2 += 2) {
+            const uint32_t a0 = codes_lo<CENTRED>(x0), a1 = codes_lo<CENTRED>(x1), a2 = codes_hi<CENTRED>(x0),
+                           a3 = codes_hi<CENTRED>(x1);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int term = 0; term < TERMS; ++term)
-                mma16816(o[nt][2 * w + i2], a0, a1, a2, a3, pf[term][nt][w / WPG][0], pf[term][nt][w / WPG][1]);
-            y0 >>= 8;
-            y1 >>= 8;
+                mma16816(acc[nt], a0, a1, a2, a3, qw[term][nt][i2], qw[term][nt][i2 + 1]);
+            x0 >>= 8;
+            x1 >>= 8;
           }
+        }
+        const float2 p0 = lds_half2(unit + kp_base(D) + (r * NG + g) * 4);
+        const float2 p1 = lds_half2(unit + kp_base(D) + ((r + 8) * NG + g) * 4);
+        const float off0 = CENTRED ? p0.y : fmaf(-8.0f, p0.x, p0.y), off1 = CENTRED ? p1.y : fmaf(-8.0f, p1.x, p1.y);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float off = qs[nt][e & 1][g] * (e < 2 ? off0 : off1);
+            s[u][nt][e] = fmaf(acc[nt][e], e < 2 ? p0.x : p1.x, g ? s[u][nt][e] + off : off);
+          }
+      }
+      if constexpr (MASKED) {
+        const int t = ts + u * kUnit + r;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (t + (e < 2 ? 0 : 8) >= vis[nt][e & 1]) s[u][nt][e] = -INFINITY;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        top[nt][0] = fmaxf(top[nt][0], fmaxf(s[u][nt][0], s[u][nt][2]));
+        top[nt][1] = fmaxf(top[nt][1], fmaxf(s[u][nt][1], s[u][nt][3]));
+      }
+    }
+
+    // value parameters; raise the references where they have to be
+    float2 vp[SUB][2][NG];
+    float vtop = 0.0f;
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int i2 = 0; i2 < 2; ++i2)
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          float2 p = lds_half2(sub + u * UB + vp_base(D, NG) + ((r + 8 * i2) * NG + g) * 4);
+          if (MASKED && ts + u * kUnit + r + 8 * i2 >= t_end) p = make_float2(0.0f, 0.0f);
+          vp[u][i2][g] = p;
+          vtop = fmaxf(vtop, p.x);
+        }
+    bool raise = vtop > cap;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) raise |= top[nt][0] > mt[nt][0] || top[nt][1] > mt[nt][1];
+    if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+      for (int k = 4; k <= 16; k <<= 1) {
+        vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, k));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) top[nt][j] = fmaxf(top[nt][j], __shfl_xor_sync(0xffffffffu, top[nt][j], k));
+      }
+      float fcap = 1.0f;
+      if (vtop > cap) {  // the next power of two above it
+        const float up = 2.0f * __uint_as_float(__float_as_uint(vtop) & 0x7F800000u);
+        fcap = cap / up;
+        cap = up;
+        hold = kTop / up;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float f = 1.0f;
+          if (top[nt][j] > mt[nt][j]) {
+            const float m2 = top[nt][j] * fac[nt][j];
+            f = ex2(mf[nt][j] - m2);
+            mf[nt][j] = m2;
+            mt[nt][j] = top[nt][j] + (fac[nt][j] > 0.0f ? kRaise / fac[nt][j] : 1.0e38f);
+          }
+          l[nt][j] *= f;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) z[nt][j][g] *= f;
+          f *= fcap;
+#pragma unroll
+          for (int i2 = 0; i2 < 2 * W; ++i2) o[nt][i2][j] *= f, o[nt][i2][j + 2] *= f;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) zc[nt][g][j] *= f;
+        }
+    }
+
+    // weights and the second product
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      const uint32_t unit = sub + u * UB;
+      uint32_t v0[W], v1[W];
+      lds_words<W>(unit + v_chunk<D>(0, lane), v0);
+      lds_words<W>(unit + v_chunk<D>(1, lane), v1);
+      uint32_t pf[TERMS][NT][NG][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[e] = ex2(fmaf(s[u][nt][e], fac[nt][e & 1], -mf[nt][e & 1]));
+          if (MASKED && s[u][nt][e] == -INFINITY) p[e] = 0.0f;
+          l[nt][e & 1] += p[e];
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+          for (int i2 = 0; i2 < 2; ++i2) {
+            const float2 vs = vp[u][i2][g];
+            const float held = vs.x * hold;
+            float w0 = p[2 * i2] * held, w1 = p[2 * i2 + 1] * held;
+            if constexpr (MASKED) {  // a token that a column does not see may hold NaN
+              const bool n0 = s[u][nt][2 * i2] == -INFINITY, n1 = s[u][nt][2 * i2 + 1] == -INFINITY;
+              w0 = n0 ? 0.0f : w0;
+              w1 = n1 ? 0.0f : w1;
+              z[nt][0][g] += n0 ? 0.0f : p[2 * i2] * vs.y;
+              z[nt][1][g] += n1 ? 0.0f : p[2 * i2 + 1] * vs.y;
+            } else {
+              z[nt][0][g] = fmaf(p[2 * i2], vs.y, z[nt][0][g]);
+              z[nt][1][g] = fmaf(p[2 * i2 + 1], vs.y, z[nt][1][g]);
+            }
+            const uint32_t hi = pack_half2(w0, w1);
+            pf[0][nt][g][i2] = transpose8x8(hi);
+            if constexpr (TERMS == 2) {
+              const float2 got = unpack_half2(hi);
+              pf[1][nt][g][i2] = transpose8x8(pack_half2(w0 - got.x, w1 - got.y));
+            }
+          }
+        if constexpr (!CENTRED) {  // the rounded weights' sums: a product with ones
+#pragma unroll
+          for (int g = 0; g < NG; ++g)
+            mma16816(zc[nt][g], 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, pf[0][nt][g][0], pf[0][nt][g][1]);
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        uint32_t y0 = v0[w], y1 = v1[w];
+#pragma unroll
+        for (int i2 = 0; i2 < 2; ++i2) {
+          const uint32_t a0 = codes_lo<CENTRED>(y0), a1 = codes_hi<CENTRED>(y0), a2 = codes_lo<CENTRED>(y1),
+                         a3 = codes_hi<CENTRED>(y1);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int term = 0; term < TERMS; ++term)
+              mma16816(o[nt][2 * w + i2], a0, a1, a2, a3, pf[term][nt][w / WPG][0], pf[term][nt][w / WPG][1]);
+          y0 >>= 8;
+          y1 >>= 8;
         }
       }
     }
+  };
+
+  const uint32_t stages = tc::smem_u32(smem) + warp * STAGES * Sm::stage;
+  for (int i = 0, stage = 0, parity = 0; i < mine; ++i) {
+    if (__any_sync(0xffffffffu, !tc::mbar_wait(&full[warp][stage], parity, 402))) {
+      // give up: wait (bounded) for the copies still in flight, then return
+      for (int k = i + 1; k < i + STAGES && k < mine; ++k)
+        tc::mbar_wait(&full[warp][k % STAGES], (k / STAGES) & 1, 402);
+      break;
+    }
+    const int t0 = t_begin + (warp + i * WARPS) * TOKENS;
+    if (t0 + TOKENS <= t_free) {
+#pragma unroll 1
+      for (int u = 0; u < UNITS; u += SUB) absorb(stages + stage * Sm::stage + u * UB, t0 + u * kUnit, std::false_type{});
+    } else {
+#pragma unroll 1
+      for (int u = 0; u < UNITS; u += SUB) absorb(stages + stage * Sm::stage + u * UB, t0 + u * kUnit, std::true_type{});
+    }
     __syncwarp();  // every lane has read the stage
-    if (i + STAGES < mine) issue(i + STAGES);
+    if (i + STAGES < mine) issue(i + STAGES, stage);
+    if (++stage == STAGES) stage = 0, parity ^= 1;
   }
 
   // ---- join the warps' results through shared memory
@@ -524,16 +586,16 @@ __global__ void __launch_bounds__(Shape<D, NT, TERMS>::warps * 32, Shape<D, NT, 
 #pragma unroll
         for (int g = 0; g < NG; ++g) z[nt][j][g] += __shfl_xor_sync(0xffffffffu, z[nt][j][g], k);
       }
-      const float unhold = cap * (1.0f / kTop), f0 = unhold * (CENTRED ? 1.0f : 16777216.0f), f1 = f0 * 0.0625f;
+      const float unhold = cap * (1.0f / kTop), f0 = unhold * kCode, f1 = f0 * 0.0625f;
       float* dst = so + (warp * COLS + col) * Sm::o_stride + 4 * r;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        const float zg = z[nt][j][w / WPG];
+        const float zg = CENTRED ? z[nt][j][w / WPG] : fmaf(-8.0f * unhold, zc[nt][w / WPG][j], z[nt][j][w / WPG]);
         *reinterpret_cast<float4*>(dst + 32 * w) =
             make_float4(fmaf(o[nt][2 * w][j + 2], f1, zg), fmaf(o[nt][2 * w][j], f0, zg),
                         fmaf(o[nt][2 * w + 1][j + 2], f1, zg), fmaf(o[nt][2 * w + 1][j], f0, zg));
       }
-      if (r == 0) sml[warp * COLS + col] = make_float2(m[nt][j], l[nt][j]);
+      if (r == 0) sml[warp * COLS + col] = make_float2(mf[nt][j], l[nt][j]);
     }
   }
   __syncthreads();
@@ -628,7 +690,7 @@ int launch(const Layout& L, const Step& S, const Split& P, const void* pool, con
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sm::bytes);
   if (e != cudaSuccess) return fail(KVC_ERR_LAUNCH, std::string("attend_kernel: ") + cudaGetErrorString(e));
   const dim3 grid((unsigned)n_items, (unsigned)L.n_kv, (unsigned)col_tiles);
-  kernel<<<grid, Shape<D, NT, TERMS>::warps * 32, Sm::bytes, st>>>(L, S, P, static_cast<const uint8_t*>(pool), a, part);
+  kernel<<<grid, Shape<D, WPG, NT, TERMS>::warps * 32, Sm::bytes, st>>>(L, S, P, static_cast<const uint8_t*>(pool), a, part);
   return check_launch("attend_kernel");
 }
 
@@ -679,6 +741,7 @@ extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* 
   if (!aligned16(pool)) return fail(KVC_ERR_ALIGN, "kvc_kv4_attend: pool not 16-byte aligned");
   if (n_q < 1 || n_q % layout->n_kv) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: n_q must be a multiple of n_kv");
   if (step->n_tokens == 0 || split->n_items == 0) return KVC_OK;
+  if (!split->items || !aligned16(split->items)) return fail(KVC_ERR_ALIGN, "kvc_kv4_attend: items not 16-byte aligned");
   if (step->n_tokens < 0 || step->n_tokens > INT32_MAX || step->max_new < 1 || split->n_items < 0 ||
       split->n_items > INT32_MAX || split->chunk < 64 || split->chunk % 64)
     return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: bad step or split sizes");
@@ -688,7 +751,7 @@ extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* 
   if (need && (!workspace || ws_bytes < need || !aligned16(workspace)))
     return fail(KVC_ERR_WORKSPACE, "kvc_kv4_attend: workspace too small or not 16-byte aligned");
   const Step s{step->n_seqs, step->rows, step->kv_len, step->q_start};
-  const Split p{split->item_seq, split->item_first, split->item_start, split->chunk, split->max_items};
+  const Split p{reinterpret_cast<const int4*>(split->items), split->item_start, split->chunk, split->max_items};
   const Qkv a{q, out, q_seq_stride, q_token_stride, q_head_stride, o_seq_stride, o_token_stride, o_head_stride,
               packed, dtype, n_q, causal, scale};
   Partial part{static_cast<float*>(workspace), nullptr, cols};

@@ -388,9 +388,10 @@ int kvc_kv4_read(const kvc_kv4_layout* layout, const void* pool, int64_t layer_b
  * over their sequences' pages.  causal: query i of a sequence's n sees the
  * first kv_len - n + 1 + i tokens, otherwise all kv_len.  A query that sees
  * nothing gets zeros.  Strides in elements, as for kvc_kv4_write. */
-/* kvc_kv4_attend_tiles: blocks that work on one item of one KV head, for choosing
- * the split. */
-int kvc_kv4_attend_tiles(const kvc_kv4_layout* layout, const kvc_kv4_step* step, int n_q, int dtype);
+/* For choosing the split: the blocks that work on one item of one KV head
+ * (tiles) and the blocks that the current device runs at once (resident). */
+int kvc_kv4_attend_shape(const kvc_kv4_layout* layout, const kvc_kv4_step* step, int n_q, int dtype, int* tiles,
+                         int* resident);
 size_t kvc_kv4_attend_workspace_bytes(const kvc_kv4_layout* layout, const kvc_kv4_step* step,
                                       const kvc_kv4_split* split, int n_q);
 int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* step, const kvc_kv4_split* split,

@@ -46,7 +46,7 @@ class CacheStep:
     cache: Any = field(repr=False)
     meta: torch.Tensor = field(repr=False)  # device arrays that ``desc`` points into
     desc: Kv4Step = field(repr=False)
-    splits: dict[int, tuple[Kv4Split, torch.Tensor]] = field(default_factory=dict, repr=False)
+    splits: dict[tuple[int, int], tuple[Kv4Split, torch.Tensor]] = field(default_factory=dict, repr=False)
 
     @property
     def tokens(self) -> int:
@@ -148,7 +148,6 @@ class PagedKVCache:
         self._layers = [self.pool.data_ptr() + i * self.pool.stride(0) for i in range(self.n_layers)]
         self._layout = Kv4Layout(self.table.data_ptr(), self.table.stride(0), self.pages.n_pages, self.n_kv_heads,
                                  self.head_dim, self.page_size, self.group_size)
-        self._slots = 2 * torch.cuda.get_device_properties(device).multi_processor_count
 
     # ---- sequences ---------------------------------------------------------
 
@@ -221,18 +220,19 @@ class PagedKVCache:
                        int(q_start[-1]))
         return CacheStep(seqs, counts, lengths.tolist(), writable, self.pages.epoch, self, meta, desc)
 
-    def _split(self, step: CacheStep, copies: int) -> Kv4Split:
-        got = step.splits.get(copies)
+    def _split(self, step: CacheStep, n_q: int, code: int) -> Kv4Split:
+        got = step.splits.get((n_q, code))
         if got is None:
             lengths = np.array(step.lengths, dtype=np.int64)
-            chunk = split_chunk(lengths, copies, self._slots)
+            tiles, resident = ops.kv4_attend_shape(self._layout, step.desc, n_q, code, self.device)
+            chunk = split_chunk(lengths, self.n_kv_heads * tiles, resident)
             items = np.maximum(1, -(-lengths // chunk))
             start = _prefix(items)
             seq = np.repeat(np.arange(len(step.seqs)), items)
             rows = np.array([self.pages.row(s) for s in step.seqs], dtype=np.int64)
             table = np.stack((seq, (np.arange(int(start[-1])) - start[seq]) * chunk, rows[seq], lengths[seq]), 1)
             buf, at = _upload((table.reshape(-1), start), self.device)
-            got = step.splits[copies] = (Kv4Split(at[0], at[1], int(start[-1]), chunk, int(items.max(initial=1))), buf)
+            got = step.splits[n_q, code] = (Kv4Split(at[0], at[1], int(start[-1]), chunk, int(items.max(initial=1))), buf)
         return got[0]
 
     def _check(self, what: str, layer: int, step: CacheStep) -> int:
@@ -269,7 +269,7 @@ class PagedKVCache:
         tokens up to its own position, otherwise all cached tokens of its sequence;
         one that sees none gets zeros.  ``scale`` defaults to ``head_dim ** -0.5``."""
         pool = self._check("attend", layer, step)
-        return ops.kv4_attend(self._layout, step.desc, lambda copies: self._split(step, copies), pool, query,
+        return ops.kv4_attend(self._layout, step.desc, lambda n_q, code: self._split(step, n_q, code), pool, query,
                               causal=causal, scale=self.head_dim ** -0.5 if scale is None else float(scale),
                               device=self.device)
 

@@ -115,6 +115,7 @@ __global__ void __launch_bounds__(128) kv4_write_kernel(Layout L, Step S, uint8_
                                                         const int32_t* __restrict__ half_seq,
                                                         const int32_t* __restrict__ half_start) {
   constexpr int W = D / 32, NG = W / WPG;
+  grid_go();  // the attention of these tokens may get ready
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int64_t id = blockIdx.x * 4LL + (threadIdx.x >> 5);
   if (id >= n_halves * L.n_kv * 2) return;

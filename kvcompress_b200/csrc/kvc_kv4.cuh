@@ -77,6 +77,31 @@ __device__ __forceinline__ int64_t unit_off(const Layout& L, int64_t p, int h, i
   return ((p * L.n_kv + h) * per_page + ((pos >> 4) & (per_page - 1))) * (int64_t)unit_bytes(D, L.groups);
 }
 
+// Programmatic launches: a kernel launched with launch_after may start while
+// the previous one of its stream runs; grid_wait returns when that one is
+// complete and its writes are visible, and comes before everything else in
+// every thread.  grid_go lets the next such kernel start (its grid_wait still
+// waits for this grid's end).
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename K, typename... A>
+int launch_after(const char* what, K kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_t st, const A&... args) {
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) return fail(KVC_ERR_LAUNCH, std::string(what) + ": " + cudaGetErrorString(e));
+  return check_launch(what);
+}
+
 // Host side: argument checks shared by the entry points.
 int check_layout(const kvc_kv4_layout* l, const char* what);
 Layout to_layout(const kvc_kv4_layout* l);

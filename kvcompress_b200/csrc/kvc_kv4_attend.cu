@@ -170,12 +170,12 @@ template <int D, int WPG, int NT, int TERMS>
 struct Shape {
   static constexpr int NG = D / 32 / WPG;
   // Registers a thread needs, roughly (accumulators, queries, columns' and
-  // groups' statistics): with up to 128 an SM has 16 warps (2 blocks of 8),
-  // with up to 168 it has 12 (3 of 4), else 8 (2 of 4).
+  // groups' statistics): with up to 128 an SM has 4 blocks of 4 warps, with up
+  // to 168 three, else two.
   static constexpr int regs = 45 + D / 4 * NT + (NT * TERMS == 1 ? D / 8 : 0) + 10 * NT + 8 * NG * NT +
                               units_at_once(NT, NG) * 4 * (NT + NG) + 35 * (TERMS - 1);
-  static constexpr int warps = regs < 145 ? 8 : 4;
-  static constexpr int blocks = regs < 145 ? 2 : regs < 180 ? 3 : 2;
+  static constexpr int warps = 4;
+  static constexpr int blocks = regs < 145 ? 4 : regs < 180 ? 3 : 2;
   static constexpr int units = 256 / D;  // of a stage
   static constexpr int tokens = units * kUnit;
 };
@@ -211,6 +211,8 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[WARPS][STAGES];
 
+  grid_wait();
+  grid_go();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int item = blockIdx.x, h = blockIdx.y, col0 = blockIdx.z * COLS;
   const int4 it = P.items[item];
@@ -633,13 +635,17 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
   }
 }
 
-// Joins the items of the sequences that have several: a warp per query and
-// head, items in their order.
+// Joins the items of the sequences that have several: a block per query and
+// head.  Group g of D / 4 threads (a float4 of features each) takes items g, g +
+// G, ..., so that eight loads a thread are on their way at once; the groups are
+// added in their order.
 template <int D>
 __global__ void __launch_bounds__(128) attend_join_kernel(Layout L, Step S, Split P, Qkv a, Partial part) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31, tok = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5);
-  if (head >= a.n_q) return;
+  constexpr int T = D / 4, G = 128 / T;
+  __shared__ float4 so[G][T];
+  __shared__ float ss[G];
+  grid_wait();
+  const int lane = threadIdx.x & 31, g = threadIdx.x / T, x = threadIdx.x % T, tok = blockIdx.x, head = blockIdx.y;
   const int b = seq_of(S, tok), i0 = P.item_start[b], i1 = P.item_start[b + 1];
   if (i1 - i0 == 1) return;
   const int q0 = S.q_start[b], n = S.q_start[b + 1] - q0, j = tok - q0, group = a.n_q / L.n_kv;
@@ -651,31 +657,42 @@ __global__ void __launch_bounds__(128) attend_join_kernel(Layout L, Step S, Spli
   for (int i = lane; i < items; i += 32) top = fmaxf(top, part.ml[at0 + i * step].x);
 #pragma unroll
   for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-  float acc[E], sum = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float sum = 0.0f;
+  for (int i = g; i < items; i += 8 * G) {
+    float4 v[8];
+    float2 ml[8];
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < items; ++i) {
-    const float2 ml = part.ml[at0 + i * step];
-    const float* o = part.o + (at0 + i * step) * D + lane * E;
-    float v[E];
-    if constexpr (E == 4) {
-      const float4 x = *reinterpret_cast<const float4*>(o);
-      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-    } else {
-      const float2 x = *reinterpret_cast<const float2*>(o);
-      v[0] = x.x, v[1] = x.y;
-    }
-    const bool none = ml.y == 0.0f;
-    const float f = none ? 0.0f : ex2(ml.x - top);
-    sum = fmaf(ml.y, f, sum);
+    for (int u = 0; u < 8; ++u)
+      if (i + u * G < items) {
+        v[u] = *reinterpret_cast<const float4*>(part.o + (at0 + (i + u * G) * step) * D + x * 4);
+        ml[u] = part.ml[at0 + (i + u * G) * step];
+      }
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = none ? acc[e] : fmaf(v[e], f, acc[e]);
+    for (int u = 0; u < 8; ++u)
+      if (i + u * G < items && ml[u].y != 0.0f) {  // 0: saw nothing
+        const float f = ex2(ml[u].x - top);
+        sum = fmaf(ml[u].y, f, sum);
+        acc.x = fmaf(v[u].x, f, acc.x), acc.y = fmaf(v[u].y, f, acc.y);
+        acc.z = fmaf(v[u].z, f, acc.z), acc.w = fmaf(v[u].w, f, acc.w);
+      }
+  }
+  so[g][x] = acc;
+  if (x == 0) ss[g] = sum;
+  __syncthreads();
+  if (g) return;
+#pragma unroll
+  for (int k = 1; k < G; ++k) {
+    const float4 v = so[k][x];
+    acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+    sum += ss[k];
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  const int64_t at = (a.packed ? (int64_t)tok * a.o_st : b * a.o_sb + j * a.o_st) + (int64_t)head * a.o_sh + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; ++e) store_dt(a.out, at + e, acc[e] * inv, a.dtype);
+  const int64_t at = (a.packed ? (int64_t)tok * a.o_st : b * a.o_sb + j * a.o_st) + (int64_t)head * a.o_sh + x * 4;
+  store_dt(a.out, at, acc.x * inv, a.dtype);
+  store_dt(a.out, at + 1, acc.y * inv, a.dtype);
+  store_dt(a.out, at + 2, acc.z * inv, a.dtype);
+  store_dt(a.out, at + 3, acc.w * inv, a.dtype);
 }
 
 // Tiles of 8 columns a block takes: as many as there are, up to what the
@@ -690,8 +707,8 @@ int launch(const Layout& L, const Step& S, const Split& P, const void* pool, con
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sm::bytes);
   if (e != cudaSuccess) return fail(KVC_ERR_LAUNCH, std::string("attend_kernel: ") + cudaGetErrorString(e));
   const dim3 grid((unsigned)n_items, (unsigned)L.n_kv, (unsigned)col_tiles);
-  kernel<<<grid, Shape<D, WPG, NT, TERMS>::warps * 32, Sm::bytes, st>>>(L, S, P, static_cast<const uint8_t*>(pool), a, part);
-  return check_launch("attend_kernel");
+  return launch_after("attend_kernel", kernel, grid, Shape<D, WPG, NT, TERMS>::warps * 32, Sm::bytes, st, L, S, P,
+                      static_cast<const uint8_t*>(pool), a, part);
 }
 
 template <int D, int WPG>
@@ -717,11 +734,24 @@ int launch_tiles(const Layout& L, const Step& S, const Split& P, const void* poo
 using namespace kvc;
 using namespace kvc::kv4;
 
-extern "C" int kvc_kv4_attend_tiles(const kvc_kv4_layout* layout, const kvc_kv4_step* step, int n_q, int dtype) {
-  if (!layout || !step || layout->n_kv < 1 || layout->group_size < 1 || n_q < 1) return 0;
-  const int64_t cols = (int64_t)step->max_new * (n_q / layout->n_kv);
-  if (cols <= 0 || cols > INT32_MAX) return 0;
-  return (int)ceil_div(cols, 8 * tiles_of((int)cols, dtype == KVC_F32 ? 2 : 1, layout->head_dim / layout->group_size));
+extern "C" int kvc_kv4_attend_shape(const kvc_kv4_layout* layout, const kvc_kv4_step* step, int n_q, int dtype,
+                                    int* tiles, int* resident) {
+  if (int rc = check_layout(layout, "kvc_kv4_attend_shape")) return rc;
+  if (!step || !tiles || !resident) return fail(KVC_ERR_ARG, "kvc_kv4_attend_shape: NULL pointer");
+  if (n_q < 1 || n_q % layout->n_kv) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend_shape: n_q must be a multiple of n_kv");
+  const int64_t cols = std::max<int64_t>(1, (int64_t)step->max_new * (n_q / layout->n_kv));
+  if (cols > INT32_MAX / 2) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend_shape: too many queries");
+  const int terms = dtype == KVC_F32 ? 2 : 1, nt = tiles_of((int)cols, terms, layout->head_dim / layout->group_size);
+  *tiles = (int)ceil_div(cols, 8 * nt);
+  int blocks = 0;
+#define KVC_F(D, WPG)                                                                                    \
+  blocks = terms == 2 ? (nt == 1 ? Shape<D, WPG, 1, 2>::blocks : Shape<D, WPG, 2, 2>::blocks)            \
+                      : (nt == 1 ? Shape<D, WPG, 1, 1>::blocks                                           \
+                                 : nt == 2 ? Shape<D, WPG, 2, 1>::blocks : Shape<D, WPG, 4, 1>::blocks)
+  KVC_KV4_DISPATCH(layout, KVC_F);
+#undef KVC_F
+  *resident = blocks * num_sms();
+  return KVC_OK;
 }
 
 extern "C" size_t kvc_kv4_attend_workspace_bytes(const kvc_kv4_layout* layout, const kvc_kv4_step* step,
@@ -739,7 +769,7 @@ extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* 
   if (!step || !split || !pool || !q || !out) return fail(KVC_ERR_ARG, "kvc_kv4_attend: NULL pointer");
   if (!dtype_ok(dtype)) return fail(KVC_ERR_DTYPE, "kvc_kv4_attend: bad dtype");
   if (!aligned16(pool)) return fail(KVC_ERR_ALIGN, "kvc_kv4_attend: pool not 16-byte aligned");
-  if (n_q < 1 || n_q % layout->n_kv) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: n_q must be a multiple of n_kv");
+  if (n_q < 1 || n_q > 65535 || n_q % layout->n_kv) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: n_q must be a multiple of n_kv");
   if (step->n_tokens == 0 || split->n_items == 0) return KVC_OK;
   if (!split->items || !aligned16(split->items)) return fail(KVC_ERR_ALIGN, "kvc_kv4_attend: items not 16-byte aligned");
   if (step->n_tokens < 0 || step->n_tokens > INT32_MAX || step->max_new < 1 || split->n_items < 0 ||
@@ -763,8 +793,7 @@ extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* 
   KVC_KV4_DISPATCH(layout, KVC_F);
 #undef KVC_F
   if (rc || split->max_items <= 1) return rc;
-  const dim3 grid((unsigned)step->n_tokens, (unsigned)ceil_div(n_q, 4));
-  if (layout->head_dim == 64) attend_join_kernel<64><<<grid, 128, 0, st>>>(L, s, p, a, part);
-  else attend_join_kernel<128><<<grid, 128, 0, st>>>(L, s, p, a, part);
-  return check_launch("attend_join_kernel");
+  const dim3 grid((unsigned)step->n_tokens, (unsigned)n_q);
+  return layout->head_dim == 64 ? launch_after("attend_join_kernel", attend_join_kernel<64>, grid, 128, 0, st, L, s, p, a, part)
+                                : launch_after("attend_join_kernel", attend_join_kernel<128>, grid, 128, 0, st, L, s, p, a, part);
 }

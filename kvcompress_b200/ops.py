@@ -730,8 +730,8 @@ def kv4_write(layout, step, pool: int, key: torch.Tensor, value: torch.Tensor, d
 def kv4_attend(layout, step, split, pool: int, query: torch.Tensor, *, causal: bool, scale: float,
                device: torch.device) -> torch.Tensor:
     """Attention of a step's queries over the pages of the layer at address
-    ``pool`` (``kvc_kv4_attend``).  ``split(copies)`` gives the split of the cached
-    tokens when each item is worked on by ``copies`` CTAs."""
+    ``pool`` (``kvc_kv4_attend``).  ``split(n_q, code)`` gives the split of the
+    cached tokens for ``n_q`` query heads of dtype ``code``."""
     code = _kv4_code(query.dtype)
     qs = _kv4_tokens(query, step, "kv4_attend", None, layout, device)
     n_q = int(query.shape[1])
@@ -743,7 +743,7 @@ def kv4_attend(layout, step, split, pool: int, query: torch.Tensor, *, causal: b
     st = out.stride()
     os_ = (0, st[0], st[1]) if qs[3] else (st[0], st[2], st[1])
     L = lib()
-    sp = split(layout.n_kv * L.kvc_kv4_attend_tiles(layout, step, n_q, code))
+    sp = split(n_q, code)
     ws_n = L.kvc_kv4_attend_workspace_bytes(layout, step, sp, n_q)
     # a buffer of this call's own: a captured graph keeps the one it was captured
     # with, and no other graph or stream writes to it
@@ -753,6 +753,15 @@ def kv4_attend(layout, step, split, pool: int, query: torch.Tensor, *, causal: b
                                code, int(causal), scale, ws.data_ptr() if ws_n else None, ws_n, _stream()),
               "kvc_kv4_attend")
     return out
+
+
+def kv4_attend_shape(layout, step, n_q: int, code: int, device: torch.device) -> tuple[int, int]:
+    """Blocks an item of one KV head is worked on by, and blocks the device runs at once."""
+    tiles, resident = ctypes.c_int(0), ctypes.c_int(0)
+    with _on(device):
+        check(lib().kvc_kv4_attend_shape(layout, step, n_q, code, ctypes.byref(tiles), ctypes.byref(resident)),
+              "kvc_kv4_attend_shape")
+    return tiles.value, resident.value
 
 
 def kv4_read(layout, pool: int, layer_bytes: int, n_layers: int, row: int, t0: int, t1: int, dtype: torch.dtype,

@@ -356,7 +356,7 @@ typedef struct {
 } kvc_kv4_step;
 
 /*
- * Split of the cached tokens into items of `chunk` tokens (a multiple of 64)
+ * Split of the cached tokens into items of `chunk` tokens (a multiple of 128)
  * for kvc_kv4_attend, device arrays of int32: items[4 j ..] (16-byte aligned) are
  * item j's sequence i, its first token, rows[i] and kv_len[i]; it covers `chunk`
  * tokens from the first one on.  The items of sequence i are item_start[i] ..

@@ -85,12 +85,12 @@ def split_chunk(lengths: np.ndarray, copies: int, slots: int) -> int:
             chunk = longest
         else:
             chunk = max(_CHUNK, -(-total * copies // (waves * slots)))
-        chunk = -(-chunk // 64) * 64
+        chunk = -(-chunk // 128) * 128
         while waves and chunk < longest:
             items = int(np.maximum(1, -(-lengths // chunk)).sum()) * copies
             if items <= waves * slots:
                 break
-            chunk += max(64, chunk // 64 // 64 * 64)
+            chunk += max(128, chunk // 64 // 128 * 128)
         items = int(np.maximum(1, -(-lengths // chunk)).sum()) * copies
         c = -(-items // slots) * (min(chunk, longest) + 192)
         if c < cost:

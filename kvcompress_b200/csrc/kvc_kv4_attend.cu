@@ -37,8 +37,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "kvc_kv4.cuh"
-#include "kvc_tma.cuh"
+#include "kvc_kv4_attend.cuh"
 
 namespace kvc {
 
@@ -49,43 +48,14 @@ int kv4_attend_read_device_error(int* out) {
   *out = v;
   int zero = 0;
   cudaMemcpyToSymbol(tc::g_kvc_device_error, &zero, sizeof(int));
-  return KVC_OK;
+  if (v == 0) return kv4::prefill_read_device_error(out);
+  return kv4::prefill_read_device_error(&zero);
 }
 
 namespace kv4 {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRaise = 4.0f;   // log2 units a logit may exceed the running maximum by
 constexpr float kTop = 2048.0f;  // weights p s' are held as (p s' / cap) * kTop <= 2^4 * 2^11 < 65504
-
-struct Qkv {
-  const void* q;
-  void* out;
-  int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;  // element strides of a sequence, a token, a head
-  int packed, dtype, n_q, causal;
-  float scale;
-};
-
-struct Split {
-  const int4* items;  // sequence, first token, table row, cached tokens
-  const int32_t* item_start;
-  int chunk, max_items;
-};
-
-// Partial results of an item: o (unnormalised) and (m, l) of each of its
-// sequence's columns, [item][KV head][column].
-struct Partial {
-  float* o;
-  float2* ml;
-  int64_t cols;  // columns of an item and KV head
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -99,18 +69,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
-}
-
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  uint32_t r;
-  memcpy(&r, &h, 4);
-  return r;
-}
-__device__ __forceinline__ float2 unpack_half2(uint32_t r) {
-  __half2 h;
-  memcpy(&h, &r, 4);
-  return __half22float2(h);
 }
 
 // Two codes of a word as a float16 operand: nibble 0 (lo) or 1 (hi, 16 fold) of
@@ -130,21 +88,6 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
   return y;
 }
 
-template <int W>
-__device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[W]) {
-  if constexpr (W == 4)
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                 : "r"(addr));
-  else
-    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
-}
-__device__ __forceinline__ float2 lds_half2(uint32_t addr) {
-  uint32_t r;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(addr));
-  return unpack_half2(r);
-}
-
 // The sequence of query token `tok` (the last one whose tokens start at or before it).
 __device__ __forceinline__ int seq_of(const Step& S, int tok) {
   int lo = 0, hi = S.n_seqs - 1;
@@ -154,11 +97,6 @@ __device__ __forceinline__ int seq_of(const Step& S, int tok) {
     else hi = mid - 1;
   }
   return lo;
-}
-
-// Tokens that query j of n sees of len.
-__device__ __forceinline__ int visible(int causal, int len, int n, int j) {
-  return causal ? max(0, len - n + 1 + j) : len;
 }
 
 // Units whose logits a thread holds at once: two give twice the independent
@@ -695,6 +633,10 @@ __global__ void __launch_bounds__(128) attend_join_kernel(Layout L, Step S, Spli
   store_dt(a.out, at + 3, acc.w * inv, a.dtype);
 }
 
+// 16-bit queries with more columns than this go to the kernel for many queries.
+constexpr int kFewColumns = 32;
+bool many(int64_t cols, int dtype) { return dtype != KVC_F32 && cols > kFewColumns; }
+
 // Tiles of 8 columns a block takes: as many as there are, up to what the
 // registers hold (4 with one float16 term and one group a head, else 2).
 int tiles_of(int cols, int terms, int groups) { return cols <= 8 ? 1 : cols <= 16 || terms == 2 || groups > 1 ? 2 : 4; }
@@ -741,6 +683,11 @@ extern "C" int kvc_kv4_attend_shape(const kvc_kv4_layout* layout, const kvc_kv4_
   if (n_q < 1 || n_q % layout->n_kv) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend_shape: n_q must be a multiple of n_kv");
   const int64_t cols = std::max<int64_t>(1, (int64_t)step->max_new * (n_q / layout->n_kv));
   if (cols > INT32_MAX / 2) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend_shape: too many queries");
+  if (many(cols, dtype)) {
+    *tiles = (int)prefill_tiles(cols);
+    *resident = num_sms();
+    return KVC_OK;
+  }
   const int terms = dtype == KVC_F32 ? 2 : 1, nt = tiles_of((int)cols, terms, layout->head_dim / layout->group_size);
   *tiles = (int)ceil_div(cols, 8 * nt);
   int blocks = 0;
@@ -773,7 +720,7 @@ extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* 
   if (step->n_tokens == 0 || split->n_items == 0) return KVC_OK;
   if (!split->items || !aligned16(split->items)) return fail(KVC_ERR_ALIGN, "kvc_kv4_attend: items not 16-byte aligned");
   if (step->n_tokens < 0 || step->n_tokens > INT32_MAX || step->max_new < 1 || split->n_items < 0 ||
-      split->n_items > INT32_MAX || split->chunk < 64 || split->chunk % 64)
+      split->n_items > INT32_MAX || split->chunk < 128 || split->chunk % 128)
     return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: bad step or split sizes");
   const int64_t cols = (int64_t)step->max_new * (n_q / layout->n_kv);
   if (cols > INT32_MAX / 2) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: too many queries");
@@ -789,9 +736,13 @@ extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* 
   const Layout L = to_layout(layout);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc = KVC_OK;
+  if (many(cols, dtype)) {
+    rc = launch_prefill(layout, s, p, static_cast<const uint8_t*>(pool), a, part, split->n_items, st);
+  } else {
 #define KVC_F(D, WPG) rc = launch_tiles<D, WPG>(L, s, p, pool, a, part, split->n_items, (int)cols, st)
-  KVC_KV4_DISPATCH(layout, KVC_F);
+    KVC_KV4_DISPATCH(layout, KVC_F);
 #undef KVC_F
+  }
   if (rc || split->max_items <= 1) return rc;
   const dim3 grid((unsigned)step->n_tokens, (unsigned)n_q);
   return layout->head_dim == 64 ? launch_after("attend_join_kernel", attend_join_kernel<64>, grid, 128, 0, st, L, s, p, a, part)

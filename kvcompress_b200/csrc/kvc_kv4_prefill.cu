@@ -1,0 +1,531 @@
+// Attention over the pages of the 4-bit KV cache, for many queries (a prompt's
+// chunk, or queries over a stored context): 16-bit queries, tcgen05.
+//
+// A block takes up to 256 rows of one sequence and KV head (a row is a query
+// and a head of the KV head's group: they share K and V) as two tiles of 128,
+// and the tokens of one item in tiles of 128.  With many rows to a token it
+// pays to dequantise once into shared memory, K and V rounded to float16 (their
+// values are at most 65119), and to feed both products from there:
+//   S = Q K^T    A, B in shared memory, M = N = 128, K = d
+//   O += P V     A = P in TMEM (over the first half of S), B = V^T, N = d
+// Roles: warps 0-3 and 4-7 hold the softmax of one row tile each (a thread a
+// row: no exchanges), warps 8-11 dequantise, one thread of warp 12 issues the
+// products, warp 13 the bulk copies of the codes.  While one tile's softmax
+// runs, the tensor cores work on the other's.
+//
+// V lies in the cache as pairs of tokens of a feature, so V^T's rows (tokens
+// contiguous) are written without a transposition; K's features lie in the
+// order that its nibbles come out (1 5 0 4 3 7 2 6 of each eight), and Q's are
+// put into the same order.
+//
+// The running maximum is a reference that is only raised when a row's logits
+// exceed it by 2^4; only then O (in TMEM) is rescaled, by the softmax threads.
+// Weights are held 2^7 fold in float16, which leaves 2^-21 of a row's largest
+// for normal numbers.  A masked token's weight is 0, but its value may be NaN:
+// such values are written as 0 and their tokens flagged, and a row that does see
+// a flagged token gets NaN in that group at the end.
+#include <type_traits>
+
+#include "kvc_kv4_attend.cuh"
+
+namespace kvc {
+
+namespace kv4 {
+
+int prefill_read_device_error(int* out) {
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, tc::g_kvc_device_error, sizeof(int));
+  if (e != cudaSuccess) return fail(KVC_ERR_LAUNCH, std::string("device error read: ") + cudaGetErrorString(e));
+  *out = v;
+  int zero = 0;
+  cudaMemcpyToSymbol(tc::g_kvc_device_error, &zero, sizeof(int));
+  return KVC_OK;
+}
+
+namespace {
+
+using namespace kvc::tc;
+
+constexpr int kTile = 128;      // rows of a row tile, tokens of a token tile
+constexpr int kThreads = 14 * 32;
+constexpr float kShift = 7.0f;  // weights are 2^7 fold
+
+template <int D, int WPG>
+struct Pre {
+  static constexpr int W = D / 32, NG = W / WPG, UB = unit_bytes(D, NG), UNITS = kTile / kUnit;
+  static constexpr int TILE = kTile * D * 2;  // bytes of a Q, K or V tile
+  static constexpr int RAW = UNITS * UB;
+  static constexpr int RAWS = 6 * TILE + 2 * RAW + 1024 <= 227 * 1024 ? 2 : 1;  // tiles of codes in flight
+  static constexpr int FLAGS = 4;  // a tile's flags outlive its codes until both softmax tiles are past it
+  static constexpr int q = 0, k = 2 * TILE, v = 4 * TILE, raw = 6 * TILE, flags = raw + RAWS * RAW;
+  static constexpr int bars = flags + FLAGS * NG * 16;
+  // barriers
+  static constexpr int q_full = 0, raw_full = 2, raw_empty = raw_full + RAWS, k_full = raw_empty + RAWS,
+                       v_full = k_full + 2, k_empty = v_full + 2, v_empty = k_empty + 2, s_full = v_empty + 2,
+                       p_full = s_full + 2, o_done = p_full + 2, n_bars = o_done + 2;
+  static constexpr int holder = bars + n_bars * 8, bytes = holder + 16;
+  static_assert(bytes <= 227 * 1024, "shared memory");
+};
+
+// A pair of codes as float16 c - 8: nibble 0 of each half from 1024 + c, nibble
+// 1 from 1024 + 16 c.  Both steps are exact.
+__device__ __forceinline__ __half2 centred_lo(uint32_t w) {
+  uint32_t x = (w & 0x000F000Fu) | 0x64006400u, off = 0x64086408u;  // 1032
+  __half2 h, o;
+  memcpy(&h, &x, 4);
+  memcpy(&o, &off, 4);
+  return __hsub2(h, o);
+}
+__device__ __forceinline__ __half2 centred_hi(uint32_t w) {
+  uint32_t x = (w & 0x00F000F0u) | 0x64006400u, scale = 0x2C002C00u, off = 0xD480D480u;  // 1 / 16, -72
+  __half2 h, s, o;
+  memcpy(&h, &x, 4);
+  memcpy(&s, &scale, 4);
+  memcpy(&o, &off, 4);
+  return __hfma2(h, s, o);
+}
+__device__ __forceinline__ uint32_t bits(__half2 h) {
+  uint32_t r;
+  memcpy(&r, &h, 4);
+  return r;
+}
+__device__ __forceinline__ __half2 half2_of(uint32_t r) {
+  __half2 h;
+  memcpy(&h, &r, 4);
+  return h;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t r;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ bool is_nan(uint32_t half_bits) { return (half_bits & 0x7FFFu) > 0x7C00u; }
+
+template <typename T, int D, int WPG>
+__global__ void __launch_bounds__(kThreads, 1)
+    prefill_kernel(Layout L, Step S, Split P, const uint8_t* __restrict__ pool, Qkv a, Partial part, int q_vec, int o_vec) {
+  using C = Pre<D, WPG>;
+  constexpr int W = C::W, NG = C::NG;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  grid_wait();
+  grid_go();
+  const int4 it = P.items[blockIdx.z];
+  const int b = it.x, t_begin = it.y, len = it.w, h = blockIdx.y;
+  const int q0 = S.q_start[b], n = S.q_start[b + 1] - q0, group = a.n_q / L.n_kv, rows = n * group;
+  // late rows see the most tokens: they go first
+  const int tiles = (rows + 2 * kTile - 1) / (2 * kTile), tile = tiles - 1 - (int)blockIdx.x;
+  if (tile < 0) return;
+  const int row0 = tile * 2 * kTile, last = min(row0 + 2 * kTile, rows) - 1;
+  const int t_end = min(t_begin + P.chunk, visible(a.causal, len, n, last / group));
+  if (t_begin > 0 && t_begin >= t_end) return;  // nothing of this item is seen: the join knows
+  const int steps = t_end > t_begin ? (t_end - t_begin + kTile - 1) / kTile : 0;
+  const int halves = row0 + kTile < rows ? 2 : 1;  // row tiles with rows
+
+  const uint32_t base = smem_u32(smem);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::bars);
+  uint32_t* holder = reinterpret_cast<uint32_t*>(smem + C::holder);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::n_bars; ++i) {
+      const bool per_unit = i >= C::raw_full && i < C::raw_empty;
+      const bool by_mma = (i >= C::k_empty && i < C::p_full) || i >= C::o_done;
+      mbar_init(&bars[i], per_unit ? C::UNITS : by_mma ? 1 : kTile);
+    }
+    mbar_fence_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(holder, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *holder;
+
+  if (warp < 8) {
+    // ---- softmax: a thread a row
+    const int half = warp >> 2, i = threadIdx.x & (kTile - 1), row = row0 + half * kTile + i;
+    if (half < halves) {
+      const bool valid = row < rows;
+      const int j = min(row, rows - 1) / group, g0 = min(row, rows - 1) % group;
+      const int vis = visible(a.causal, len, n, j);
+      const int t_free = visible(a.causal, len, n, (row0 + half * kTile) / group);  // every row of the tile sees them
+      float fac;
+      {  // the row of Q, a power of two and maybe a sign off, in K's order of features
+        const T* src = static_cast<const T*>(a.q) + (a.packed ? (int64_t)(q0 + j) * a.q_st : b * a.q_sb + j * a.q_st) +
+                       (int64_t)(h * group + g0) * a.q_sh;
+        uint4 x[D / 8];
+#pragma unroll
+        for (int w = 0; w < D / 8; ++w) {
+          x[w] = make_uint4(0, 0, 0, 0);
+          if (valid && q_vec) {
+            x[w] = __ldg(reinterpret_cast<const uint4*>(src) + w);
+          } else if (valid) {
+            T e[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) e[k] = src[8 * w + k];
+            memcpy(&x[w], e, 16);
+          }
+        }
+        float top = 0.0f;
+#pragma unroll
+        for (int w = 0; w < D / 8; ++w) {
+          T e[8];
+          memcpy(e, &x[w], 16);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(Elt<T>::to_f32(e[k])));
+        }
+        const int k2 = min(100, max(-100, 13 + 127 - (int)(__float_as_uint(top) >> 23)));
+        const float up = __uint_as_float((uint32_t)(127 + k2) << 23), sign = a.scale < 0.0f ? -up : up;
+        fac = __uint_as_float((uint32_t)(127 - k2) << 23) * fabsf(a.scale) * kLog2e;
+        const uint32_t qt = base + C::q + half * C::TILE;
+#pragma unroll
+        for (int w = 0; w < D / 8; ++w) {
+          T e[8];
+          memcpy(e, &x[w], 16);
+          float f[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) f[k] = Elt<T>::to_f32(e[k]) * sign;
+          sts128(qt + sw128_off(i, 8 * w, kTile), pack_half2(f[1], f[5]), pack_half2(f[0], f[4]), pack_half2(f[3], f[7]),
+                 pack_half2(f[2], f[6]));
+        }
+        fence_async_smem();
+        mbar_arrive(&bars[C::q_full + half]);
+      }
+      const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 TMEM lanes
+      const uint32_t ts = tmem + lanes + half * kTile, to = tmem + lanes + 2 * kTile + half * D;
+      float mf = -INFINITY, mt = -INFINITY;
+      uint64_t l2 = f2_pack(0.0f, 0.0f);
+      uint32_t poison = 0;
+      bool ok = true;
+
+      auto absorb = [&](int step, auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
+        const int seen = vis - (t_begin + step * kTile);  // columns below it are seen
+        float top = -INFINITY;
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {
+          float s[32];
+          tmem_ld32(ts + ch * 32, s);
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            if (MASKED) {
+              if (ch * 32 + k >= seen) s[k] = -INFINITY;
+              if (ch * 32 + k + 1 >= seen) s[k + 1] = -INFINITY;
+            }
+            top = fmaxf(top, fmaxf(s[k], s[k + 1]));
+          }
+        }
+        const bool raise = top > mt;
+        if (__any_sync(0xffffffffu, raise)) {
+          float f = 1.0f;
+          if (raise) {
+            const float m2 = top * fac - kShift;
+            f = ex2(mf - m2);
+            mf = m2;
+            mt = top + (fac > 0.0f ? kRaise / fac : 1.0e38f);
+          }
+          l2 = f2_mul(l2, f2_pack(f, f));
+          if (step > 0) {
+            ok = ok && mbar_wait(&bars[C::o_done + half], (step - 1) & 1, 410);
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+#pragma unroll
+            for (int ch = 0; ch < D / 32; ++ch) {
+              float o[32];
+              uint32_t r[32];
+              tmem_ld32(to + ch * 32, o);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(o[k] * f);
+              tmem_st32(to + ch * 32, r);
+            }
+          }
+        }
+        const uint64_t fac2 = f2_pack(fac, fac), off2 = f2_pack(-mf, -mf);
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {  // 64 tokens: 32 registers of P over columns of S that have been read
+          uint32_t p[32];
+#pragma unroll
+          for (int ch = 0; ch < 2; ++ch) {
+            float s[32];
+            tmem_ld32(ts + hf * 64 + ch * 32, s);
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) {
+              float x, y;
+              f2_unpack(f2_fma(f2_pack(s[k], s[k + 1]), fac2, off2), x, y);
+              x = ex2(x);
+              y = ex2(y);
+              if (MASKED) {
+                if (hf * 64 + ch * 32 + k >= seen) x = 0.0f;
+                if (hf * 64 + ch * 32 + k + 1 >= seen) y = 0.0f;
+              }
+              l2 = f2_add(l2, f2_pack(x, y));
+              p[ch * 16 + k / 2] = pack_half2(x, y);
+            }
+          }
+          tmem_st32(ts + hf * 32, p);
+        }
+        // values that are NaN were written as 0: remember the rows that see them
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          uint32_t fl[4];
+          lds_words<4>(base + C::flags + ((step % C::FLAGS) * NG + g) * 16, fl);
+          if (fl[0] | fl[1] | fl[2] | fl[3]) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int m = seen - 32 * k;
+              if (m > 0 && (fl[k] & (m >= 32 ? 0xFFFFFFFFu : (1u << m) - 1u))) poison |= 1u << g;
+            }
+          }
+        }
+      };
+
+      for (int step = 0; step < steps; ++step) {
+        // (the flags of these tokens were written before K's barrier, which the
+        // issuing thread waited for before it issued S)
+        ok = ok && mbar_wait(&bars[C::s_full + half], step & 1, 411);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tc_fence_after();
+        if (t_begin + (step + 1) * kTile <= t_free) absorb(step, std::false_type{});
+        else absorb(step, std::true_type{});
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bars[C::p_full + half]);
+      }
+
+      // ---- the row's result
+      float l, l1;
+      f2_unpack(l2, l, l1);
+      l += l1;
+      if (steps > 0) ok = ok && mbar_wait(&bars[C::o_done + half], (steps - 1) & 1, 413);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      const bool alone = P.item_start[b + 1] - P.item_start[b] == 1;
+      const float inv = l == 0.0f ? 0.0f : alone ? 1.0f / l : 1.0f;
+      const int64_t at = alone ? (a.packed ? (int64_t)(q0 + j) * a.o_st : b * a.o_sb + j * a.o_st) + (int64_t)(h * group + g0) * a.o_sh
+                               : (((int64_t)blockIdx.z * L.n_kv + h) * part.cols + row) * D;
+#pragma unroll
+      for (int ch = 0; ch < D / 32; ++ch) {
+        float o[32];
+        __syncwarp();
+        if (steps > 0) tmem_ld32(to + ch * 32, o);
+        const bool bad = (poison >> (ch / WPG)) & 1;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) o[k] = bad ? __uint_as_float(0x7FC00000u) : l == 0.0f ? 0.0f : o[k] * inv;
+        if (valid && alone && o_vec) {
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at + ch * 32);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            T e[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) e[x] = Elt<T>::from(o[8 * k + x]);
+            uint4 y;
+            memcpy(&y, e, 16);
+            dst[k] = y;
+          }
+        } else if (valid && alone) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) static_cast<T*>(a.out)[at + ch * 32 + k] = Elt<T>::from(o[k]);
+        } else if (valid) {
+          float4* dst = reinterpret_cast<float4*>(part.o + at + ch * 32);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+        }
+      }
+      if (valid && !alone) part.ml[at / D] = make_float2(mf, l);
+      tc_fence_before();
+    }
+  } else if (warp < 12) {
+    // ---- dequantise: 128 threads
+    const int i = threadIdx.x - 8 * 32, w4 = warp - 8;
+    bool ok = true;
+    for (int step = 0; step < steps; ++step) {
+      const int rs = step % C::RAWS, buf = step & 1, t0 = t_begin + step * kTile;
+      const uint32_t raw = base + C::raw + rs * C::RAW;
+      ok = mbar_wait(&bars[C::raw_full + rs], (step / C::RAWS) & 1, 420);
+      if (ok && step >= 2) ok = mbar_wait(&bars[C::k_empty + buf], ((step >> 1) + 1) & 1, 421);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      // flags: token i's value parameters
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const uint32_t p = lds32(raw + (i >> 4) * C::UB + vp_base(D, NG) + ((i & 15) * NG + g) * 4);
+        const uint32_t fl = __ballot_sync(0xffffffffu, (is_nan(p) || is_nan(p >> 16)) && t0 + i < t_end);
+        if (lane == 0)
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + C::flags + ((step % C::FLAGS) * NG + g) * 16 + w4 * 4), "r"(fl)
+                       : "memory");
+      }
+      // K: four (token, chunk) a thread.  Eight lanes of a store hold tokens t and
+      // t + 4, whose swizzles differ: no two meet a bank
+      const uint32_t kt = base + C::k + buf * C::TILE;
+#pragma unroll
+      for (int rep = 0; rep < 4; ++rep) {
+        const int c = lane & 3, t = rep * 32 + w4 * 8 + ((lane >> 2) & 1) * 4 + (lane >> 3);
+        const uint32_t unit = raw + (t >> 4) * C::UB;
+        uint32_t x[W];
+        lds_words<W>(unit + k_chunk<D>(t & 15, c), x);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const __half2 sz = half2_of(lds32(unit + kp_base(D) + ((t & 15) * NG + w / WPG) * 4));
+          const __half2 s2 = __low2half2(sz), z2 = __high2half2(sz);
+          const uint32_t y = x[w] >> 8;
+          sts128(kt + sw128_off(t, 32 * w + 8 * c, kTile), bits(__hfma2(centred_lo(x[w]), s2, z2)),
+                 bits(__hfma2(centred_hi(x[w]), s2, z2)), bits(__hfma2(centred_lo(y), s2, z2)),
+                 bits(__hfma2(centred_hi(y), s2, z2)));
+        }
+      }
+      fence_async_smem();
+      mbar_arrive(&bars[C::k_full + buf]);
+      // V^T: eight tokens (16-byte chunk q8 of a row) of the features 32 u + 4 r + 0..3
+      if (step >= 2) ok = mbar_wait(&bars[C::v_empty + buf], ((step >> 1) + 1) & 1, 422);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const uint32_t vt = base + C::v + buf * C::TILE;
+      const int q8 = (lane & 3) | ((lane >> 3) << 2), r = ((lane >> 2) & 1) | (w4 << 1);
+      const uint32_t unit = raw + (q8 >> 1) * C::UB;
+      uint32_t x[4][W];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) lds_words<W>(unit + v_chunk<D>(q8 & 1, r * 4 + c), x[c]);
+      __half2 s2[4], z2[4];
+#pragma unroll
+      for (int u = 0; u < W; ++u) {
+        if (u % WPG == 0) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t p[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int t = (q8 & 1) * 8 + 2 * c + k;
+              p[k] = lds32(unit + vp_base(D, NG) + (t * NG + u / WPG) * 4);
+              if (is_nan(p[k]) || is_nan(p[k] >> 16) || t0 + (q8 >> 1) * 16 + t >= t_end) p[k] = 0;
+            }
+            s2[c] = __lows2half2(half2_of(p[0]), half2_of(p[1]));
+            z2[c] = __highs2half2(half2_of(p[0]), half2_of(p[1]));
+          }
+        }
+        // nibbles 0..3 are features 1, 0, 3, 2
+        uint32_t o[4][4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t y = x[c][u] >> 8;
+          o[1][c] = bits(__hfma2(centred_lo(x[c][u]), s2[c], z2[c]));
+          o[0][c] = bits(__hfma2(centred_hi(x[c][u]), s2[c], z2[c]));
+          o[3][c] = bits(__hfma2(centred_lo(y), s2[c], z2[c]));
+          o[2][c] = bits(__hfma2(centred_hi(y), s2[c], z2[c]));
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          sts128(vt + sw128_off(32 * u + 4 * r + k, 8 * q8, D), o[k][0], o[k][1], o[k][2], o[k][3]);
+      }
+      mbar_arrive(&bars[C::raw_empty + rs]);
+      fence_async_smem();
+      mbar_arrive(&bars[C::v_full + buf]);
+    }
+  } else if (warp == 12) {
+    // ---- issue the products
+    if (lane == 0 && steps > 0) {
+      constexpr uint32_t id_s = idesc_f16(kTile, kTile, false), id_o = idesc_f16(kTile, D, false);
+      bool ok = true;
+      auto scores = [&](int half, int step) {
+        const uint32_t qa = base + C::q + half * C::TILE, kb = base + C::k + (step & 1) * C::TILE;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = (uint32_t)((ks >> 2) * (kTile * 128) + (ks & 3) * 32);
+          umma_f16(tmem + half * kTile, desc_sw128(qa + off), desc_sw128(kb + off), id_s, ks ? 1u : 0u);
+        }
+        umma_commit(&bars[C::s_full + half]);
+      };
+      for (int half = 0; half < halves; ++half) ok = ok && mbar_wait(&bars[C::q_full + half], 0, 430);
+      ok = ok && mbar_wait(&bars[C::k_full], 0, 431);
+      tc_fence_after();
+      if (ok) {
+        for (int half = 0; half < halves; ++half) scores(half, 0);
+        if (steps > 2) umma_commit(&bars[C::k_empty]);
+      }
+      for (int step = 0; ok && step < steps; ++step) {
+        ok = mbar_wait(&bars[C::v_full + (step & 1)], (step >> 1) & 1, 432);
+        if (ok && step + 1 < steps) ok = mbar_wait(&bars[C::k_full + ((step + 1) & 1)], ((step + 1) >> 1) & 1, 433);
+        for (int half = 0; ok && half < halves; ++half) {
+          ok = mbar_wait(&bars[C::p_full + half], step & 1, 434);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t vb = base + C::v + (step & 1) * C::TILE;
+#pragma unroll
+          for (int ks = 0; ks < kTile / 16; ++ks)
+            umma_f16_ts(tmem + 2 * kTile + half * D, tmem + half * kTile + ks * 8,
+                        desc_sw128(vb + (uint32_t)((ks >> 2) * (D * 128) + (ks & 3) * 32)), id_o, step || ks ? 1u : 0u);
+          umma_commit(&bars[C::o_done + half]);
+          if (step + 1 < steps) scores(half, step + 1);
+        }
+        if (!ok) break;
+        // only where somebody waits: none may be on its way when the block ends
+        if (step + 2 < steps) umma_commit(&bars[C::v_empty + (step & 1)]);
+        if (step + 3 < steps) umma_commit(&bars[C::k_empty + ((step + 1) & 1)]);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- bring the codes: lane u copies unit u of each tile
+    bool ok = true;
+    auto page = [&](int step) -> const uint8_t* {
+      const int t = t_begin + step * kTile + lane * kUnit;
+      if (lane >= C::UNITS || step >= steps || t >= t_end) return nullptr;
+      const int64_t p = page_of(L, it.z, t, &g_kvc_device_error);
+      return pool + unit_off<D>(L, p < 0 ? 0 : p, h, t);  // a bad entry reads page 0: wrong, but in range
+    };
+    const uint8_t* src = page(0);
+    for (int step = 0; step < steps; ++step) {
+      const uint8_t* next = page(step + 1);
+      const int rs = step % C::RAWS;
+      if (step >= C::RAWS) ok = mbar_wait(&bars[C::raw_empty + rs], (step / C::RAWS + 1) & 1, 440);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      if (lane < C::UNITS) {
+        if (src) {
+          mbar_expect_tx(&bars[C::raw_full + rs], C::UB);
+          bulk_load(base + C::raw + rs * C::RAW + lane * C::UB, src, C::UB, &bars[C::raw_full + rs]);
+        } else {
+          mbar_arrive(&bars[C::raw_full + rs]);
+        }
+      }
+      src = next;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int D, int WPG>
+int launch(const Layout& L, const Step& S, const Split& P, const uint8_t* pool, const Qkv& a, const Partial& part,
+           const dim3& grid, cudaStream_t st) {
+  using C = Pre<D, WPG>;
+  auto kernel = prefill_kernel<T, D, WPG>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::bytes);
+  if (e != cudaSuccess) return fail(KVC_ERR_LAUNCH, std::string("prefill_kernel: ") + cudaGetErrorString(e));
+  const int q_vec = aligned16(a.q) && ((a.q_sb | a.q_st | a.q_sh) & 7) == 0;
+  const int o_vec = aligned16(a.out) && ((a.o_sb | a.o_st | a.o_sh) & 7) == 0;
+  return launch_after("prefill_kernel", kernel, grid, kThreads, C::bytes, st, L, S, P, pool, a, part, q_vec, o_vec);
+}
+
+}  // namespace
+
+int launch_prefill(const kvc_kv4_layout* l, const Step& S, const Split& P, const uint8_t* pool, const Qkv& a,
+                   const Partial& part, int64_t n_items, cudaStream_t st) {
+  const Layout L = to_layout(l);
+  const int64_t tiles = prefill_tiles(part.cols);
+  if (n_items > 65535 || L.n_kv > 65535 || tiles > INT32_MAX)
+    return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: too many queries, items or KV heads");
+  const dim3 grid((unsigned)tiles, (unsigned)L.n_kv, (unsigned)n_items);
+  int rc = KVC_OK;
+#define KVC_F(D, WPG)                                                                             \
+  rc = a.dtype == KVC_F16 ? launch<__half, D, WPG>(L, S, P, pool, a, part, grid, st)              \
+                          : launch<__nv_bfloat16, D, WPG>(L, S, P, pool, a, part, grid, st)
+  KVC_KV4_DISPATCH(l, KVC_F);
+#undef KVC_F
+  return rc;
+}
+
+}  // namespace kv4
+}  // namespace kvc

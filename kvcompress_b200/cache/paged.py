@@ -72,27 +72,25 @@ def _prefix(counts: np.ndarray) -> np.ndarray:
     return out
 
 
-def split_chunk(lengths: np.ndarray, copies: int, slots: int) -> int:
+def split_chunk(lengths: np.ndarray, copies: int, slots: int, joined: int = 0) -> int:
     """Tokens of an item so that ``copies`` CTAs an item fill ``slots`` resident
-    CTAs evenly: of one to four full waves (or no split at all) the choice with
-    the least waves x (tokens + a CTA's fixed cost in tokens)."""
+    CTAs evenly: of one to four full waves (or no split at all) the choice that
+    costs least.  In tokens of a CTA (about 20 ns each): a wave costs its item and
+    192 for a CTA's start and end, joining 200 and a token for every 100 kB of
+    partial results (``joined`` bytes an item of every sequence)."""
     longest = int(lengths.max(initial=1))
     total = max(1, int(lengths.sum()))
     best, cost = 0, float("inf")
-    for waves in (1, 2, 3, 4, 0):
-        chunk = _CHUNK
-        if waves == 0:
-            chunk = longest
-        else:
-            chunk = max(_CHUNK, -(-total * copies // (waves * slots)))
+    for waves in (0, 1, 2, 3, 4):
+        chunk = longest if waves == 0 else max(_CHUNK, -(-total * copies // (waves * slots)))
         chunk = -(-chunk // 128) * 128
-        while waves and chunk < longest:
-            items = int(np.maximum(1, -(-lengths // chunk)).sum()) * copies
-            if items <= waves * slots:
-                break
+        items = int(np.maximum(1, -(-lengths // chunk)).sum())
+        while waves and chunk < longest and items * copies > waves * slots:
             chunk += max(128, chunk // 64 // 128 * 128)
-        items = int(np.maximum(1, -(-lengths // chunk)).sum()) * copies
-        c = -(-items // slots) * (min(chunk, longest) + 192)
+            items = int(np.maximum(1, -(-lengths // chunk)).sum())
+        c = -(-items * copies // slots) * (min(chunk, longest) + 192)
+        if items > lengths.size:
+            c += 200 + joined * items / lengths.size * 1e-5
         if c < cost:
             best, cost = chunk, c
     return best
@@ -225,7 +223,7 @@ class PagedKVCache:
         if got is None:
             lengths = np.array(step.lengths, dtype=np.int64)
             tiles, resident = ops.kv4_attend_shape(self._layout, step.desc, n_q, code, self.device)
-            chunk = split_chunk(lengths, self.n_kv_heads * tiles, resident)
+            chunk = split_chunk(lengths, self.n_kv_heads * tiles, resident, 8 * step.tokens * n_q * (self.head_dim + 2))
             items = np.maximum(1, -(-lengths // chunk))
             start = _prefix(items)
             seq = np.repeat(np.arange(len(step.seqs)), items)

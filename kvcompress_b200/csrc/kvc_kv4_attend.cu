@@ -573,17 +573,21 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
   }
 }
 
-// Joins the items of the sequences that have several: a block per query and
-// head.  Group g of D / 4 threads (a float4 of features each) takes items g, g +
-// G, ..., so that eight loads a thread are on their way at once; the groups are
+// Joins the items of the sequences that have several.  D / 4 threads, a float4
+// of features each, take a row's (a query and head's) items in turn, up to eight
+// loads at once.  With few items a block of 128 threads holds G = 512 / D rows;
+// with many it holds one, group g taking items g, g + G, ..., and the groups are
 // added in their order.
-template <int D>
-__global__ void __launch_bounds__(128) attend_join_kernel(Layout L, Step S, Split P, Qkv a, Partial part) {
-  constexpr int T = D / 4, G = 128 / T;
+template <int D, bool WIDE>
+__global__ void __launch_bounds__(128) attend_join_kernel(Layout L, Step S, Split P, Qkv a, Partial part, int64_t rows) {
+  constexpr int T = D / 4, G = 128 / T, STEP = WIDE ? G : 1;
   __shared__ float4 so[G][T];
   __shared__ float ss[G];
   grid_wait();
-  const int lane = threadIdx.x & 31, g = threadIdx.x / T, x = threadIdx.x % T, tok = blockIdx.x, head = blockIdx.y;
+  const int g = threadIdx.x / T, x = threadIdx.x % T;
+  const int64_t id = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * G + g;
+  if (id >= rows) return;
+  const int tok = (int)(id / a.n_q), head = (int)(id % a.n_q);
   const int b = seq_of(S, tok), i0 = P.item_start[b], i1 = P.item_start[b + 1];
   if (i1 - i0 == 1) return;
   const int q0 = S.q_start[b], n = S.q_start[b + 1] - q0, j = tok - q0, group = a.n_q / L.n_kv;
@@ -592,38 +596,40 @@ __global__ void __launch_bounds__(128) attend_join_kernel(Layout L, Step S, Spli
   const int items = max(1, min(i1 - i0, (vis + P.chunk - 1) / P.chunk));
   const int64_t at0 = ((int64_t)i0 * L.n_kv + h) * part.cols + j * group + head % group, step = L.n_kv * part.cols;
   float top = -INFINITY;
-  for (int i = lane; i < items; i += 32) top = fmaxf(top, part.ml[at0 + i * step].x);
+  for (int i = x; i < items; i += T) top = fmaxf(top, part.ml[at0 + i * step].x);
 #pragma unroll
-  for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+  for (int k = T / 2; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(T == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16), top, k));
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float sum = 0.0f;
-  for (int i = g; i < items; i += 8 * G) {
+  for (int i = WIDE ? g : 0; i < items; i += 8 * STEP) {
     float4 v[8];
     float2 ml[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-      if (i + u * G < items) {
-        v[u] = *reinterpret_cast<const float4*>(part.o + (at0 + (i + u * G) * step) * D + x * 4);
-        ml[u] = part.ml[at0 + (i + u * G) * step];
+      if (i + u * STEP < items) {
+        v[u] = *reinterpret_cast<const float4*>(part.o + (at0 + (i + u * STEP) * step) * D + x * 4);
+        ml[u] = part.ml[at0 + (i + u * STEP) * step];
       }
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-      if (i + u * G < items && ml[u].y != 0.0f) {  // 0: saw nothing
+      if (i + u * STEP < items && ml[u].y != 0.0f) {  // 0: saw nothing
         const float f = ex2(ml[u].x - top);
         sum = fmaf(ml[u].y, f, sum);
         acc.x = fmaf(v[u].x, f, acc.x), acc.y = fmaf(v[u].y, f, acc.y);
         acc.z = fmaf(v[u].z, f, acc.z), acc.w = fmaf(v[u].w, f, acc.w);
       }
   }
-  so[g][x] = acc;
-  if (x == 0) ss[g] = sum;
-  __syncthreads();
-  if (g) return;
+  if constexpr (WIDE) {
+    so[g][x] = acc;
+    if (x == 0) ss[g] = sum;
+    __syncthreads();
+    if (g) return;
 #pragma unroll
-  for (int k = 1; k < G; ++k) {
-    const float4 v = so[k][x];
-    acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-    sum += ss[k];
+    for (int k = 1; k < G; ++k) {
+      const float4 v = so[k][x];
+      acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+      sum += ss[k];
+    }
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   const int64_t at = (a.packed ? (int64_t)tok * a.o_st : b * a.o_sb + j * a.o_st) + (int64_t)head * a.o_sh + x * 4;
@@ -631,6 +637,16 @@ __global__ void __launch_bounds__(128) attend_join_kernel(Layout L, Step S, Spli
   store_dt(a.out, at + 1, acc.y * inv, a.dtype);
   store_dt(a.out, at + 2, acc.z * inv, a.dtype);
   store_dt(a.out, at + 3, acc.w * inv, a.dtype);
+}
+
+template <int D>
+int join(const Layout& L, const Step& S, const Split& P, const Qkv& a, const Partial& part, int64_t tokens, cudaStream_t st) {
+  const int64_t rows = tokens * a.n_q;
+  const bool wide = P.max_items > 8;
+  const int64_t blocks = wide ? rows : ceil_div(rows, 512 / D);
+  if (blocks > INT32_MAX) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: too many queries");
+  return wide ? launch_after("attend_join_kernel", attend_join_kernel<D, true>, dim3((unsigned)blocks), 128, 0, st, L, S, P, a, part, rows)
+              : launch_after("attend_join_kernel", attend_join_kernel<D, false>, dim3((unsigned)blocks), 128, 0, st, L, S, P, a, part, rows);
 }
 
 // 16-bit queries with more columns than this go to the kernel for many queries.
@@ -744,7 +760,5 @@ extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* 
 #undef KVC_F
   }
   if (rc || split->max_items <= 1) return rc;
-  const dim3 grid((unsigned)step->n_tokens, (unsigned)n_q);
-  return layout->head_dim == 64 ? launch_after("attend_join_kernel", attend_join_kernel<64>, grid, 128, 0, st, L, s, p, a, part)
-                                : launch_after("attend_join_kernel", attend_join_kernel<128>, grid, 128, 0, st, L, s, p, a, part);
+  return layout->head_dim == 64 ? join<64>(L, s, p, a, part, step->n_tokens, st) : join<128>(L, s, p, a, part, step->n_tokens, st);
 }

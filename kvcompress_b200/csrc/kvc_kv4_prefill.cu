@@ -10,8 +10,9 @@
 //   O += P V     A = P in TMEM (over the first half of S), B = V^T, N = d
 // Roles: warps 0-3 and 4-7 hold the softmax of one row tile each (a thread a
 // row: no exchanges), warps 8-11 dequantise, one thread of warp 12 issues the
-// products, warp 13 the bulk copies of the codes.  While one tile's softmax
-// runs, the tensor cores work on the other's.
+// products, warp 13 the bulk copies of the codes (14 and 15 only give up their
+// registers: a softmax thread holds its row's 128 logits).  While one tile's
+// softmax runs, the tensor cores work on the other's.
 //
 // V lies in the cache as pairs of tokens of a feature, so V^T's rows (tokens
 // contiguous) are written without a transposition; K's features lie in the
@@ -24,8 +25,6 @@
 // for normal numbers.  A masked token's weight is 0, but its value may be NaN:
 // such values are written as 0 and their tokens flagged, and a row that does see
 // a flagged token gets NaN in that group at the end.
-#include <type_traits>
-
 #include "kvc_kv4_attend.cuh"
 
 namespace kvc {
@@ -47,7 +46,7 @@ namespace {
 using namespace kvc::tc;
 
 constexpr int kTile = 128;      // rows of a row tile, tokens of a token tile
-constexpr int kThreads = 14 * 32;
+constexpr int kThreads = 16 * 32;
 constexpr float kShift = 7.0f;  // weights are 2^7 fold
 
 template <int D, int WPG>
@@ -102,6 +101,56 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// 32 columns of this thread's row, not waited for; tmem_arrived() is the wait,
+// and no use of r may move before it.
+__device__ __forceinline__ void tmem_fetch32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_arrived(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ bool is_nan(uint32_t half_bits) { return (half_bits & 0x7FFFu) > 0x7C00u; }
 
 template <typename T, int D, int WPG>
@@ -145,8 +194,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *holder;
 
+  // registers: 8 x 192 + 4 x 88 + 4 x 40 a lane = 16 x 128, what the block was launched with
   if (warp < 8) {
     // ---- softmax: a thread a row
+    more_registers<192>();
     const int half = warp >> 2, i = threadIdx.x & (kTile - 1), row = row0 + half * kTile + i;
     if (half < halves) {
       const bool valid = row < rows;
@@ -180,7 +231,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const int k2 = min(100, max(-100, 13 + 127 - (int)(__float_as_uint(top) >> 23)));
         const float up = __uint_as_float((uint32_t)(127 + k2) << 23), sign = a.scale < 0.0f ? -up : up;
-        fac = __uint_as_float((uint32_t)(127 - k2) << 23) * fabsf(a.scale) * kLog2e;
+        // (not 0, so that a masked logit stays -inf: a factor this small makes every weight 1)
+        fac = fmaxf(__uint_as_float((uint32_t)(127 - k2) << 23) * fabsf(a.scale) * kLog2e, 1.0e-30f);
         const uint32_t qt = base + C::q + half * C::TILE;
 #pragma unroll
         for (int w = 0; w < D / 8; ++w) {
@@ -202,23 +254,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t poison = 0;
       bool ok = true;
 
-      auto absorb = [&](int step, auto masked) {
-        constexpr bool MASKED = decltype(masked)::value;
+      for (int step = 0; step < steps; ++step) {
+        // (the flags of these tokens were written before K's barrier, which the
+        // issuing thread waited for before it issued S)
+        ok = ok && mbar_wait(&bars[C::s_full + half], step & 1, 411);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tc_fence_after();
         const int seen = vis - (t_begin + step * kTile);  // columns below it are seen
-        float top = -INFINITY;
+        uint32_t r[4][32];
 #pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
-          float s[32];
-          tmem_ld32(ts + ch * 32, s);
+        for (int ch = 0; ch < 4; ++ch) tmem_fetch32(ts + ch * 32, r[ch]);
 #pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            if (MASKED) {
-              if (ch * 32 + k >= seen) s[k] = -INFINITY;
-              if (ch * 32 + k + 1 >= seen) s[k + 1] = -INFINITY;
-            }
-            top = fmaxf(top, fmaxf(s[k], s[k + 1]));
-          }
+        for (int ch = 0; ch < 4; ++ch) tmem_arrived(r[ch]);
+        if (t_begin + (step + 1) * kTile > t_free) {
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch)
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (ch * 32 + k >= seen) r[ch][k] = 0xFF800000u;  // -inf
         }
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int k = 0; k < 32; k += 2)
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch)
+            tops[ch] = fmaxf(tops[ch], fmaxf(__uint_as_float(r[ch][k]), __uint_as_float(r[ch][k + 1])));
+        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         const bool raise = top > mt;
         if (__any_sync(0xffffffffu, raise)) {
           float f = 1.0f;
@@ -226,45 +287,37 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float m2 = top * fac - kShift;
             f = ex2(mf - m2);
             mf = m2;
-            mt = top + (fac > 0.0f ? kRaise / fac : 1.0e38f);
+            mt = top + kRaise / fac;
           }
           l2 = f2_mul(l2, f2_pack(f, f));
           if (step > 0) {
             ok = ok && mbar_wait(&bars[C::o_done + half], (step - 1) & 1, 410);
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
+#pragma unroll 1
+            for (int ch = 0; ch < D / 16; ++ch) {
+              uint32_t o[16];
+              tmem_ld16(to + ch * 16, o);
 #pragma unroll
-            for (int ch = 0; ch < D / 32; ++ch) {
-              float o[32];
-              uint32_t r[32];
-              tmem_ld32(to + ch * 32, o);
-#pragma unroll
-              for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(o[k] * f);
-              tmem_st32(to + ch * 32, r);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st16(to + ch * 16, o);
             }
           }
         }
-        const uint64_t fac2 = f2_pack(fac, fac), off2 = f2_pack(-mf, -mf);
+        const float off = mf == -INFINITY ? 0.0f : -mf;  // (nothing seen yet: every logit is -inf)
+        const uint64_t fac2 = f2_pack(fac, fac), off2 = f2_pack(off, off);
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {  // 64 tokens: 32 registers of P over columns of S that have been read
+        for (int hf = 0; hf < 2; ++hf) {
           uint32_t p[32];
 #pragma unroll
-          for (int ch = 0; ch < 2; ++ch) {
-            float s[32];
-            tmem_ld32(ts + hf * 64 + ch * 32, s);
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              float x, y;
-              f2_unpack(f2_fma(f2_pack(s[k], s[k + 1]), fac2, off2), x, y);
-              x = ex2(x);
-              y = ex2(y);
-              if (MASKED) {
-                if (hf * 64 + ch * 32 + k >= seen) x = 0.0f;
-                if (hf * 64 + ch * 32 + k + 1 >= seen) y = 0.0f;
-              }
-              l2 = f2_add(l2, f2_pack(x, y));
-              p[ch * 16 + k / 2] = pack_half2(x, y);
-            }
+          for (int k = 0; k < 64; k += 2) {
+            float x, y;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * hf + k / 32][k % 32]), __uint_as_float(r[2 * hf + k / 32][k % 32 + 1])),
+                             fac2, off2), x, y);
+            x = ex2(x);
+            y = ex2(y);
+            l2 = f2_add(l2, f2_pack(x, y));
+            p[k / 2] = pack_half2(x, y);
           }
           tmem_st32(ts + hf * 32, p);
         }
@@ -281,16 +334,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-      };
-
-      for (int step = 0; step < steps; ++step) {
-        // (the flags of these tokens were written before K's barrier, which the
-        // issuing thread waited for before it issued S)
-        ok = ok && mbar_wait(&bars[C::s_full + half], step & 1, 411);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        tc_fence_after();
-        if (t_begin + (step + 1) * kTile <= t_free) absorb(step, std::false_type{});
-        else absorb(step, std::true_type{});
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&bars[C::p_full + half]);
@@ -340,6 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp < 12) {
     // ---- dequantise: 128 threads
+    fewer_registers<88>();
     const int i = threadIdx.x - 8 * 32, w4 = warp - 8;
     bool ok = true;
     for (int step = 0; step < steps; ++step) {
@@ -422,73 +466,76 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_async_smem();
       mbar_arrive(&bars[C::v_full + buf]);
     }
-  } else if (warp == 12) {
-    // ---- issue the products
-    if (lane == 0 && steps > 0) {
-      constexpr uint32_t id_s = idesc_f16(kTile, kTile, false), id_o = idesc_f16(kTile, D, false);
-      bool ok = true;
-      auto scores = [&](int half, int step) {
-        const uint32_t qa = base + C::q + half * C::TILE, kb = base + C::k + (step & 1) * C::TILE;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (uint32_t)((ks >> 2) * (kTile * 128) + (ks & 3) * 32);
-          umma_f16(tmem + half * kTile, desc_sw128(qa + off), desc_sw128(kb + off), id_s, ks ? 1u : 0u);
-        }
-        umma_commit(&bars[C::s_full + half]);
-      };
-      for (int half = 0; half < halves; ++half) ok = ok && mbar_wait(&bars[C::q_full + half], 0, 430);
-      ok = ok && mbar_wait(&bars[C::k_full], 0, 431);
-      tc_fence_after();
-      if (ok) {
-        for (int half = 0; half < halves; ++half) scores(half, 0);
-        if (steps > 2) umma_commit(&bars[C::k_empty]);
-      }
-      for (int step = 0; ok && step < steps; ++step) {
-        ok = mbar_wait(&bars[C::v_full + (step & 1)], (step >> 1) & 1, 432);
-        if (ok && step + 1 < steps) ok = mbar_wait(&bars[C::k_full + ((step + 1) & 1)], ((step + 1) >> 1) & 1, 433);
-        for (int half = 0; ok && half < halves; ++half) {
-          ok = mbar_wait(&bars[C::p_full + half], step & 1, 434);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t vb = base + C::v + (step & 1) * C::TILE;
-#pragma unroll
-          for (int ks = 0; ks < kTile / 16; ++ks)
-            umma_f16_ts(tmem + 2 * kTile + half * D, tmem + half * kTile + ks * 8,
-                        desc_sw128(vb + (uint32_t)((ks >> 2) * (D * 128) + (ks & 3) * 32)), id_o, step || ks ? 1u : 0u);
-          umma_commit(&bars[C::o_done + half]);
-          if (step + 1 < steps) scores(half, step + 1);
-        }
-        if (!ok) break;
-        // only where somebody waits: none may be on its way when the block ends
-        if (step + 2 < steps) umma_commit(&bars[C::v_empty + (step & 1)]);
-        if (step + 3 < steps) umma_commit(&bars[C::k_empty + ((step + 1) & 1)]);
-      }
-    }
-    __syncwarp();
   } else {
-    // ---- bring the codes: lane u copies unit u of each tile
-    bool ok = true;
-    auto page = [&](int step) -> const uint8_t* {
-      const int t = t_begin + step * kTile + lane * kUnit;
-      if (lane >= C::UNITS || step >= steps || t >= t_end) return nullptr;
-      const int64_t p = page_of(L, it.z, t, &g_kvc_device_error);
-      return pool + unit_off<D>(L, p < 0 ? 0 : p, h, t);  // a bad entry reads page 0: wrong, but in range
-    };
-    const uint8_t* src = page(0);
-    for (int step = 0; step < steps; ++step) {
-      const uint8_t* next = page(step + 1);
-      const int rs = step % C::RAWS;
-      if (step >= C::RAWS) ok = mbar_wait(&bars[C::raw_empty + rs], (step / C::RAWS + 1) & 1, 440);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      if (lane < C::UNITS) {
-        if (src) {
-          mbar_expect_tx(&bars[C::raw_full + rs], C::UB);
-          bulk_load(base + C::raw + rs * C::RAW + lane * C::UB, src, C::UB, &bars[C::raw_full + rs]);
-        } else {
-          mbar_arrive(&bars[C::raw_full + rs]);
+    fewer_registers<40>();
+    if (warp == 12) {
+      // ---- issue the products
+      if (lane == 0 && steps > 0) {
+        constexpr uint32_t id_s = idesc_f16(kTile, kTile, false), id_o = idesc_f16(kTile, D, false);
+        bool ok = true;
+        auto scores = [&](int half, int step) {
+          const uint32_t qa = base + C::q + half * C::TILE, kb = base + C::k + (step & 1) * C::TILE;
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            const uint32_t off = (uint32_t)((ks >> 2) * (kTile * 128) + (ks & 3) * 32);
+            umma_f16(tmem + half * kTile, desc_sw128(qa + off), desc_sw128(kb + off), id_s, ks ? 1u : 0u);
+          }
+          umma_commit(&bars[C::s_full + half]);
+        };
+        for (int half = 0; half < halves; ++half) ok = ok && mbar_wait(&bars[C::q_full + half], 0, 430);
+        ok = ok && mbar_wait(&bars[C::k_full], 0, 431);
+        tc_fence_after();
+        if (ok) {
+          for (int half = 0; half < halves; ++half) scores(half, 0);
+          if (steps > 2) umma_commit(&bars[C::k_empty]);
+        }
+        for (int step = 0; ok && step < steps; ++step) {
+          ok = mbar_wait(&bars[C::v_full + (step & 1)], (step >> 1) & 1, 432);
+          if (ok && step + 1 < steps) ok = mbar_wait(&bars[C::k_full + ((step + 1) & 1)], ((step + 1) >> 1) & 1, 433);
+          for (int half = 0; ok && half < halves; ++half) {
+            ok = mbar_wait(&bars[C::p_full + half], step & 1, 434);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t vb = base + C::v + (step & 1) * C::TILE;
+#pragma unroll
+            for (int ks = 0; ks < kTile / 16; ++ks)
+              umma_f16_ts(tmem + 2 * kTile + half * D, tmem + half * kTile + ks * 8,
+                          desc_sw128(vb + (uint32_t)((ks >> 2) * (D * 128) + (ks & 3) * 32)), id_o, step || ks ? 1u : 0u);
+            umma_commit(&bars[C::o_done + half]);
+            if (step + 1 < steps) scores(half, step + 1);
+          }
+          if (!ok) break;
+          // only where somebody waits: none may be on its way when the block ends
+          if (step + 2 < steps) umma_commit(&bars[C::v_empty + (step & 1)]);
+          if (step + 3 < steps) umma_commit(&bars[C::k_empty + ((step + 1) & 1)]);
         }
       }
-      src = next;
+      __syncwarp();
+    } else if (warp == 13) {
+      // ---- bring the codes: lane u copies unit u of each tile
+      bool ok = true;
+      auto page = [&](int step) -> const uint8_t* {
+        const int t = t_begin + step * kTile + lane * kUnit;
+        if (lane >= C::UNITS || step >= steps || t >= t_end) return nullptr;
+        const int64_t p = page_of(L, it.z, t, &g_kvc_device_error);
+        return pool + unit_off<D>(L, p < 0 ? 0 : p, h, t);  // a bad entry reads page 0: wrong, but in range
+      };
+      const uint8_t* src = page(0);
+      for (int step = 0; step < steps; ++step) {
+        const uint8_t* next = page(step + 1);
+        const int rs = step % C::RAWS;
+        if (step >= C::RAWS) ok = mbar_wait(&bars[C::raw_empty + rs], (step / C::RAWS + 1) & 1, 440);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (lane < C::UNITS) {
+          if (src) {
+            mbar_expect_tx(&bars[C::raw_full + rs], C::UB);
+            bulk_load(base + C::raw + rs * C::RAW + lane * C::UB, src, C::UB, &bars[C::raw_full + rs]);
+          } else {
+            mbar_arrive(&bars[C::raw_full + rs]);
+          }
+        }
+        src = next;
+      }
     }
   }
   tc_fence_before();

@@ -151,8 +151,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-__device__ __forceinline__ bool is_nan(uint32_t half_bits) { return (half_bits & 0x7FFFu) > 0x7C00u; }
-
 template <typename T, int D, int WPG>
 __global__ void __launch_bounds__(kThreads, 1)
     prefill_kernel(Layout L, Step S, Split P, const uint8_t* __restrict__ pool, Qkv a, Partial part, int q_vec, int o_vec) {
@@ -384,83 +382,111 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp < 12) {
     // ---- dequantise: 128 threads
     fewer_registers<88>();
-    const int i = threadIdx.x - 8 * 32, w4 = warp - 8;
+    const int w4 = warp - 8;
     bool ok = true;
+    // K: a thread takes chunk c of four tokens, 32 apart.  Eight lanes of a store
+    // hold tokens t and t + 4, whose swizzles differ: no two meet a bank.
+    const int c = lane & 3, t = w4 * 8 + ((lane >> 2) & 1) * 4 + (lane >> 3);
+    const uint32_t k_src = base + C::raw + (t >> 4) * C::UB + k_chunk<D>(t & 15, c);
+    const uint32_t kp_src = base + C::raw + (t >> 4) * C::UB + kp_base(D) + (t & 15) * NG * 4;
+    uint32_t k_dst[2];  // of words w with w % 2 = 0, 1
+#pragma unroll
+    for (int w = 0; w < 2; ++w) k_dst[w] = base + C::k + sw128_off(t, 32 * w + 8 * c, kTile);
+    // V^T: a thread takes eight tokens (16-byte chunk q8 of a row) of the features
+    // 32 u + 4 r + 0..3
+    const int q8 = (lane & 3) | ((lane >> 3) << 2), r = ((lane >> 2) & 1) | (w4 << 1);
+    const uint32_t v_src = base + C::raw + (q8 >> 1) * C::UB + v_chunk<D>(q8 & 1, r * 4);
+    const uint32_t vp_src = base + C::raw + (q8 >> 1) * C::UB + vp_base(D, NG) + (q8 & 1) * 8 * NG * 4;
+    uint32_t v_dst[4];  // of the features with f % 4 = 0..3
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v_dst[k] = base + C::v + sw128_off(4 * r + k, 8 * q8, D);
+
     for (int step = 0; step < steps; ++step) {
       const int rs = step % C::RAWS, buf = step & 1, t0 = t_begin + step * kTile;
-      const uint32_t raw = base + C::raw + rs * C::RAW;
+      const uint32_t raw = rs * C::RAW, tile_at = buf * C::TILE;
       ok = mbar_wait(&bars[C::raw_full + rs], (step / C::RAWS) & 1, 420);
       if (ok && step >= 2) ok = mbar_wait(&bars[C::k_empty + buf], ((step >> 1) + 1) & 1, 421);
       if (!__all_sync(0xffffffffu, ok)) break;
-      // flags: token i's value parameters
+      // flags of the tokens whose values are NaN
+      bool dirty = t0 + kTile > t_end;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const uint32_t p = lds32(raw + (i >> 4) * C::UB + vp_base(D, NG) + ((i & 15) * NG + g) * 4);
-        const uint32_t fl = __ballot_sync(0xffffffffu, (is_nan(p) || is_nan(p >> 16)) && t0 + i < t_end);
-        if (lane == 0)
-          asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + C::flags + ((step % C::FLAGS) * NG + g) * 16 + w4 * 4), "r"(fl)
-                       : "memory");
-      }
-      // K: four (token, chunk) a thread.  Eight lanes of a store hold tokens t and
-      // t + 4, whose swizzles differ: no two meet a bank
-      const uint32_t kt = base + C::k + buf * C::TILE;
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int tok = 32 * k + lane;
+          const uint32_t p = lds32(base + C::raw + raw + (tok >> 4) * C::UB + vp_base(D, NG) + ((tok & 15) * NG + g) * 4);
+          const bool nan = __hisnan(__low2half(half2_of(p))) || __hisnan(__high2half(half2_of(p)));
+          const uint32_t fl = __ballot_sync(0xffffffffu, nan && t0 + tok < t_end);
+          dirty |= fl != 0;
+          if (threadIdx.x == 8 * 32)
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + C::flags + ((step % C::FLAGS) * NG + g) * 16 + k * 4), "r"(fl)
+                         : "memory");
+        }
 #pragma unroll
       for (int rep = 0; rep < 4; ++rep) {
-        const int c = lane & 3, t = rep * 32 + w4 * 8 + ((lane >> 2) & 1) * 4 + (lane >> 3);
-        const uint32_t unit = raw + (t >> 4) * C::UB;
         uint32_t x[W];
-        lds_words<W>(unit + k_chunk<D>(t & 15, c), x);
+        lds_words<W>(k_src + raw + rep * 2 * C::UB, x);
+        __half2 s2, z2;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          const __half2 sz = half2_of(lds32(unit + kp_base(D) + ((t & 15) * NG + w / WPG) * 4));
-          const __half2 s2 = __low2half2(sz), z2 = __high2half2(sz);
+          if (w % WPG == 0) {
+            const __half2 sz = half2_of(lds32(kp_src + raw + rep * 2 * C::UB + w / WPG * 4));
+            s2 = __low2half2(sz), z2 = __high2half2(sz);
+          }
           const uint32_t y = x[w] >> 8;
-          sts128(kt + sw128_off(t, 32 * w + 8 * c, kTile), bits(__hfma2(centred_lo(x[w]), s2, z2)),
+          sts128(k_dst[w & 1] + tile_at + (w >> 1) * (kTile * 128) + rep * 4096, bits(__hfma2(centred_lo(x[w]), s2, z2)),
                  bits(__hfma2(centred_hi(x[w]), s2, z2)), bits(__hfma2(centred_lo(y), s2, z2)),
                  bits(__hfma2(centred_hi(y), s2, z2)));
         }
       }
       fence_async_smem();
       mbar_arrive(&bars[C::k_full + buf]);
-      // V^T: eight tokens (16-byte chunk q8 of a row) of the features 32 u + 4 r + 0..3
+
       if (step >= 2) ok = mbar_wait(&bars[C::v_empty + buf], ((step >> 1) + 1) & 1, 422);
       if (!__all_sync(0xffffffffu, ok)) break;
-      const uint32_t vt = base + C::v + buf * C::TILE;
-      const int q8 = (lane & 3) | ((lane >> 3) << 2), r = ((lane >> 2) & 1) | (w4 << 1);
-      const uint32_t unit = raw + (q8 >> 1) * C::UB;
       uint32_t x[4][W];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) lds_words<W>(unit + v_chunk<D>(q8 & 1, r * 4 + c), x[c]);
+      for (int k = 0; k < 4; ++k) lds_words<W>(v_src + raw + k * (v_chunk<D>(0, 1) - v_chunk<D>(0, 0)), x[k]);
       __half2 s2[4], z2[4];
 #pragma unroll
       for (int u = 0; u < W; ++u) {
         if (u % WPG == 0) {
+          uint32_t p[8];
+          if constexpr (NG == 1) {
+            uint32_t p0[4], p1[4];
+            lds_words<4>(vp_src + raw, p0);
+            lds_words<4>(vp_src + raw + 16, p1);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t p[2];
+            for (int k = 0; k < 4; ++k) p[k] = p0[k], p[4 + k] = p1[k];
+          } else {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int t = (q8 & 1) * 8 + 2 * c + k;
-              p[k] = lds32(unit + vp_base(D, NG) + (t * NG + u / WPG) * 4);
-              if (is_nan(p[k]) || is_nan(p[k] >> 16) || t0 + (q8 >> 1) * 16 + t >= t_end) p[k] = 0;
+            for (int k = 0; k < 8; ++k) p[k] = lds32(vp_src + raw + (k * NG + u / WPG) * 4);
+          }
+          if (dirty) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const __half2 h = half2_of(p[k]);
+              if (__hisnan(__low2half(h)) || __hisnan(__high2half(h)) || t0 + 8 * q8 + k >= t_end) p[k] = 0;
             }
-            s2[c] = __lows2half2(half2_of(p[0]), half2_of(p[1]));
-            z2[c] = __highs2half2(half2_of(p[0]), half2_of(p[1]));
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            s2[k] = __lows2half2(half2_of(p[2 * k]), half2_of(p[2 * k + 1]));
+            z2[k] = __highs2half2(half2_of(p[2 * k]), half2_of(p[2 * k + 1]));
           }
         }
         // nibbles 0..3 are features 1, 0, 3, 2
         uint32_t o[4][4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint32_t y = x[c][u] >> 8;
-          o[1][c] = bits(__hfma2(centred_lo(x[c][u]), s2[c], z2[c]));
-          o[0][c] = bits(__hfma2(centred_hi(x[c][u]), s2[c], z2[c]));
-          o[3][c] = bits(__hfma2(centred_lo(y), s2[c], z2[c]));
-          o[2][c] = bits(__hfma2(centred_hi(y), s2[c], z2[c]));
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t y = x[k][u] >> 8;
+          o[1][k] = bits(__hfma2(centred_lo(x[k][u]), s2[k], z2[k]));
+          o[0][k] = bits(__hfma2(centred_hi(x[k][u]), s2[k], z2[k]));
+          o[3][k] = bits(__hfma2(centred_lo(y), s2[k], z2[k]));
+          o[2][k] = bits(__hfma2(centred_hi(y), s2[k], z2[k]));
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          sts128(vt + sw128_off(32 * u + 4 * r + k, 8 * q8, D), o[k][0], o[k][1], o[k][2], o[k][3]);
+        for (int k = 0; k < 4; ++k) sts128(v_dst[k] + tile_at + u * 4096, o[k][0], o[k][1], o[k][2], o[k][3]);
       }
       mbar_arrive(&bars[C::raw_empty + rs]);
       fence_async_smem();

@@ -61,7 +61,7 @@ struct Pre {
   // barriers
   static constexpr int q_full = 0, raw_full = 2, raw_empty = raw_full + RAWS, k_full = raw_empty + RAWS,
                        v_full = k_full + 2, k_empty = v_full + 2, v_empty = k_empty + 2, s_full = v_empty + 2,
-                       p_full = s_full + 2, o_done = p_full + 2, n_bars = o_done + 2;
+                       p_full = s_full + 2, o_done = p_full + 4, n_bars = o_done + 2;
   static constexpr int holder = bars + n_bars * 8, bytes = holder + 16;
   static_assert(bytes <= 227 * 1024, "shared memory");
 };
@@ -101,6 +101,12 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
 template <int N>
 __device__ __forceinline__ void more_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -318,6 +324,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             p[k / 2] = pack_half2(x, y);
           }
           tmem_st32(ts + hf * 32, p);
+          // the product with the first 64 tokens starts while the others' weights are formed
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&bars[C::p_full + 2 * half + hf]);
         }
         // values that are NaN were written as 0: remember the rows that see them
 #pragma unroll
@@ -332,9 +342,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&bars[C::p_full + half]);
       }
 
       // ---- the row's result
@@ -495,48 +502,66 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     fewer_registers<40>();
     if (warp == 12) {
-      // ---- issue the products
-      if (lane == 0 && steps > 0) {
-        constexpr uint32_t id_s = idesc_f16(kTile, kTile, false), id_o = idesc_f16(kTile, D, false);
-        bool ok = true;
-        auto scores = [&](int half, int step) {
-          const uint32_t qa = base + C::q + half * C::TILE, kb = base + C::k + (step & 1) * C::TILE;
+      // ---- issue the products.  The whole warp walks the loop with uniform values
+      // and one elected lane issues: a product takes 64 cycles, so there is time
+      // for few instructions between two of them
+      constexpr uint32_t id_s = idesc_f16(kTile, kTile, false), id_o = idesc_f16(kTile, D, false);
+      const uint64_t q_desc = desc_sw128(base + C::q), k_desc = desc_sw128(base + C::k), v_desc = desc_sw128(base + C::v);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      bool ok = true;
+      auto scores = [&](int half, int step) {
+        const uint64_t qd = q_desc + (uint32_t)half * (C::TILE >> 4), kd = k_desc + (uint32_t)(step & 1) * (C::TILE >> 4);
+        if (elect_one()) {
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks) {
-            const uint32_t off = (uint32_t)((ks >> 2) * (kTile * 128) + (ks & 3) * 32);
-            umma_f16(tmem + half * kTile, desc_sw128(qa + off), desc_sw128(kb + off), id_s, ks ? 1u : 0u);
+            const uint32_t off = ((ks >> 2) * (kTile * 128) + (ks & 3) * 32) >> 4;
+            umma_f16(tm + half * kTile, qd + off, kd + off, id_s, ks ? 1u : 0u);
           }
           umma_commit(&bars[C::s_full + half]);
-        };
+        }
+        __syncwarp();
+      };
+      if (steps > 0) {
         for (int half = 0; half < halves; ++half) ok = ok && mbar_wait(&bars[C::q_full + half], 0, 430);
         ok = ok && mbar_wait(&bars[C::k_full], 0, 431);
+        ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
         if (ok) {
           for (int half = 0; half < halves; ++half) scores(half, 0);
-          if (steps > 2) umma_commit(&bars[C::k_empty]);
+          if (steps > 2 && elect_one()) umma_commit(&bars[C::k_empty]);
+          __syncwarp();
         }
-        for (int step = 0; ok && step < steps; ++step) {
-          ok = mbar_wait(&bars[C::v_full + (step & 1)], (step >> 1) & 1, 432);
-          if (ok && step + 1 < steps) ok = mbar_wait(&bars[C::k_full + ((step + 1) & 1)], ((step + 1) >> 1) & 1, 433);
-          for (int half = 0; ok && half < halves; ++half) {
-            ok = mbar_wait(&bars[C::p_full + half], step & 1, 434);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t vb = base + C::v + (step & 1) * C::TILE;
+      }
+      for (int step = 0; ok && step < steps; ++step) {
+        ok = mbar_wait(&bars[C::v_full + (step & 1)], (step >> 1) & 1, 432);
+        const uint64_t vd = v_desc + (uint32_t)(step & 1) * (C::TILE >> 4);
+        for (int half = 0; half < halves; ++half) {
 #pragma unroll
-            for (int ks = 0; ks < kTile / 16; ++ks)
-              umma_f16_ts(tmem + 2 * kTile + half * D, tmem + half * kTile + ks * 8,
-                          desc_sw128(vb + (uint32_t)((ks >> 2) * (D * 128) + (ks & 3) * 32)), id_o, step || ks ? 1u : 0u);
-            umma_commit(&bars[C::o_done + half]);
-            if (step + 1 < steps) scores(half, step + 1);
+          for (int hf = 0; hf < 2; ++hf) {
+            ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars[C::p_full + 2 * half + hf], step & 1, 434));
+            tc_fence_after();
+            if (ok && elect_one()) {
+#pragma unroll
+              for (int ks = 0; ks < kTile / 32; ++ks)
+                umma_f16_ts(tm + 2 * kTile + half * D, tm + half * kTile + hf * 32 + ks * 8,
+                            vd + ((hf * (D * 128) + ks * 32) >> 4), id_o, step || hf || ks ? 1u : 0u);
+              if (hf == 1) umma_commit(&bars[C::o_done + half]);
+            }
+            __syncwarp();
           }
-          if (!ok) break;
-          // only where somebody waits: none may be on its way when the block ends
+          if (half == 0 && step + 1 < steps) {
+            ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars[C::k_full + ((step + 1) & 1)], ((step + 1) >> 1) & 1, 433));
+            tc_fence_after();
+          }
+          if (ok && step + 1 < steps) scores(half, step + 1);
+        }
+        // only where somebody waits: none may be on its way when the block ends
+        if (ok && elect_one()) {
           if (step + 2 < steps) umma_commit(&bars[C::v_empty + (step & 1)]);
           if (step + 3 < steps) umma_commit(&bars[C::k_empty + ((step + 1) & 1)]);
         }
+        __syncwarp();
       }
-      __syncwarp();
     } else if (warp == 13) {
       // ---- bring the codes: lane u copies unit u of each tile
       bool ok = true;

@@ -15,6 +15,7 @@ Magnitudes above 65024 are held as 65024; a NaN makes its group NaN.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
+from functools import partial
 from typing import Any, Sequence
 
 import numpy as np
@@ -46,7 +47,7 @@ class CacheStep:
     cache: Any = field(repr=False)
     meta: torch.Tensor = field(repr=False)  # device arrays that ``desc`` points into
     desc: Kv4Step = field(repr=False)
-    splits: dict[tuple[int, int], tuple[Kv4Split, torch.Tensor]] = field(default_factory=dict, repr=False)
+    splits: dict[tuple[int, int], tuple[tuple[Kv4Split, int], torch.Tensor]] = field(default_factory=dict, repr=False)
 
     @property
     def tokens(self) -> int:
@@ -139,6 +140,7 @@ class PagedKVCache:
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         self.device = device
+        self._scale = self.head_dim ** -0.5
         self.page_bytes = ops.kv4_page_bytes(self.n_kv_heads, self.head_dim, self.page_size, self.group_size)
         # zeros: a page's bytes are defined before its first tokens are written
         self.pool = torch.zeros(self.n_layers, self.pages.n_pages, self.page_bytes, dtype=torch.uint8, device=device)
@@ -218,11 +220,11 @@ class PagedKVCache:
                        int(q_start[-1]))
         return CacheStep(seqs, counts, lengths.tolist(), writable, self.pages.epoch, self, meta, desc)
 
-    def _split(self, step: CacheStep, n_q: int, code: int) -> Kv4Split:
+    def _split(self, step: CacheStep, n_q: int, code: int) -> tuple[Kv4Split, int]:
         got = step.splits.get((n_q, code))
         if got is None:
             lengths = np.array(step.lengths, dtype=np.int64)
-            tiles, resident = ops.kv4_attend_shape(self._layout, step.desc, n_q, code, self.device)
+            tiles, resident = ops.kv4_attend_split(self._layout, step.desc, n_q, code, self.device)
             chunk = split_chunk(lengths, self.n_kv_heads * tiles, resident, 8 * step.tokens * n_q * (self.head_dim + 2))
             items = np.maximum(1, -(-lengths // chunk))
             start = _prefix(items)
@@ -230,7 +232,9 @@ class PagedKVCache:
             rows = np.array([self.pages.row(s) for s in step.seqs], dtype=np.int64)
             table = np.stack((seq, (np.arange(int(start[-1])) - start[seq]) * chunk, rows[seq], lengths[seq]), 1)
             buf, at = _upload((table.reshape(-1), start), self.device)
-            got = step.splits[n_q, code] = (Kv4Split(at[0], at[1], int(start[-1]), chunk, int(items.max(initial=1))), buf)
+            split = Kv4Split(at[0], at[1], int(start[-1]), chunk, int(items.max(initial=1)))
+            got = (split, ops.kv4_attend_workspace(self._layout, step.desc, split, n_q)), buf
+            step.splits[n_q, code] = got
         return got[0]
 
     def _check(self, what: str, layer: int, step: CacheStep) -> int:
@@ -267,9 +271,8 @@ class PagedKVCache:
         tokens up to its own position, otherwise all cached tokens of its sequence;
         one that sees none gets zeros.  ``scale`` defaults to ``head_dim ** -0.5``."""
         pool = self._check("attend", layer, step)
-        return ops.kv4_attend(self._layout, step.desc, lambda n_q, code: self._split(step, n_q, code), pool, query,
-                              causal=causal, scale=self.head_dim ** -0.5 if scale is None else float(scale),
-                              device=self.device)
+        return ops.kv4_attend(self._layout, step.desc, partial(self._split, step), pool, query, causal=causal,
+                              scale=self._scale if scale is None else float(scale), device=self.device)
 
     def read(self, seq: int, *, layers: Sequence[int] | None = None, t0: int = 0, t1: int | None = None,
              dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:

@@ -6,6 +6,7 @@
 // (4 lanes: 64 contiguous bytes) and word w of K's chunk c, so K's codes need
 // no exchange at all and V's one shuffle a word with the neighbouring token.
 #include <algorithm>
+#include <type_traits>
 
 #include "kvc_kv4.cuh"
 #include "kvc_tc.cuh"
@@ -261,16 +262,19 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(Layout L, const uint8_t* 
 
 // ---- page copies ------------------------------------------------------------
 
-constexpr int kPairs = 1024;  // page pairs of a launch, by value: no staging buffer to keep alive
+// Page pairs of a launch, by value: no staging buffer to keep alive.  Few pairs
+// (a fork's) go in a small one, since a launch copies its parameters.
+constexpr int kPairs = 1024, kFewPairs = 32;
 constexpr int kCopyBytes = 16384;
 
+template <int N>
 struct CopyPairs {
-  int32_t src[kPairs], dst[kPairs];
+  int32_t src[N], dst[N];
 };
 
-template <typename V>
+template <typename V, int N>
 __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CellPtrsMut pools,
-                                                         const __grid_constant__ CopyPairs pairs, int64_t page_bytes,
+                                                         const __grid_constant__ CopyPairs<N> pairs, int64_t page_bytes,
                                                          int parts) {
   const int pair = blockIdx.x / parts, part = blockIdx.x % parts;
   uint8_t* base = static_cast<uint8_t*>(pools.p[blockIdx.y]);
@@ -392,17 +396,25 @@ extern "C" int kvc_copy_pages(int n_pools, void* const* pools, int64_t n_pages, 
       return fail(KVC_ERR_SHAPE, "kvc_copy_pages: page out of range");
   const int64_t parts = ceil_div(page_bytes, kCopyBytes);
   if (parts > INT32_MAX / kPairs) return fail(KVC_ERR_SHAPE, "kvc_copy_pages: page too large");
-  for (int64_t at = 0; at < n_pairs; at += kPairs) {
-    const int n = (int)std::min<int64_t>(kPairs, n_pairs - at);
-    CopyPairs pr;
-    memcpy(pr.src, src + at, n * sizeof(int32_t));
-    memcpy(pr.dst, dst + at, n * sizeof(int32_t));
-    const dim3 grid((unsigned)(n * parts), (unsigned)n_pools);
+  auto launch = [&](auto& pr, auto limit) {
+    constexpr int N = decltype(limit)::value;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a16) copy_pages_kernel<uint4><<<grid, 256, 0, st>>>(p, pr, page_bytes, (int)parts);
-    else if (a4) copy_pages_kernel<uint32_t><<<grid, 256, 0, st>>>(p, pr, page_bytes, (int)parts);
-    else copy_pages_kernel<uint8_t><<<grid, 256, 0, st>>>(p, pr, page_bytes, (int)parts);
-    if (int rc = check_launch("copy_pages_kernel")) return rc;
+    for (int64_t at = 0; at < n_pairs; at += N) {
+      const int n = (int)std::min<int64_t>(N, n_pairs - at);
+      memcpy(pr.src, src + at, n * sizeof(int32_t));
+      memcpy(pr.dst, dst + at, n * sizeof(int32_t));
+      const dim3 grid((unsigned)(n * parts), (unsigned)n_pools);
+      if (a16) copy_pages_kernel<uint4, N><<<grid, 256, 0, st>>>(p, pr, page_bytes, (int)parts);
+      else if (a4) copy_pages_kernel<uint32_t, N><<<grid, 256, 0, st>>>(p, pr, page_bytes, (int)parts);
+      else copy_pages_kernel<uint8_t, N><<<grid, 256, 0, st>>>(p, pr, page_bytes, (int)parts);
+      if (int rc = check_launch("copy_pages_kernel")) return rc;
+    }
+    return (int)KVC_OK;
+  };
+  if (n_pairs <= kFewPairs) {
+    CopyPairs<kFewPairs> pr;
+    return launch(pr, std::integral_constant<int, kFewPairs>{});
   }
-  return KVC_OK;
+  CopyPairs<kPairs> pr;
+  return launch(pr, std::integral_constant<int, kPairs>{});
 }

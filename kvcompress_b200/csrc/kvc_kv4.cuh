@@ -20,6 +20,8 @@
 //    first token in its low half, of the second in its high half.
 #pragma once
 
+#include <atomic>
+
 #include "kvc_common.cuh"
 
 namespace kvc {
@@ -100,6 +102,20 @@ int launch_after(const char* what, K kernel, dim3 grid, unsigned threads, size_t
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e != cudaSuccess) return fail(KVC_ERR_LAUNCH, std::string(what) + ": " + cudaGetErrorString(e));
   return check_launch(what);
+}
+
+// Allow a kernel `bytes` of dynamic shared memory, once for each device (`done`
+// is the kernel's own: a bit a device).
+template <typename K>
+int allow_shared(const char* what, K kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = dev >= 0 && dev < 64 ? uint64_t(1) << dev : 0;
+  if (e == cudaSuccess && (done.load(std::memory_order_relaxed) & bit)) return KVC_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return fail(KVC_ERR_LAUNCH, std::string(what) + ": " + cudaGetErrorString(e));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return KVC_OK;
 }
 
 // Host side: argument checks shared by the entry points.

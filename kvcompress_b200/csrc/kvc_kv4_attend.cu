@@ -662,8 +662,8 @@ int launch(const Layout& L, const Step& S, const Split& P, const void* pool, con
            int64_t n_items, int col_tiles, cudaStream_t st) {
   using Sm = Smem<D, WPG, NT, TERMS>;
   auto kernel = attend_kernel<D, WPG, NT, TERMS>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sm::bytes);
-  if (e != cudaSuccess) return fail(KVC_ERR_LAUNCH, std::string("attend_kernel: ") + cudaGetErrorString(e));
+  static std::atomic<uint64_t> done{0};
+  if (int rc = allow_shared("attend_kernel", kernel, Sm::bytes, done)) return rc;
   const dim3 grid((unsigned)n_items, (unsigned)L.n_kv, (unsigned)col_tiles);
   return launch_after("attend_kernel", kernel, grid, Shape<D, WPG, NT, TERMS>::warps * 32, Sm::bytes, st, L, S, P,
                       static_cast<const uint8_t*>(pool), a, part);

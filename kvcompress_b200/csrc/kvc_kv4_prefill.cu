@@ -600,8 +600,8 @@ int launch(const Layout& L, const Step& S, const Split& P, const uint8_t* pool, 
            const dim3& grid, cudaStream_t st) {
   using C = Pre<D, WPG>;
   auto kernel = prefill_kernel<T, D, WPG>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::bytes);
-  if (e != cudaSuccess) return fail(KVC_ERR_LAUNCH, std::string("prefill_kernel: ") + cudaGetErrorString(e));
+  static std::atomic<uint64_t> done{0};
+  if (int rc = allow_shared("prefill_kernel", kernel, C::bytes, done)) return rc;
   const int q_vec = aligned16(a.q) && ((a.q_sb | a.q_st | a.q_sh) & 7) == 0;
   const int o_vec = aligned16(a.out) && ((a.o_sb | a.o_st | a.o_sh) & 7) == 0;
   return launch_after("prefill_kernel", kernel, grid, kThreads, C::bytes, st, L, S, P, pool, a, part, q_vec, o_vec);

@@ -673,6 +673,21 @@ def cast(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 
 
 # ---- paged 4-bit cache -----------------------------------------------------
+#
+# These run once a layer and token while a model decodes, where the host's own
+# time is what a step costs: arguments are checked once, device and trace
+# contexts are entered only where they do something.
+
+
+def _call(name: str, device: torch.device, nbytes: int, fn, *args) -> None:
+    """One library call on ``device``'s current stream, which is its last argument."""
+    if _TRACE is None and device.index == torch._C._cuda_getDevice():
+        rc = fn(*args, _raw_stream(device.index))
+    else:
+        with _on(device), _Stage(name, 1, nbytes):
+            rc = fn(*args, _raw_stream(device.index))
+    if rc != KVC.OK:
+        check(rc, "kvc_" + name)
 
 
 def kv4_page_bytes(n_kv: int, head_dim: int, page_size: int, group_size: int) -> int:
@@ -680,26 +695,30 @@ def kv4_page_bytes(n_kv: int, head_dim: int, page_size: int, group_size: int) ->
     return int(lib().kvc_kv4_page_bytes(n_kv, head_dim, page_size, group_size))
 
 
+_KV4_CODE = {torch.float32: KVC.F32, torch.float16: KVC.F16, torch.bfloat16: KVC.BF16}
+
+
 def _kv4_code(dtype: torch.dtype) -> int:
-    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+    code = _KV4_CODE.get(dtype)
+    if code is None:
         raise TypeError(f"unsupported dtype {dtype}: float32, float16 or bfloat16")
-    return DTYPE_CODE[dtype]
+    return code
 
 
 def _kv4_tokens(x: torch.Tensor, step, what: str, n_heads: int | None, layout, device) -> tuple[int, int, int, int]:
     """Check a step's per-token tensor; (sequence, token, head) strides and whether it is packed."""
-    if not x.is_cuda:
-        raise RuntimeError(f"{what}: kvcompress_b200 runs on CUDA tensors only (got {x.device})")
     if x.device != device:
+        if not x.is_cuda:
+            raise RuntimeError(f"{what}: kvcompress_b200 runs on CUDA tensors only (got {x.device})")
         raise ValueError(f"{what}: tensor on {x.device}, cache on {device}")
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{what}: there is no gradient through a cache in 4 bits; use torch.no_grad() or detach()")
     d, shape, st = layout.head_dim, x.shape, x.stride()
-    if x.dim() == 3:
+    if len(shape) == 3:
         if shape[0] != step.n_tokens or shape[2] != d or (n_heads is not None and shape[1] != n_heads):
             raise ValueError(f"{what}: expected ({step.n_tokens}, {n_heads or 'heads'}, {d}), got {tuple(shape)}")
         out = (0, st[0], st[1], 1)
-    elif x.dim() == 4:
+    elif len(shape) == 4:
         t = step.max_new
         if (shape[0] != step.n_seqs or shape[2] != t or t * step.n_seqs != step.n_tokens or shape[3] != d
                 or (n_heads is not None and shape[1] != n_heads)):
@@ -720,42 +739,37 @@ def kv4_write(layout, step, pool: int, key: torch.Tensor, value: torch.Tensor, d
     code = _kv4_code(key.dtype)
     if key.stride() != value.stride():
         key, value = key.contiguous(), value.contiguous()
-    strides = _kv4_tokens(key, step, "kv4_write", layout.n_kv, layout, device)
     _kv4_tokens(value, step, "kv4_write", layout.n_kv, layout, device)
-    with _on(device), _Stage("kv4_write", 1, 2 * key.numel() * key.element_size()):
-        check(lib().kvc_kv4_write(layout, step, pool, key.data_ptr(), value.data_ptr(), code, *strides, _stream()),
-              "kvc_kv4_write")
+    strides = _kv4_tokens(key, step, "kv4_write", layout.n_kv, layout, device)
+    _call("kv4_write", device, 2 * key.numel() * key.element_size(), lib().kvc_kv4_write, layout, step, pool,
+          key.data_ptr(), value.data_ptr(), code, *strides)
 
 
 def kv4_attend(layout, step, split, pool: int, query: torch.Tensor, *, causal: bool, scale: float,
                device: torch.device) -> torch.Tensor:
     """Attention of a step's queries over the pages of the layer at address
     ``pool`` (``kvc_kv4_attend``).  ``split(n_q, code)`` gives the split of the
-    cached tokens for ``n_q`` query heads of dtype ``code``."""
+    cached tokens for ``n_q`` query heads of dtype ``code``, and the workspace's bytes."""
     code = _kv4_code(query.dtype)
-    qs = _kv4_tokens(query, step, "kv4_attend", None, layout, device)
-    n_q = int(query.shape[1])
+    sb, st, sh, packed = _kv4_tokens(query, step, "kv4_attend", None, layout, device)
+    n_q = query.shape[1]
     if n_q % layout.n_kv or n_q == 0:
         raise ValueError(f"kv4_attend: {n_q} query heads are no multiple of {layout.n_kv} KV heads")
     out = torch.empty(query.shape, dtype=query.dtype, device=device)
     if step.n_tokens == 0:
         return out
-    st = out.stride()
-    os_ = (0, st[0], st[1]) if qs[3] else (st[0], st[2], st[1])
-    L = lib()
-    sp = split(n_q, code)
-    ws_n = L.kvc_kv4_attend_workspace_bytes(layout, step, sp, n_q)
+    o = out.stride()
+    sp, ws_n = split(n_q, code)
     # a buffer of this call's own: a captured graph keeps the one it was captured
     # with, and no other graph or stream writes to it
     ws = torch.empty(ws_n, dtype=torch.uint8, device=device) if ws_n else None
-    with _on(device), _Stage("kv4_attend", 1, 2 * query.numel() * query.element_size()):
-        check(L.kvc_kv4_attend(layout, step, sp, pool, n_q, query.data_ptr(), *qs[:3], out.data_ptr(), *os_, qs[3],
-                               code, int(causal), scale, ws.data_ptr() if ws_n else None, ws_n, _stream()),
-              "kvc_kv4_attend")
+    _call("kv4_attend", device, 2 * query.numel() * query.element_size(), lib().kvc_kv4_attend, layout, step, sp, pool,
+          n_q, query.data_ptr(), sb, st, sh, out.data_ptr(), 0 if packed else o[0], o[0] if packed else o[2], o[1],
+          packed, code, causal, scale, ws.data_ptr() if ws_n else None, ws_n)
     return out
 
 
-def kv4_attend_shape(layout, step, n_q: int, code: int, device: torch.device) -> tuple[int, int]:
+def kv4_attend_split(layout, step, n_q: int, code: int, device: torch.device) -> tuple[int, int]:
     """Blocks an item of one KV head is worked on by, and blocks the device runs at once."""
     tiles, resident = ctypes.c_int(0), ctypes.c_int(0)
     with _on(device):
@@ -764,17 +778,20 @@ def kv4_attend_shape(layout, step, n_q: int, code: int, device: torch.device) ->
     return tiles.value, resident.value
 
 
+def kv4_attend_workspace(layout, step, split, n_q: int) -> int:
+    """Bytes of ``kvc_kv4_attend``'s workspace."""
+    return int(lib().kvc_kv4_attend_workspace_bytes(layout, step, split, n_q))
+
+
 def kv4_read(layout, pool: int, layer_bytes: int, n_layers: int, row: int, t0: int, t1: int, dtype: torch.dtype,
              device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
     """Dense K and V, ``(n_layers, n_kv, t1 - t0, d)``, of table row ``row`` (``kvc_kv4_read``)."""
     code = _kv4_code(dtype)
     shape = (n_layers, layout.n_kv, t1 - t0, layout.head_dim)
-    k = torch.empty(shape, dtype=dtype, device=device)
-    v = torch.empty(shape, dtype=dtype, device=device)
+    k, v = torch.empty((2, *shape), dtype=dtype, device=device).unbind(0)  # one allocation
     if k.numel():
-        with _on(device), _Stage("kv4_read", 1, 2 * k.numel() * k.element_size()):
-            check(lib().kvc_kv4_read(layout, pool, layer_bytes, n_layers, row, t0, t1, code, k.data_ptr(),
-                                     v.data_ptr(), _stream()), "kvc_kv4_read")
+        _call("kv4_read", device, 2 * k.numel() * k.element_size(), lib().kvc_kv4_read, layout, pool, layer_bytes,
+              n_layers, row, t0, t1, code, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -787,40 +804,40 @@ def copy_pages(pools, src: Sequence[int], dst: Sequence[int]) -> None:
     on the host.  A page may be copied to several places; no page may be written
     twice, or be read and written (``ValueError``)."""
     if isinstance(pools, torch.Tensor):
-        if pools.dim() < 2:
+        shape = pools.shape
+        if len(shape) < 2:
             raise ValueError("copy_pages: expected (pools, pages, ...)")
         if not pools.is_cuda:
             raise RuntimeError(f"copy_pages: kvcompress_b200 runs on CUDA tensors only (got {pools.device})")
         if not pools.is_contiguous():
             raise ValueError("copy_pages: pools must be contiguous")
-        n, step = int(pools.shape[0]), pools.stride(0) * pools.element_size()
-        ptrs, first = [pools.data_ptr() + i * step for i in range(n)], pools
-        n_pages, elems = int(pools.shape[1]), pools[0].numel() if n else 0
+        base, step, size = pools.data_ptr(), pools.stride(0) * pools.element_size(), pools.element_size()
+        ptrs, n_pages, elems, device = [base + i * step for i in range(shape[0])], shape[1], pools.stride(0), pools.device
     else:
         xs = list(pools)
         for i in range(0, len(xs), KVC.MAX_CELLS):
             _cells(xs[i:i + KVC.MAX_CELLS], "copy_pages")
             if xs[i].dim() < 1 or xs[i].shape != xs[0].shape or xs[i].dtype != xs[0].dtype or xs[i].device != xs[0].device:
                 raise ValueError("copy_pages: pools must share shape, dtype and device")
-        ptrs, first = [x.data_ptr() for x in xs], xs[0] if xs else None
-        n_pages, elems = (int(first.shape[0]), first.numel()) if xs else (0, 0)
-    src, dst = [int(i) for i in src], [int(i) for i in dst]
-    if len(src) != len(dst):
-        raise ValueError(f"copy_pages: {len(src)} sources but {len(dst)} destinations")
-    if not src or not ptrs:
-        return
-    to = set(dst)
-    if len(to) != len(dst):
-        raise ValueError("copy_pages: a page is written twice")
-    if not to.isdisjoint(src):
-        raise ValueError("copy_pages: a page is both read and written")
-    if min(min(src), min(dst)) < 0 or max(max(src), max(dst)) >= n_pages:
-        raise ValueError(f"copy_pages: page out of range (pool of {n_pages})")
-    page_bytes = elems // n_pages * first.element_size()
+        if not xs:
+            return
+        ptrs, n_pages, elems, device = [x.data_ptr() for x in xs], xs[0].shape[0], xs[0].numel(), xs[0].device
+        size = xs[0].element_size()
     n = len(src)
+    if n != len(dst):
+        raise ValueError(f"copy_pages: {n} sources but {len(dst)} destinations")
+    if n == 0 or not ptrs:
+        return
     a, b = (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst)
-    with _on(first.device), _Stage("copy_pages", 1, 2 * n * page_bytes * len(ptrs)):
-        for i in range(0, len(ptrs), KVC.MAX_CELLS):
-            part = ptrs[i:i + KVC.MAX_CELLS]
-            check(lib().kvc_copy_pages(len(part), ptr_array(part), n_pages, page_bytes, n, a, b, _stream()),
-                  "kvc_copy_pages")
+    to = set(b)
+    if len(to) != n:
+        raise ValueError("copy_pages: a page is written twice")
+    if not to.isdisjoint(a):
+        raise ValueError("copy_pages: a page is both read and written")
+    if min(min(a), min(b)) < 0 or max(max(a), max(b)) >= n_pages:
+        raise ValueError(f"copy_pages: page out of range (pool of {n_pages})")
+    page_bytes = elems // n_pages * size
+    for i in range(0, len(ptrs), KVC.MAX_CELLS):
+        part = ptrs[i:i + KVC.MAX_CELLS]
+        _call("copy_pages", device, 2 * n * page_bytes * len(part), lib().kvc_copy_pages, len(part),
+              (ctypes.c_void_p * len(part))(*part), n_pages, page_bytes, n, a, b)

@@ -70,37 +70,65 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 
 // ---- the quantiser ------------------------------------------------------------
 
-// scale = (hi - lo) / 15 and zero = lo + 8 scale, each to float32 and then to
-// float16; the quotient and the sum are formed in 64 bits so that a float16
-// step is never decided by an earlier rounding.  A NaN in the group makes both
-// NaN.
+// scale = (hi - lo) / 15 and zero = lo + 8 scale, each rounded to float32 and then
+// to float16.  One float32 operation rounds its exact result once: the sum
+// always, the quotient where hi - lo is exact, as it nearly always is for 16-bit
+// elements; elsewhere the quotient is formed in 64 bits.  A NaN in the group
+// makes both NaN.
 __device__ __forceinline__ __half2 params_of(float lo, float hi, bool nan) {
   if (nan) return __half2half2(__ushort_as_half(0x7FFF));
-  const __half s = __float2half_rn((float)(((double)hi - (double)lo) / 15.0));
-  const __half z = __float2half_rn((float)((double)lo + 8.0 * (double)__half2float(s)));
+  const float d = hi - lo, bb = d - hi, err = (hi - (d - bb)) + (-lo - bb);  // two-sum: d + err = hi - lo
+  float q = __fdiv_rn(d, 15.0f);
+  if (err != 0.0f) q = (float)(((double)hi - (double)lo) / 15.0);
+  const __half s = __float2half_rn(q);
+  const __half z = __float2half_rn(__fadd_rn(lo, 8.0f * __half2float(s)));
   return __halves2half2(s, z);
 }
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
-// clamp(rint((x - z) / s), -8, 7) of the exact quotient.  (x - z) * (1 / s) in
-// float32 is within 1.5e-6 of it (|quotient| <= 8.5, three roundings), so only
-// a result that close to a half needs more: there the sign of
-// (x - z) - (n + 1/2) s decides, which is exact: (n + 1/2) s has 16 bits, the
-// rounded x - z is next to it (their difference is exact by Sterbenz' lemma),
-// and the rounding error of x - z is itself a float32 (Knuth's two-sum).
-// NaN gives -8.
-__device__ __forceinline__ float level_of(float x, float s, float z, float inv) {
-  const float a = x - z;
-  const float t = fminf(fmaxf(a * inv, -8.0f), 7.0f);
-  float n = rintf(t);
-  if (fabsf(t - n) > 0.499996f) {
-    const float f = floorf(t), h = (f + 0.5f) * s;
-    const float bb = a - x;
-    const float err = (x - (a - bb)) + (-z - bb);
-    const float res = (a - h) + err;
-    const bool odd = (((int)f) & 1) != 0;
-    n = res > 0.0f || (res == 0.0f && odd) ? f + 1.0f : f;
+// Codes 0..15: clamp(rint((x - z) / s), -8, 7) + 8 of the exact quotient.
+//
+// In float32, v = sat((x - z) / (15 s) + 8 / 15) is the code over 15, and 15 v +
+// 1.5 2^23 rounds it to an integer; the distance from there, 15 v - n, says how
+// near a half it was.  The roundings make an error below 4e-6, so only a
+// distance above 0.49999 needs more: there the sign of (x - z) - (n + 1/2) s
+// decides, which is exact: (n + 1/2) s has 16 bits, the rounded x - z is next to
+// it (their difference is exact by Sterbenz' lemma), and the rounding error of
+// x - z is itself a float32 (Knuth's two-sum).  A NaN gives 0.
+constexpr float kMagic = 12582912.0f;
+
+__device__ __noinline__ float code_near_half(float x, float s, float z, float t) {
+  const float f = floorf(t) - 8.0f, h = (f + 0.5f) * s;
+  const float a = x - z, bb = a - x;
+  const float err = (x - (a - bb)) + (-z - bb);
+  const float res = (a - h) + err;
+  const bool odd = (((int)f) & 1) != 0;
+  return (res > 0.0f || (res == 0.0f && odd) ? f + 1.0f : f) + 8.0f;
+}
+
+// The word of eight elements (the first of each byte in its high nibble).
+__device__ __forceinline__ uint32_t word_of(const float (&x)[8], float s, float z, float inv15) {
+  float n[8], t[8], far = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float v = __saturatef(fmaf(x[e] - z, inv15, 8.0f / 15.0f));
+    n[e] = fmaf(v, 15.0f, kMagic) - kMagic;
+    t[e] = v;
+    far = fmaxf(far, fabsf(fmaf(v, 15.0f, -n[e])));
   }
-  return n;
+  if (far > 0.49999f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (fabsf(fmaf(t[e], 15.0f, -n[e])) > 0.49999f) n[e] = code_near_half(x[e], s, z, t[e] * 15.0f);
+  }
+  // four codes are an integer below 2^16, exact in float32
+  const float lo = fmaf(fmaf(fmaf(n[2], 16.0f, n[3]), 16.0f, n[0]), 16.0f, n[1]) + kMagic;
+  const float hi = fmaf(fmaf(fmaf(n[6], 16.0f, n[7]), 16.0f, n[4]), 16.0f, n[5]) + kMagic;
+  return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x5410);
 }
 
 struct KvIn {
@@ -112,19 +140,19 @@ struct KvIn {
 
 // W = D / 32 words a lane; WPG words a quantisation group.
 template <typename T, int D, int WPG>
-__global__ void __launch_bounds__(128) kv4_write_kernel(Layout L, Step S, uint8_t* pool, KvIn in, int64_t n_halves,
+__global__ void __launch_bounds__(128) kv4_write_kernel(Layout L, Step S, uint8_t* pool, KvIn in, int n_halves,
                                                         const int32_t* __restrict__ half_seq,
                                                         const int32_t* __restrict__ half_start) {
   constexpr int W = D / 32, NG = W / WPG;
+  grid_wait();
   grid_go();  // the attention of these tokens may get ready
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const int64_t id = blockIdx.x * 4LL + (threadIdx.x >> 5);
-  if (id >= n_halves * L.n_kv * 2) return;
-  const int is_v = (int)(id & 1), h = (int)((id >> 1) % L.n_kv);
-  const int64_t half = (id >> 1) / L.n_kv;
+  const int id = (int)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (id >= n_halves * 2) return;
+  const int is_v = id & 1, half = id >> 1, h = blockIdx.y;
   const int b = half_seq[half];
   const int len = S.kv_len[b], q0 = S.q_start[b], n = S.q_start[b + 1] - q0, first = len - n;
-  const int tok0 = (first / 8 + (int)(half - half_start[b])) * 8, pos = tok0 + r;
+  const int tok0 = (first / 8 + half - half_start[b]) * 8, pos = tok0 + r;
   const bool valid = pos >= first && pos < len;
   const int64_t page = page_of(L, S.rows[b], tok0, &tc::g_kvc_device_error);
   if (page < 0) return;
@@ -147,32 +175,39 @@ __global__ void __launch_bounds__(128) kv4_write_kernel(Layout L, Step S, uint8_
   uint32_t word[W];
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    float lo = 3.0e38f, hi = -3.0e38f;
-    bool nan = false;
+    float lo = x[g * WPG][0], hi = lo, odd = 0.0f;  // odd: NaN where an element is NaN or infinite
 #pragma unroll
     for (int w = g * WPG; w < (g + 1) * WPG; ++w)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        nan |= x[w][e] != x[w][e];
-        x[w][e] = fminf(fmaxf(x[w][e], -kLimit), kLimit);
-        lo = fminf(lo, x[w][e]);
-        hi = fmaxf(hi, x[w][e]);
+      for (int e = 0; e < 8; e += 2) {
+        lo = fminf(lo, fminf(x[w][e], x[w][e + 1]));
+        hi = fmaxf(hi, fmaxf(x[w][e], x[w][e + 1]));
+        odd = fmaf(x[w][e], 0.0f, odd);
+        odd = fmaf(x[w][e + 1], 0.0f, odd);
       }
 #pragma unroll
     for (int o = 1; o <= 2; o <<= 1) {
       lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
       hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      nan |= __shfl_xor_sync(0xffffffffu, (int)nan, o) != 0;
+    }
+    bool nan = false;
+    if (__any_sync(0xffffffffu, !(odd == 0.0f) || lo < -kLimit || hi > kLimit)) {
+#pragma unroll
+      for (int w = g * WPG; w < (g + 1) * WPG; ++w)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          nan |= x[w][e] != x[w][e];
+          x[w][e] = fminf(fmaxf(x[w][e], -kLimit), kLimit);
+        }
+      nan |= __shfl_xor_sync(0xffffffffu, (int)nan, 1) != 0;
+      nan |= __shfl_xor_sync(0xffffffffu, (int)nan, 2) != 0;
+      lo = fminf(fmaxf(lo, -kLimit), kLimit);
+      hi = fminf(fmaxf(hi, -kLimit), kLimit);
     }
     const __half2 sz = params_of(lo, hi, nan);
-    const float s = __low2float(sz), z = __high2float(sz), inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
+    const float s = __low2float(sz), z = __high2float(sz), inv15 = s > 0.0f ? rcp_approx(15.0f * s) : 0.0f;
 #pragma unroll
-    for (int w = g * WPG; w < (g + 1) * WPG; ++w) {
-      uint32_t bits = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) bits |= (uint32_t)((int)level_of(x[w][e], s, z, inv) + 8) << (4 * (e ^ 1));
-      word[w] = bits;
-    }
+    for (int w = g * WPG; w < (g + 1) * WPG; ++w) word[w] = word_of(x[w], s, z, inv15);
     if (valid && c == 0)
       reinterpret_cast<__half2*>(unit + (is_v ? vp_base(D, NG) : kp_base(D)))[t * NG + g] = sz;
   }
@@ -211,15 +246,14 @@ __global__ void __launch_bounds__(128) kv4_write_kernel(Layout L, Step S, uint8_
 // Dense (layers, n_kv, t1 - t0, D) K and V of tokens [t0, t1) of one sequence.
 template <typename T, int D, int WPG>
 __global__ void __launch_bounds__(128) kv4_read_kernel(Layout L, const uint8_t* pool, int64_t layer_bytes, int row,
-                                                       int t0, int t1, int64_t n_halves, int64_t n_warps,
-                                                       T* __restrict__ ko, T* __restrict__ vo) {
+                                                       int t0, int t1, int n_halves, T* __restrict__ ko,
+                                                       T* __restrict__ vo) {
   constexpr int W = D / 32, NG = W / WPG;
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const int64_t id = blockIdx.x * 4LL + (threadIdx.x >> 5);
-  if (id >= n_warps) return;
-  const int is_v = (int)(id & 1), h = (int)((id >> 1) % L.n_kv);
-  const int64_t half = ((id >> 1) / L.n_kv) % n_halves, layer = ((id >> 1) / L.n_kv) / n_halves;
-  const int tok0 = (int)(t0 / 8 + half) * 8, pos = tok0 + r, t = pos & 15;
+  const int id = (int)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (id >= n_halves * 2) return;
+  const int is_v = id & 1, half = id >> 1, h = blockIdx.y, layer = blockIdx.z;
+  const int tok0 = (t0 / 8 + half) * 8, pos = tok0 + r, t = pos & 15;
   const int64_t page = page_of(L, row, tok0, &tc::g_kvc_device_error);
   if (page < 0) return;
   const uint8_t* unit = pool + layer * layer_bytes + unit_off<D>(L, page, h, tok0);
@@ -244,17 +278,20 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(Layout L, const uint8_t* 
   }
   if (pos < t0 || pos >= t1) return;
   const __half2* par = reinterpret_cast<const __half2*>(unit + (is_v ? vp_base(D, NG) : kp_base(D))) + t * NG;
-  T* dst = (is_v ? vo : ko) + ((layer * L.n_kv + h) * (int64_t)(t1 - t0) + (pos - t0)) * D + 8 * c;
+  T* dst = (is_v ? vo : ko) + (((int64_t)layer * L.n_kv + h) * (int64_t)(t1 - t0) + (pos - t0)) * D + 8 * c;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
     const __half2 sz = par[w / WPG];
     const float s = __low2float(sz), z = __high2float(sz);
+    // nibbles i and i + 4 of a word, elements i ^ 1 and (i ^ 1) + 4, as float16
+    // c - 8 (exact), then zero + scale * q in float32
     float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      // 2^23 + code as a float's bits; the subtraction leaves code - 8 exactly
-      const float q = __uint_as_float(0x4B000000u | ((word[w] >> (4 * (e ^ 1))) & 15u)) - 8388616.0f;
-      x[e] = fmaf(q, s, z);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t y = word[w] >> (i & 2 ? 8 : 0);
+      const float2 q = i & 1 ? __half22float2(centred_hi(y)) : __half22float2(centred_lo(y));
+      x[i ^ 1] = fmaf(q.x, s, z);
+      x[(i ^ 1) + 4] = fmaf(q.y, s, z);
     }
     store8(dst + 32 * w, x);
   }
@@ -336,21 +373,24 @@ extern "C" int kvc_kv4_write(const kvc_kv4_layout* layout, const kvc_kv4_step* s
   if (step->n_halves < 0 || step->n_seqs < 0) return fail(KVC_ERR_SHAPE, "kvc_kv4_write: negative size");
   if (step->n_halves == 0) return KVC_OK;
   if (!k || !v) return fail(KVC_ERR_ARG, "kvc_kv4_write: NULL pointer");
-  const int64_t warps = step->n_halves * layout->n_kv * 2, blocks = ceil_div(warps, 4);
-  if (blocks > INT32_MAX) return fail(KVC_ERR_SHAPE, "kvc_kv4_write: too many tokens in one call");
+  if (step->n_halves > INT32_MAX / 4 || layout->n_kv > 65535)
+    return fail(KVC_ERR_SHAPE, "kvc_kv4_write: too many tokens or KV heads in one call");
+  const dim3 grid((unsigned)ceil_div(step->n_halves * 2, 4), (unsigned)layout->n_kv);
   const int64_t e = (int64_t)dtype_size(dtype);
   const bool vec = aligned16(k) && aligned16(v) && (seq_stride * e) % 16 == 0 && (token_stride * e) % 16 == 0 &&
                    (head_stride * e) % 16 == 0;
   const KvIn in{k, v, seq_stride, token_stride, head_stride, packed, vec};
   const Step s{step->n_seqs, step->rows, step->kv_len, step->q_start};
   const Layout L = to_layout(layout);
-#define KVC_F(D, WPG)                                                                                         \
-  KVC_DISPATCH_DTYPE(dtype, T,                                                                                \
-                     (kv4_write_kernel<T, D, WPG><<<(unsigned)blocks, 128, 0, static_cast<cudaStream_t>(stream)>>>( \
-                         L, s, static_cast<uint8_t*>(pool), in, step->n_halves, step->half_seq, step->half_start)))
+  int rc = KVC_OK;
+#define KVC_F(D, WPG)                                                                                               \
+  KVC_DISPATCH_DTYPE(dtype, T,                                                                                      \
+                     rc = launch_after("kv4_write_kernel", kv4_write_kernel<T, D, WPG>, grid, 128, 0,               \
+                                       static_cast<cudaStream_t>(stream), L, s, static_cast<uint8_t*>(pool), in,    \
+                                       (int)step->n_halves, step->half_seq, step->half_start))
   KVC_KV4_DISPATCH(layout, KVC_F);
 #undef KVC_F
-  return check_launch("kv4_write_kernel");
+  return rc;
 }
 
 extern "C" int kvc_kv4_read(const kvc_kv4_layout* layout, const void* pool, int64_t layer_bytes, int n_layers, int row,
@@ -363,14 +403,14 @@ extern "C" int kvc_kv4_read(const kvc_kv4_layout* layout, const void* pool, int6
   if (n_layers < 0 || row < 0 || t0 < 0 || t1 < t0 || t1 > layout->table_stride * layout->page_size || t1 > INT32_MAX)
     return fail(KVC_ERR_SHAPE, "kvc_kv4_read: bad layers or token range");
   if (t0 == t1 || n_layers == 0) return KVC_OK;
-  const int64_t halves = (t1 - 1) / 8 - t0 / 8 + 1, warps = halves * layout->n_kv * 2 * n_layers;
-  const int64_t blocks = ceil_div(warps, 4);
-  if (blocks > INT32_MAX) return fail(KVC_ERR_SHAPE, "kvc_kv4_read: too many tokens in one call");
+  const int64_t halves = (t1 - 1) / 8 - t0 / 8 + 1;
+  if (layout->n_kv > 65535 || n_layers > 65535) return fail(KVC_ERR_SHAPE, "kvc_kv4_read: too many layers or KV heads");
+  const dim3 grid((unsigned)ceil_div(halves * 2, 4), (unsigned)layout->n_kv, (unsigned)n_layers);
   const Layout L = to_layout(layout);
 #define KVC_F(D, WPG)                                                                                        \
   KVC_DISPATCH_DTYPE(dtype, T,                                                                               \
-                     (kv4_read_kernel<T, D, WPG><<<(unsigned)blocks, 128, 0, static_cast<cudaStream_t>(stream)>>>( \
-                         L, static_cast<const uint8_t*>(pool), layer_bytes, row, (int)t0, (int)t1, halves, warps,  \
+                     (kv4_read_kernel<T, D, WPG><<<grid, 128, 0, static_cast<cudaStream_t>(stream)>>>(             \
+                         L, static_cast<const uint8_t*>(pool), layer_bytes, row, (int)t0, (int)t1, (int)halves,    \
                          static_cast<T*>(k_out), static_cast<T*>(v_out))))
   KVC_KV4_DISPATCH(layout, KVC_F);
 #undef KVC_F

@@ -66,23 +66,6 @@ struct Pre {
   static_assert(bytes <= 227 * 1024, "shared memory");
 };
 
-// A pair of codes as float16 c - 8: nibble 0 of each half from 1024 + c, nibble
-// 1 from 1024 + 16 c.  Both steps are exact.
-__device__ __forceinline__ __half2 centred_lo(uint32_t w) {
-  uint32_t x = (w & 0x000F000Fu) | 0x64006400u, off = 0x64086408u;  // 1032
-  __half2 h, o;
-  memcpy(&h, &x, 4);
-  memcpy(&o, &off, 4);
-  return __hsub2(h, o);
-}
-__device__ __forceinline__ __half2 centred_hi(uint32_t w) {
-  uint32_t x = (w & 0x00F000F0u) | 0x64006400u, scale = 0x2C002C00u, off = 0xD480D480u;  // 1 / 16, -72
-  __half2 h, s, o;
-  memcpy(&h, &x, 4);
-  memcpy(&s, &scale, 4);
-  memcpy(&o, &off, 4);
-  return __hfma2(h, s, o);
-}
 __device__ __forceinline__ uint32_t bits(__half2 h) {
   uint32_t r;
   memcpy(&r, &h, 4);

@@ -1,7 +1,7 @@
 // Writing, reading and moving the pages of the 4-bit KV cache.
 //
-// All three are bound by memory.  A warp of the write and read kernels takes
-// 8 tokens of one head's K or V, 4 lanes a token: lane c of a token holds the
+// All three are bound by memory.  A warp of the write kernel takes 8 tokens of
+// one head's K and V, one of the read kernel of K or V, 4 lanes a token: lane c of a token holds the
 // features 32 w + 8 c + 0..7, which is both a 16-byte load of a 16-bit input
 // (4 lanes: 64 contiguous bytes) and word w of K's chunk c, so K's codes need
 // no exchange at all and V's one shuffle a word with the neighbouring token.
@@ -28,27 +28,76 @@ namespace {
 
 // ---- element access ---------------------------------------------------------
 
-// Eight consecutive elements as float32.  vec: 16-byte aligned.
+// Eight consecutive elements: as they lie in memory (packed pairs of 16-bit
+// ones, so that a warp holds K and V at once), and as float32.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, float (&x)[8]) {
-  if (!vec) {
+struct Eight {
+  static constexpr int N = sizeof(T) * 2;  // 32-bit words
+  uint32_t r[N];
+
+  __device__ __forceinline__ void load(const T* p, bool vec) {  // vec: 16-byte aligned
+    if (vec) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = Elt<T>::to_f32(p[i]);
-    return;
-  }
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+      for (int i = 0; i < N; i += 4) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+        r[i] = a.x, r[i + 1] = a.y, r[i + 2] = a.z, r[i + 3] = a.w;
+      }
+    } else {
+      T e[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      T e[2];
-      memcpy(e, &w[i], 4);
-      x[2 * i] = Elt<T>::to_f32(e[0]);
-      x[2 * i + 1] = Elt<T>::to_f32(e[1]);
+      for (int i = 0; i < 8; ++i) e[i] = p[i];
+      memcpy(r, e, sizeof r);
     }
+  }
+  __device__ __forceinline__ void floats(float (&x)[8]) const {
+    T e[8];
+    memcpy(e, r, sizeof r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = Elt<T>::to_f32(e[i]);
+  }
+};
+
+// Smallest and largest of several Eights (NaN left out), and 0 if all are
+// finite, else NaN; 16-bit elements two at a time.
+template <typename T, int W>
+__device__ __forceinline__ void extremes(const Eight<T>* x, float& lo, float& hi, float& odd) {
+  if constexpr (sizeof(T) == 4) {
+    lo = hi = __uint_as_float(x[0].r[0]);
+    odd = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const float a = __uint_as_float(x[w].r[i]), b = __uint_as_float(x[w].r[i + 1]);
+        lo = fminf(lo, fminf(a, b));
+        hi = fmaxf(hi, fmaxf(a, b));
+        odd = fmaf(b, 0.0f, fmaf(a, 0.0f, odd));
+      }
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    T2 l, h, o, zero;
+    memcpy(&l, &x[0].r[0], 4);
+    h = l;
+    const uint32_t none = 0;
+    memcpy(&zero, &none, 4);
+    o = zero;
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        T2 v;
+        memcpy(&v, &x[w].r[i], 4);
+        l = __hmin2(l, v);
+        h = __hmax2(h, v);
+        o = __hfma2(v, zero, o);
+      }
+    T a[2];
+    memcpy(a, &l, 4);
+    lo = fminf(Elt<T>::to_f32(a[0]), Elt<T>::to_f32(a[1]));
+    memcpy(a, &h, 4);
+    hi = fmaxf(Elt<T>::to_f32(a[0]), Elt<T>::to_f32(a[1]));
+    memcpy(a, &o, 4);
+    odd = Elt<T>::to_f32(a[0]) + Elt<T>::to_f32(a[1]);
   }
 }
 
@@ -112,22 +161,29 @@ __device__ __noinline__ float code_near_half(float x, float s, float z, float t)
 
 // The word of eight elements (the first of each byte in its high nibble).
 __device__ __forceinline__ uint32_t word_of(const float (&x)[8], float s, float z, float inv15) {
-  float n[8], t[8], far = 0.0f;
+  using namespace tc;
+  const uint64_t z2 = f2_pack(-z, -z), c15 = f2_pack(15.0f, 15.0f), m15 = f2_pack(-15.0f, -15.0f),
+                 magic = f2_pack(kMagic, kMagic), unmagic = f2_pack(-kMagic, -kMagic);
+  float n[8], t[8], far = 0.0f;  // n: the codes, negative
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float v = __saturatef(fmaf(x[e] - z, inv15, 8.0f / 15.0f));
-    n[e] = fmaf(v, 15.0f, kMagic) - kMagic;
-    t[e] = v;
-    far = fmaxf(far, fabsf(fmaf(v, 15.0f, -n[e])));
+  for (int e = 0; e < 8; e += 2) {
+    float a, b;
+    f2_unpack(f2_add(f2_pack(x[e], x[e + 1]), z2), a, b);
+    t[e] = __saturatef(fmaf(a, inv15, 8.0f / 15.0f));
+    t[e + 1] = __saturatef(fmaf(b, inv15, 8.0f / 15.0f));
+    const uint64_t t2 = f2_pack(t[e], t[e + 1]), n2 = f2_add(f2_fma(t2, m15, magic), unmagic);
+    f2_unpack(n2, n[e], n[e + 1]);
+    f2_unpack(f2_fma(t2, c15, n2), a, b);
+    far = fmaxf(far, fmaxf(fabsf(a), fabsf(b)));
   }
   if (far > 0.49999f) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (fabsf(fmaf(t[e], 15.0f, -n[e])) > 0.49999f) n[e] = code_near_half(x[e], s, z, t[e] * 15.0f);
+      if (fabsf(fmaf(t[e], 15.0f, n[e])) > 0.49999f) n[e] = -code_near_half(x[e], s, z, t[e] * 15.0f);
   }
   // four codes are an integer below 2^16, exact in float32
-  const float lo = fmaf(fmaf(fmaf(n[2], 16.0f, n[3]), 16.0f, n[0]), 16.0f, n[1]) + kMagic;
-  const float hi = fmaf(fmaf(fmaf(n[6], 16.0f, n[7]), 16.0f, n[4]), 16.0f, n[5]) + kMagic;
+  const float lo = kMagic - fmaf(fmaf(fmaf(n[2], 16.0f, n[3]), 16.0f, n[0]), 16.0f, n[1]);
+  const float hi = kMagic - fmaf(fmaf(fmaf(n[6], 16.0f, n[7]), 16.0f, n[4]), 16.0f, n[5]);
   return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x5410);
 }
 
@@ -138,6 +194,55 @@ struct KvIn {
   int vec;             // 16-byte loads are aligned
 };
 
+// Quantise this lane's W words: their codes, and the parameters of its token's
+// groups.
+template <typename T, int W, int WPG>
+__device__ __forceinline__ void quantise(const Eight<T> (&x)[W], uint32_t (&word)[W], __half2 (&par)[W / WPG]) {
+#pragma unroll
+  for (int g = 0; g < W / WPG; ++g) {
+    float lo, hi, odd;
+    extremes<T, WPG>(&x[g * WPG], lo, hi, odd);
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    const bool rare = __any_sync(0xffffffffu, !(odd == 0.0f) || lo < -kLimit || hi > kLimit);
+    bool nan = false;
+    if (rare) {
+#pragma unroll
+      for (int w = 0; w < WPG; ++w) {
+        float f[8];
+        x[g * WPG + w].floats(f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) nan |= f[e] != f[e];
+      }
+      nan |= __shfl_xor_sync(0xffffffffu, (int)nan, 1) != 0;
+      nan |= __shfl_xor_sync(0xffffffffu, (int)nan, 2) != 0;
+      lo = fminf(fmaxf(lo, -kLimit), kLimit);
+      hi = fminf(fmaxf(hi, -kLimit), kLimit);
+    }
+    par[g] = params_of(lo, hi, nan);
+    const float s = __low2float(par[g]), z = __high2float(par[g]), inv15 = s > 0.0f ? rcp_approx(15.0f * s) : 0.0f;
+#pragma unroll
+    for (int w = g * WPG; w < (g + 1) * WPG; ++w) {
+      float f[8];
+      x[w].floats(f);
+      if (rare) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = fminf(fmaxf(f[e], -kLimit), kLimit);
+      }
+      word[w] = word_of(f, s, z, inv15);
+    }
+  }
+}
+
+template <int W>
+__device__ __forceinline__ void store_words(uint8_t* dst, const uint32_t (&word)[W]) {
+  if constexpr (W == 4) *reinterpret_cast<uint4*>(dst) = make_uint4(word[0], word[1], word[2], word[3]);
+  else *reinterpret_cast<uint2*>(dst) = make_uint2(word[0], word[1]);
+}
+
 // W = D / 32 words a lane; WPG words a quantisation group.
 template <typename T, int D, int WPG>
 __global__ void __launch_bounds__(128) kv4_write_kernel(Layout L, Step S, uint8_t* pool, KvIn in, int n_halves,
@@ -147,78 +252,45 @@ __global__ void __launch_bounds__(128) kv4_write_kernel(Layout L, Step S, uint8_
   grid_wait();
   grid_go();  // the attention of these tokens may get ready
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const int id = (int)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (id >= n_halves * 2) return;
-  const int is_v = id & 1, half = id >> 1, h = blockIdx.y;
+  const int half = (int)blockIdx.x * 4 + (threadIdx.x >> 5), h = blockIdx.y;
+  if (half >= n_halves) return;
   const int b = half_seq[half];
   const int len = S.kv_len[b], q0 = S.q_start[b], n = S.q_start[b + 1] - q0, first = len - n;
   const int tok0 = (first / 8 + half - half_start[b]) * 8, pos = tok0 + r;
   const bool valid = pos >= first && pos < len;
-  const int64_t page = page_of(L, S.rows[b], tok0, &tc::g_kvc_device_error);
-  if (page < 0) return;
-
-  float x[W][8];
+  Eight<T> k[W], v[W];
   if (valid) {
     const int64_t row = (int64_t)(pos - first) + (in.packed ? q0 : 0);
-    const T* src = static_cast<const T*>(is_v ? in.v : in.k) + (in.packed ? 0 : b * in.sb) + row * in.st + h * in.sh;
+    const int64_t at = (in.packed ? 0 : b * in.sb) + row * in.st + h * in.sh + 8 * c;
 #pragma unroll
-    for (int w = 0; w < W; ++w) load8(src + 32 * w + 8 * c, in.vec != 0, x[w]);
+    for (int w = 0; w < W; ++w) k[w].load(static_cast<const T*>(in.k) + at + 32 * w, in.vec != 0);
+#pragma unroll
+    for (int w = 0; w < W; ++w) v[w].load(static_cast<const T*>(in.v) + at + 32 * w, in.vec != 0);
   } else {
 #pragma unroll
     for (int w = 0; w < W; ++w)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[w][e] = 0.0f;
+      for (int i = 0; i < Eight<T>::N; ++i) k[w].r[i] = v[w].r[i] = 0;
   }
-
+  const int64_t page = page_of(L, S.rows[b], tok0, &tc::g_kvc_device_error);
+  if (page < 0) return;
   uint8_t* unit = pool + unit_off<D>(L, page, h, tok0);
   const int t = pos & 15, p = (tok0 >> 3) & 1;
   uint32_t word[W];
+  __half2 par[NG];
+
+  quantise<T, W, WPG>(k, word, par);
+  if (valid) {
+    store_words<W>(unit + k_chunk<D>(t, c), word);
+    if (c == 0)
 #pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    float lo = x[g * WPG][0], hi = lo, odd = 0.0f;  // odd: NaN where an element is NaN or infinite
-#pragma unroll
-    for (int w = g * WPG; w < (g + 1) * WPG; ++w)
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        lo = fminf(lo, fminf(x[w][e], x[w][e + 1]));
-        hi = fmaxf(hi, fmaxf(x[w][e], x[w][e + 1]));
-        odd = fmaf(x[w][e], 0.0f, odd);
-        odd = fmaf(x[w][e + 1], 0.0f, odd);
-      }
-#pragma unroll
-    for (int o = 1; o <= 2; o <<= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    bool nan = false;
-    if (__any_sync(0xffffffffu, !(odd == 0.0f) || lo < -kLimit || hi > kLimit)) {
-#pragma unroll
-      for (int w = g * WPG; w < (g + 1) * WPG; ++w)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          nan |= x[w][e] != x[w][e];
-          x[w][e] = fminf(fmaxf(x[w][e], -kLimit), kLimit);
-        }
-      nan |= __shfl_xor_sync(0xffffffffu, (int)nan, 1) != 0;
-      nan |= __shfl_xor_sync(0xffffffffu, (int)nan, 2) != 0;
-      lo = fminf(fmaxf(lo, -kLimit), kLimit);
-      hi = fminf(fmaxf(hi, -kLimit), kLimit);
-    }
-    const __half2 sz = params_of(lo, hi, nan);
-    const float s = __low2float(sz), z = __high2float(sz), inv15 = s > 0.0f ? rcp_approx(15.0f * s) : 0.0f;
-#pragma unroll
-    for (int w = g * WPG; w < (g + 1) * WPG; ++w) word[w] = word_of(x[w], s, z, inv15);
-    if (valid && c == 0)
-      reinterpret_cast<__half2*>(unit + (is_v ? vp_base(D, NG) : kp_base(D)))[t * NG + g] = sz;
+      for (int g = 0; g < NG; ++g) reinterpret_cast<__half2*>(unit + kp_base(D))[t * NG + g] = par[g];
   }
 
-  if (!is_v) {
-    if (!valid) return;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(unit + k_chunk<D>(t, c));
-    if constexpr (W == 4) *reinterpret_cast<uint4*>(dst) = make_uint4(word[0], word[1], word[2], word[3]);
-    else *reinterpret_cast<uint2*>(dst) = make_uint2(word[0], word[1]);
-    return;
-  }
+  quantise<T, W, WPG>(v, word, par);
+  if (valid && c == 0)
+#pragma unroll
+    for (int g = 0; g < NG; ++g) reinterpret_cast<__half2*>(unit + vp_base(D, NG))[t * NG + g] = par[g];
   const int cc = r >> 1, odd = r & 1;
   if (tok0 >= first && tok0 + 8 <= len) {
     // token pairs are neighbouring lanes (lane ^ 4): the even token's lane
@@ -228,9 +300,7 @@ __global__ void __launch_bounds__(128) kv4_write_kernel(Layout L, Step S, uint8_
       const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? word[w] & 0xFFFFu : word[w] >> 16, 4);
       word[w] = odd ? got | (word[w] & 0xFFFF0000u) : (word[w] & 0xFFFFu) | got << 16;
     }
-    uint32_t* dst = reinterpret_cast<uint32_t*>(unit + v_chunk<D>(p, (2 * c + odd) * 4 + cc));
-    if constexpr (W == 4) *reinterpret_cast<uint4*>(dst) = make_uint4(word[0], word[1], word[2], word[3]);
-    else *reinterpret_cast<uint2*>(dst) = make_uint2(word[0], word[1]);
+    store_words<W>(unit + v_chunk<D>(p, (2 * c + odd) * 4 + cc), word);
   } else if (valid) {
     // other tokens of the half keep their codes: two bytes hold four features
     // of one token
@@ -375,7 +445,7 @@ extern "C" int kvc_kv4_write(const kvc_kv4_layout* layout, const kvc_kv4_step* s
   if (!k || !v) return fail(KVC_ERR_ARG, "kvc_kv4_write: NULL pointer");
   if (step->n_halves > INT32_MAX / 4 || layout->n_kv > 65535)
     return fail(KVC_ERR_SHAPE, "kvc_kv4_write: too many tokens or KV heads in one call");
-  const dim3 grid((unsigned)ceil_div(step->n_halves * 2, 4), (unsigned)layout->n_kv);
+  const dim3 grid((unsigned)ceil_div(step->n_halves, 4), (unsigned)layout->n_kv);
   const int64_t e = (int64_t)dtype_size(dtype);
   const bool vec = aligned16(k) && aligned16(v) && (seq_stride * e) % 16 == 0 && (token_stride * e) % 16 == 0 &&
                    (head_stride * e) % 16 == 0;

@@ -332,6 +332,11 @@ int kvc_set_kernel_policy(int policy);
  * the device: token t of row r is in page table[r][t / page_size].  An entry
  * that is no page sets the device error word (401); it is never followed, and
  * what stands for its tokens is not defined.
+ *
+ * The table and the arrays of kvc_kv4_step and kvc_kv4_split are written by
+ * copies (cudaMemcpyAsync): the kernels may read them before the kernel in
+ * front of them in the stream has ended, if that one allows it (programmatic
+ * dependent launch).
  */
 typedef struct {
   const int32_t* table;

@@ -98,9 +98,12 @@ __device__ __forceinline__ __half2 centred_hi(uint32_t w) {
 }
 // Programmatic launches: a kernel launched with launch_after may start while
 // the previous one of its stream runs; grid_wait returns when that one is
-// complete and its writes are visible, and comes before everything else in
-// every thread.  grid_go lets the next such kernel start (its grid_wait still
-// waits for this grid's end).
+// complete and its writes are visible.  Every thread comes by it, before it
+// ends too, so that a kernel's end is also the end of those before it.  Only a
+// step's own arrays and the page table are read earlier: they are written by
+// copies.  grid_go lets the next such kernel start (its grid_wait still waits
+// for this grid's end); it comes after grid_wait, so that no more than two
+// kernels are under way.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -149,18 +149,20 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[WARPS][STAGES];
 
-  grid_wait();
-  grid_go();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int item = blockIdx.x, h = blockIdx.y, col0 = blockIdx.z * COLS;
   const int4 it = P.items[item];
   const int b = it.x, t_begin = it.y, len = it.w;
   const int q0 = S.q_start[b], n = S.q_start[b + 1] - q0, group = a.n_q / L.n_kv;
   const int cols = n * group;
-  if (col0 >= cols) return;
   const int last = min(col0 + COLS, cols) - 1;
-  const int t_end = min(t_begin + P.chunk, visible(a.causal, len, n, last / group));
-  if (t_begin > 0 && t_begin >= t_end) return;  // nothing of this item is seen: the join knows
+  const int t_end = min(t_begin + P.chunk, visible(a.causal, len, n, max(last, 0) / group));
+  // no such columns, or nothing of this item is seen: the join knows
+  if (col0 >= cols || (t_begin > 0 && t_begin >= t_end)) {
+    grid_wait();
+    grid_go();
+    return;
+  }
   const int t_free = visible(a.causal, len, n, col0 / group);  // below it no column masks anything
 
   if (lane == 0)
@@ -175,16 +177,17 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
   const int mine = runs > warp ? (runs - warp + WARPS - 1) / WARPS : 0;
   const uint32_t ring = tc::smem_u32(smem) + warp * STAGES * Sm::stage + (lane % UNITS) * UB;
   const uint8_t* src = nullptr;
-  auto issue = [&](int i, int stage) {
-    if (i % AHEAD == 0) {  // pages of runs i .. i + AHEAD - 1
-      const int t = t_begin + (warp + (i + lane / UNITS) * WARPS) * TOKENS + (lane % UNITS) * kUnit;
-      src = nullptr;
-      if (t < t_end) {
-        const int64_t page = page_of(L, it.z, t, &tc::g_kvc_device_error);
-        // a bad entry reads page 0: its place in the sum is wrong, but in range
-        src = pool + unit_off<D>(L, page < 0 ? 0 : page, h, t);
-      }
+  auto look = [&](int i) {  // pages of runs i .. i + AHEAD - 1
+    const int t = t_begin + (warp + (i + lane / UNITS) * WARPS) * TOKENS + (lane % UNITS) * kUnit;
+    src = nullptr;
+    if (t < t_end) {
+      const int64_t page = page_of(L, it.z, t, &tc::g_kvc_device_error);
+      // a bad entry reads page 0: its place in the sum is wrong, but in range
+      src = pool + unit_off<D>(L, page < 0 ? 0 : page, h, t);
     }
+  };
+  auto issue = [&](int i, int stage) {
+    if (i % AHEAD == 0 && i > 0) look(i);
     if (lane / UNITS == i % AHEAD) {
       uint64_t* bar = &full[warp][stage];
       if (src) {
@@ -195,6 +198,10 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
       }
     }
   };
+  look(0);
+  // (what was read so far is the step's own arrays and the page table)
+  grid_wait();
+  grid_go();
   for (int i = 0; i < STAGES && i < mine; ++i) issue(i, i);
 
   // ---- queries: lane (r, c) holds features 32 w + 8 c + 0..7 of column r of each tile
@@ -583,18 +590,18 @@ __global__ void __launch_bounds__(128) attend_join_kernel(Layout L, Step S, Spli
   constexpr int T = D / 4, G = 128 / T, STEP = WIDE ? G : 1;
   __shared__ float4 so[G][T];
   __shared__ float ss[G];
-  grid_wait();
   const int g = threadIdx.x / T, x = threadIdx.x % T;
   const int64_t id = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * G + g;
-  if (id >= rows) return;
+  if (id >= rows) return grid_wait();
   const int tok = (int)(id / a.n_q), head = (int)(id % a.n_q);
   const int b = seq_of(S, tok), i0 = P.item_start[b], i1 = P.item_start[b + 1];
-  if (i1 - i0 == 1) return;
+  if (i1 - i0 == 1) return grid_wait();
   const int q0 = S.q_start[b], n = S.q_start[b + 1] - q0, j = tok - q0, group = a.n_q / L.n_kv;
   const int vis = visible(a.causal, S.kv_len[b], n, j), h = head / group;
   // items past what the query sees hold nothing of it; the first always holds something
   const int items = max(1, min(i1 - i0, (vis + P.chunk - 1) / P.chunk));
   const int64_t at0 = ((int64_t)i0 * L.n_kv + h) * part.cols + j * group + head % group, step = L.n_kv * part.cols;
+  grid_wait();
   float top = -INFINITY;
   for (int i = x; i < items; i += T) top = fmaxf(top, part.ml[at0 + i * step].x);
 #pragma unroll
@@ -653,9 +660,11 @@ int join(const Layout& L, const Step& S, const Split& P, const Qkv& a, const Par
 constexpr int kFewColumns = 32;
 bool many(int64_t cols, int dtype) { return dtype != KVC_F32 && cols > kFewColumns; }
 
-// Tiles of 8 columns a block takes: as many as there are, up to what the
-// registers hold (4 with one float16 term and one group a head, else 2).
-int tiles_of(int cols, int terms, int groups) { return cols <= 8 ? 1 : cols <= 16 || terms == 2 || groups > 1 ? 2 : 4; }
+// Tiles of 8 columns a block takes.  Four, with 8 warps an SM for their
+// registers, were slower than two blocks of two that read the codes twice
+// (32 columns over 8 x 8192 tokens of 8 KV heads, d = 128: 66.5 against 57.4 us;
+// d = 64, 4 KV heads: 27.1 against 25.8 us).
+int tiles_of(int cols) { return cols <= 8 ? 1 : 2; }
 
 template <int D, int WPG, int NT, int TERMS>
 int launch(const Layout& L, const Step& S, const Split& P, const void* pool, const Qkv& a, const Partial& part,
@@ -672,17 +681,14 @@ int launch(const Layout& L, const Step& S, const Split& P, const void* pool, con
 template <int D, int WPG>
 int launch_tiles(const Layout& L, const Step& S, const Split& P, const void* pool, const Qkv& a, const Partial& part,
                  int64_t n_items, int cols, cudaStream_t st) {
-  const int terms = a.dtype == KVC_F32 ? 2 : 1, nt = tiles_of(cols, terms, D / 32 / WPG);
+  const int terms = a.dtype == KVC_F32 ? 2 : 1, nt = tiles_of(cols);
   const int tiles = (int)ceil_div(cols, 8 * nt);
   if (tiles > 65535 || L.n_kv > 65535) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: too many queries or KV heads");
   if (terms == 2)
     return nt == 1 ? launch<D, WPG, 1, 2>(L, S, P, pool, a, part, n_items, tiles, st)
                    : launch<D, WPG, 2, 2>(L, S, P, pool, a, part, n_items, tiles, st);
-  if (nt == 1) return launch<D, WPG, 1, 1>(L, S, P, pool, a, part, n_items, tiles, st);
-  if constexpr (D / 32 == WPG) {
-    if (nt == 4) return launch<D, WPG, 4, 1>(L, S, P, pool, a, part, n_items, tiles, st);
-  }
-  return launch<D, WPG, 2, 1>(L, S, P, pool, a, part, n_items, tiles, st);
+  return nt == 1 ? launch<D, WPG, 1, 1>(L, S, P, pool, a, part, n_items, tiles, st)
+                 : launch<D, WPG, 2, 1>(L, S, P, pool, a, part, n_items, tiles, st);
 }
 
 }  // namespace
@@ -704,13 +710,12 @@ extern "C" int kvc_kv4_attend_shape(const kvc_kv4_layout* layout, const kvc_kv4_
     *resident = num_sms();
     return KVC_OK;
   }
-  const int terms = dtype == KVC_F32 ? 2 : 1, nt = tiles_of((int)cols, terms, layout->head_dim / layout->group_size);
+  const int terms = dtype == KVC_F32 ? 2 : 1, nt = tiles_of((int)cols);
   *tiles = (int)ceil_div(cols, 8 * nt);
   int blocks = 0;
 #define KVC_F(D, WPG)                                                                                    \
   blocks = terms == 2 ? (nt == 1 ? Shape<D, WPG, 1, 2>::blocks : Shape<D, WPG, 2, 2>::blocks)            \
-                      : (nt == 1 ? Shape<D, WPG, 1, 1>::blocks                                           \
-                                 : nt == 2 ? Shape<D, WPG, 2, 1>::blocks : Shape<D, WPG, 4, 1>::blocks)
+                      : (nt == 1 ? Shape<D, WPG, 1, 1>::blocks : Shape<D, WPG, 2, 1>::blocks)
   KVC_KV4_DISPATCH(layout, KVC_F);
 #undef KVC_F
   *resident = blocks * num_sms();

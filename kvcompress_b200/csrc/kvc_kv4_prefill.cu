@@ -146,17 +146,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = Pre<D, WPG>;
   constexpr int W = C::W, NG = C::NG;
   extern __shared__ __align__(1024) uint8_t smem[];
-  grid_wait();
-  grid_go();
   const int4 it = P.items[blockIdx.z];
   const int b = it.x, t_begin = it.y, len = it.w, h = blockIdx.y;
   const int q0 = S.q_start[b], n = S.q_start[b + 1] - q0, group = a.n_q / L.n_kv, rows = n * group;
   // late rows see the most tokens: they go first
   const int tiles = (rows + 2 * kTile - 1) / (2 * kTile), tile = tiles - 1 - (int)blockIdx.x;
-  if (tile < 0) return;
   const int row0 = tile * 2 * kTile, last = min(row0 + 2 * kTile, rows) - 1;
-  const int t_end = min(t_begin + P.chunk, visible(a.causal, len, n, last / group));
-  if (t_begin > 0 && t_begin >= t_end) return;  // nothing of this item is seen: the join knows
+  const int t_end = min(t_begin + P.chunk, visible(a.causal, len, n, max(last, 0) / group));
+  // no such rows, or nothing of this item is seen: the join knows
+  if (tile < 0 || (t_begin > 0 && t_begin >= t_end)) {
+    grid_wait();
+    grid_go();
+    return;
+  }
   const int steps = t_end > t_begin ? (t_end - t_begin + kTile - 1) / kTile : 0;
   const int halves = row0 + kTile < rows ? 2 : 1;  // row tiles with rows
 
@@ -180,6 +182,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *holder;
+  // (what was read so far is the step's own arrays)
+  grid_wait();
+  grid_go();
 
   // registers: 8 x 192 + 4 x 88 + 4 x 40 a lane = 16 x 128, what the block was launched with
   if (warp < 8) {

@@ -30,6 +30,45 @@ __all__ = ["CacheStep", "PagedKVCache"]
 _CHUNK = 256  # tokens of the smallest item of the attention's split
 
 
+class _Upload:
+    """int32 arrays in one device buffer, copied from pinned memory on the
+    current stream (torch keeps that until the copy is done).
+
+    Kernels index with these arrays, so on whatever stream one is launched, it
+    has to come after the copy, and the buffer must not be reused before it."""
+
+    __slots__ = ("buf", "at", "streams", "event")
+
+    def __init__(self, arrays: Sequence[np.ndarray], device: torch.device) -> None:
+        host = torch.empty(max(1, sum(a.size for a in arrays)), dtype=torch.int32, pin_memory=True)
+        view, n, offsets = host.numpy(), 0, []
+        for a in arrays:
+            view[n:n + a.size] = a
+            offsets.append(n)
+            n += a.size
+        with torch.cuda.device(device):
+            self.buf = host.to(device, non_blocking=True)
+            self.event = torch.cuda.Event()
+            self.event.record()
+        self.at = [self.buf.data_ptr() + 4 * o for o in offsets]  # the arrays' addresses
+        self.streams = {ops._raw_stream(device.index)}  # streams that are behind the copy
+
+    def use(self, stream: int) -> None:
+        """Put the raw ``stream``, the device's current one, behind the copy."""
+        if stream not in self.streams:
+            self._join(stream)
+
+    def _join(self, stream: int) -> None:
+        # a stream under capture cannot wait for one outside; its graph runs after
+        # whatever the program made sure was done before
+        if torch.cuda.is_current_stream_capturing():
+            return
+        cur = torch.cuda.current_stream(self.buf.device)
+        cur.wait_event(self.event)
+        self.buf.record_stream(cur)
+        self.streams.add(stream)
+
+
 @dataclass
 class CacheStep:
     """The new tokens, or the queries, of some sequences: made by
@@ -45,26 +84,13 @@ class CacheStep:
     writable: bool
     epoch: int
     cache: Any = field(repr=False)
-    meta: torch.Tensor = field(repr=False)  # device arrays that ``desc`` points into
+    meta: _Upload = field(repr=False)  # the arrays that ``desc`` points into
     desc: Kv4Step = field(repr=False)
-    splits: dict[tuple[int, int], tuple[tuple[Kv4Split, int], torch.Tensor]] = field(default_factory=dict, repr=False)
+    splits: dict[tuple[int, int], tuple[Kv4Split, int, _Upload]] = field(default_factory=dict, repr=False)
 
     @property
     def tokens(self) -> int:
         return int(self.desc.n_tokens)
-
-
-def _upload(arrays: Sequence[np.ndarray], device: torch.device) -> tuple[torch.Tensor, list[int]]:
-    """int32 arrays in one device buffer (one asynchronous copy from pinned
-    memory, which torch keeps until the copy is done) and their addresses."""
-    host = torch.empty(max(1, sum(a.size for a in arrays)), dtype=torch.int32, pin_memory=True)
-    view, at, offsets = host.numpy(), 0, []
-    for a in arrays:
-        view[at:at + a.size] = a
-        offsets.append(at)
-        at += a.size
-    buf = host.to(device, non_blocking=True)
-    return buf, [buf.data_ptr() + 4 * o for o in offsets]
 
 
 def _prefix(counts: np.ndarray) -> np.ndarray:
@@ -215,8 +241,8 @@ class PagedKVCache:
             halves = np.where(n > 0, (lengths - 1) // 8 - (lengths - n) // 8 + 1, 0)
         q_start, half_start = _prefix(n), _prefix(halves)
         half_seq = np.repeat(np.arange(len(seqs)), halves)
-        meta, at = _upload((rows, lengths, q_start, half_seq, half_start), self.device)
-        desc = Kv4Step(at[0], at[1], at[2], at[3], at[4], int(half_start[-1]), len(seqs), int(n.max(initial=0)),
+        meta = _Upload((rows, lengths, q_start, half_seq, half_start), self.device)
+        desc = Kv4Step(*meta.at, int(half_start[-1]), len(seqs), int(n.max(initial=0)),
                        int(q_start[-1]))
         return CacheStep(seqs, counts, lengths.tolist(), writable, self.pages.epoch, self, meta, desc)
 
@@ -231,11 +257,11 @@ class PagedKVCache:
             seq = np.repeat(np.arange(len(step.seqs)), items)
             rows = np.array([self.pages.row(s) for s in step.seqs], dtype=np.int64)
             table = np.stack((seq, (np.arange(int(start[-1])) - start[seq]) * chunk, rows[seq], lengths[seq]), 1)
-            buf, at = _upload((table.reshape(-1), start), self.device)
-            split = Kv4Split(at[0], at[1], int(start[-1]), chunk, int(items.max(initial=1)))
-            got = (split, ops.kv4_attend_workspace(self._layout, step.desc, split, n_q)), buf
-            step.splits[n_q, code] = got
-        return got[0]
+            up = _Upload((table.reshape(-1), start), self.device)
+            split = Kv4Split(*up.at, int(start[-1]), chunk, int(items.max(initial=1)))
+            got = step.splits[n_q, code] = (split, ops.kv4_attend_workspace(self._layout, step.desc, split, n_q), up)
+        got[2].use(ops._raw_stream(self.device.index))
+        return got[0], got[1]
 
     def _check(self, what: str, layer: int, step: CacheStep) -> int:
         if step.cache is not self:
@@ -245,6 +271,7 @@ class PagedKVCache:
                                "step was made; make it again")
         if not 0 <= layer < self.n_layers:
             raise IndexError(f"PagedKVCache.{what}: layer {layer} of {self.n_layers}")
+        step.meta.use(ops._raw_stream(self.device.index))
         return self._layers[layer]
 
     # ---- data ---------------------------------------------------------------

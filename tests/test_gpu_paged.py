@@ -576,6 +576,29 @@ def test_another_stream():
     check_attend(c, q, c.view([s], [1]), [(k, v)])
 
 
+def test_a_step_used_on_another_stream_waits_for_its_arrays():
+    """The step's stream is busy when another one uses the step, and the step is
+    dropped and its memory overwritten while that one still works."""
+    c = make(2, 128, 128, 64, 40960, 2, pages=700)
+    s = c.add()
+    k, v = cells(30000, 2, 128, BF16)
+    q = queries(1, 4, 128, BF16)
+    c.write(0, k, v, c.extend([s], [30000]))
+    want = c.attend(0, q, c.view([s], [1]))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    torch.cuda._sleep(20_000_000)  # about 10 ms on the current stream
+    step = c.view([s], [1])
+    with torch.cuda.stream(side):
+        outs = [c.attend(0, q, step) for _ in range(50)]
+    del step
+    for _ in range(20):
+        torch.full((64,), 1 << 20, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    assert ops.device_error() == 0
+
+
 def test_a_bad_page_is_reported_and_skipped():
     c = make(1, 64, 64, 16, 64, 2)
     s = c.add()

@@ -140,7 +140,7 @@ def test_split_chunk_covers_and_bounds():
     for lens, copies in (([1], 1), ([0, 0], 8), ([17], 4), ([32768] * 8, 8), ([131072] * 4, 4), ([5] * 999, 64),
                          ([2 ** 31 - 300], 1), (list(range(0, 8191, 253)), 8)):
         chunk = split_chunk(np.array(lens, dtype=np.int64), copies, 296)
-        assert chunk % 128 == 0 and 256 <= chunk < 2 ** 31
+        assert chunk % 128 == 0 and 128 <= chunk < 2 ** 31
 
 
 @pytest.mark.parametrize("kw, err", [

@@ -317,6 +317,9 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
       uint32_t k0[W], k1[W];
       lds_words<W>(unit + k_chunk<D>(r, c), k0);
       lds_words<W>(unit + k_chunk<D>(r + 8, c), k1);
+      uint32_t kp0[NG], kp1[NG];  // (scale, zero) of the rows' groups
+      lds_words<NG>(unit + kp_base(D) + r * NG * 4, kp0);
+      lds_words<NG>(unit + kp_base(D) + (r + 8) * NG * 4, kp1);
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         float acc[NT][4];
@@ -350,8 +353,7 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
             x1 >>= 8;
           }
         }
-        const float2 p0 = lds_half2(unit + kp_base(D) + (r * NG + g) * 4);
-        const float2 p1 = lds_half2(unit + kp_base(D) + ((r + 8) * NG + g) * 4);
+        const float2 p0 = unpack_half2(kp0[g]), p1 = unpack_half2(kp1[g]);
         const float off0 = CENTRED ? p0.y : fmaf(-8.0f, p0.x, p0.y), off1 = CENTRED ? p1.y : fmaf(-8.0f, p1.x, p1.y);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -382,14 +384,17 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
 #pragma unroll
     for (int u = 0; u < SUB; ++u)
 #pragma unroll
-      for (int i2 = 0; i2 < 2; ++i2)
+      for (int i2 = 0; i2 < 2; ++i2) {
+        uint32_t words[NG];
+        lds_words<NG>(sub + u * UB + vp_base(D, NG) + (r + 8 * i2) * NG * 4, words);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          float2 p = lds_half2(sub + u * UB + vp_base(D, NG) + ((r + 8 * i2) * NG + g) * 4);
+          float2 p = unpack_half2(words[g]);
           if (MASKED && ts + u * kUnit + r + 8 * i2 >= t_end) p = make_float2(0.0f, 0.0f);
           vp[u][i2][g] = p;
           vtop = fmaxf(vtop, p.x);
         }
+      }
     bool raise = vtop > cap;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) raise |= top[nt][0] > mt[nt][0] || top[nt][1] > mt[nt][1];

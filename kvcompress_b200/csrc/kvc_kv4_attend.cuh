@@ -56,13 +56,10 @@ __device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[W]) {
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
                  : "r"(addr));
-  else
+  else if constexpr (W == 2)
     asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
-}
-__device__ __forceinline__ float2 lds_half2(uint32_t addr) {
-  uint32_t r;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(addr));
-  return unpack_half2(r);
+  else
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
 }
 
 // Tokens that query j of n sees of len.

@@ -396,96 +396,108 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
     for (int k = 0; k < 4; ++k) v_dst[k] = base + C::v + sw128_off(4 * r + k, 8 * q8, D);
 
-    for (int step = 0; step < steps; ++step) {
-      const int rs = step % C::RAWS, buf = step & 1, t0 = t_begin + step * kTile;
-      const uint32_t raw = rs * C::RAW, tile_at = buf * C::TILE;
-      ok = mbar_wait(&bars[C::raw_full + rs], (step / C::RAWS) & 1, 420);
-      if (ok && step >= 2) ok = mbar_wait(&bars[C::k_empty + buf], ((step >> 1) + 1) & 1, 421);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      // flags of the tokens whose values are NaN
-      bool dirty = t0 + kTile > t_end;
+    // K goes one tile ahead of V where two tiles of codes fit: the scores of the next
+    // tile are issued before the product with this one's V.
+    bool dirty_before = false;
+    for (int it = 0; it < steps + C::RAWS - 1; ++it) {
+      bool dirty = false;
+      if (it < steps) {
+        const int step = it, rs = step % C::RAWS, buf = step & 1, t0 = t_begin + step * kTile;
+        const uint32_t raw = rs * C::RAW, tile_at = buf * C::TILE;
+        ok = mbar_wait(&bars[C::raw_full + rs], (step / C::RAWS) & 1, 420);
+        if (ok && step >= 2) ok = mbar_wait(&bars[C::k_empty + buf], ((step >> 1) + 1) & 1, 421);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        // flags of the tokens whose values are NaN
+        dirty = t0 + kTile > t_end;
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int tok = 32 * k + lane;
-          const uint32_t p = lds32(base + C::raw + raw + (tok >> 4) * C::UB + vp_base(D, NG) + ((tok & 15) * NG + g) * 4);
-          const bool nan = __hisnan(__low2half(half2_of(p))) || __hisnan(__high2half(half2_of(p)));
-          const uint32_t fl = __ballot_sync(0xffffffffu, nan && t0 + tok < t_end);
-          dirty |= fl != 0;
-          if (threadIdx.x == 8 * 32)
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + C::flags + ((step % C::FLAGS) * NG + g) * 16 + k * 4), "r"(fl)
-                         : "memory");
-        }
-#pragma unroll
-      for (int rep = 0; rep < 4; ++rep) {
-        uint32_t x[W];
-        lds_words<W>(k_src + raw + rep * 2 * C::UB, x);
-        __half2 s2, z2;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          if (w % WPG == 0) {
-            const __half2 sz = half2_of(lds32(kp_src + raw + rep * 2 * C::UB + w / WPG * 4));
-            s2 = __low2half2(sz), z2 = __high2half2(sz);
-          }
-          const uint32_t y = x[w] >> 8;
-          sts128(k_dst[w & 1] + tile_at + (w >> 1) * (kTile * 128) + rep * 4096, bits(__hfma2(centred_lo(x[w]), s2, z2)),
-                 bits(__hfma2(centred_hi(x[w]), s2, z2)), bits(__hfma2(centred_lo(y), s2, z2)),
-                 bits(__hfma2(centred_hi(y), s2, z2)));
-        }
-      }
-      fence_async_smem();
-      mbar_arrive(&bars[C::k_full + buf]);
-
-      if (step >= 2) ok = mbar_wait(&bars[C::v_empty + buf], ((step >> 1) + 1) & 1, 422);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      uint32_t x[4][W];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) lds_words<W>(v_src + raw + k * (v_chunk<D>(0, 1) - v_chunk<D>(0, 0)), x[k]);
-      __half2 s2[4], z2[4];
-#pragma unroll
-      for (int u = 0; u < W; ++u) {
-        if (u % WPG == 0) {
-          uint32_t p[8];
-          if constexpr (NG == 1) {
-            uint32_t p0[4], p1[4];
-            lds_words<4>(vp_src + raw, p0);
-            lds_words<4>(vp_src + raw + 16, p1);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) p[k] = p0[k], p[4 + k] = p1[k];
-          } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) p[k] = lds32(vp_src + raw + (k * NG + u / WPG) * 4);
-          }
-          if (dirty) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const __half2 h = half2_of(p[k]);
-              if (__hisnan(__low2half(h)) || __hisnan(__high2half(h)) || t0 + 8 * q8 + k >= t_end) p[k] = 0;
-            }
-          }
+        for (int g = 0; g < NG; ++g)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            s2[k] = __lows2half2(half2_of(p[2 * k]), half2_of(p[2 * k + 1]));
-            z2[k] = __highs2half2(half2_of(p[2 * k]), half2_of(p[2 * k + 1]));
+            const int tok = 32 * k + lane;
+            const uint32_t p = lds32(base + C::raw + raw + (tok >> 4) * C::UB + vp_base(D, NG) + ((tok & 15) * NG + g) * 4);
+            const bool nan = __hisnan(__low2half(half2_of(p))) || __hisnan(__high2half(half2_of(p)));
+            const uint32_t fl = __ballot_sync(0xffffffffu, nan && t0 + tok < t_end);
+            dirty |= fl != 0;
+            if (threadIdx.x == 8 * 32)
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + C::flags + ((step % C::FLAGS) * NG + g) * 16 + k * 4), "r"(fl)
+                           : "memory");
+          }
+#pragma unroll
+        for (int rep = 0; rep < 4; ++rep) {
+          uint32_t x[W];
+          lds_words<W>(k_src + raw + rep * 2 * C::UB, x);
+          __half2 s2, z2;
+#pragma unroll
+          for (int w = 0; w < W; ++w) {
+            if (w % WPG == 0) {
+              const __half2 sz = half2_of(lds32(kp_src + raw + rep * 2 * C::UB + w / WPG * 4));
+              s2 = __low2half2(sz), z2 = __high2half2(sz);
+            }
+            const uint32_t y = x[w] >> 8;
+            sts128(k_dst[w & 1] + tile_at + (w >> 1) * (kTile * 128) + rep * 4096, bits(__hfma2(centred_lo(x[w]), s2, z2)),
+                   bits(__hfma2(centred_hi(x[w]), s2, z2)), bits(__hfma2(centred_lo(y), s2, z2)),
+                   bits(__hfma2(centred_hi(y), s2, z2)));
           }
         }
-        // nibbles 0..3 are features 1, 0, 3, 2
-        uint32_t o[4][4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t y = x[k][u] >> 8;
-          o[1][k] = bits(__hfma2(centred_lo(x[k][u]), s2[k], z2[k]));
-          o[0][k] = bits(__hfma2(centred_hi(x[k][u]), s2[k], z2[k]));
-          o[3][k] = bits(__hfma2(centred_lo(y), s2[k], z2[k]));
-          o[2][k] = bits(__hfma2(centred_hi(y), s2[k], z2[k]));
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) sts128(v_dst[k] + tile_at + u * 4096, o[k][0], o[k][1], o[k][2], o[k][3]);
+        fence_async_smem();
+        mbar_arrive(&bars[C::k_full + buf]);
       }
-      mbar_arrive(&bars[C::raw_empty + rs]);
-      fence_async_smem();
-      mbar_arrive(&bars[C::v_full + buf]);
+      const int step = it - (C::RAWS - 1);
+      if (step >= 0) {
+        const int rs = step % C::RAWS, buf = step & 1, t0 = t_begin + step * kTile;
+        const uint32_t raw = rs * C::RAW, tile_at = buf * C::TILE;
+        const bool check = C::RAWS > 1 ? dirty_before : dirty;
+        if (step >= 2) ok = mbar_wait(&bars[C::v_empty + buf], ((step >> 1) + 1) & 1, 422);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        uint32_t x[4][W];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) lds_words<W>(v_src + raw + k * (v_chunk<D>(0, 1) - v_chunk<D>(0, 0)), x[k]);
+        __half2 s2[4], z2[4];
+#pragma unroll
+        for (int u = 0; u < W; ++u) {
+          if (u % WPG == 0) {
+            uint32_t p[8];
+            if constexpr (NG == 1) {
+              uint32_t p0[4], p1[4];
+              lds_words<4>(vp_src + raw, p0);
+              lds_words<4>(vp_src + raw + 16, p1);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) p[k] = p0[k], p[4 + k] = p1[k];
+            } else {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) p[k] = lds32(vp_src + raw + (k * NG + u / WPG) * 4);
+            }
+            if (check) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const __half2 h = half2_of(p[k]);
+                if (__hisnan(__low2half(h)) || __hisnan(__high2half(h)) || t0 + 8 * q8 + k >= t_end) p[k] = 0;
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              s2[k] = __lows2half2(half2_of(p[2 * k]), half2_of(p[2 * k + 1]));
+              z2[k] = __highs2half2(half2_of(p[2 * k]), half2_of(p[2 * k + 1]));
+            }
+          }
+          // nibbles 0..3 are features 1, 0, 3, 2
+          uint32_t o[4][4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t y = x[k][u] >> 8;
+            o[1][k] = bits(__hfma2(centred_lo(x[k][u]), s2[k], z2[k]));
+            o[0][k] = bits(__hfma2(centred_hi(x[k][u]), s2[k], z2[k]));
+            o[3][k] = bits(__hfma2(centred_lo(y), s2[k], z2[k]));
+            o[2][k] = bits(__hfma2(centred_hi(y), s2[k], z2[k]));
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) sts128(v_dst[k] + tile_at + u * 4096, o[k][0], o[k][1], o[k][2], o[k][3]);
+        }
+        mbar_arrive(&bars[C::raw_empty + rs]);
+        fence_async_smem();
+        mbar_arrive(&bars[C::v_full + buf]);
+      }
+      dirty_before = dirty;
     }
   } else {
     fewer_registers<40>();

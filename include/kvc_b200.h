@@ -361,16 +361,19 @@ typedef struct {
 } kvc_kv4_step;
 
 /*
- * Split of the cached tokens into items of `chunk` tokens (a multiple of 128)
- * for kvc_kv4_attend, device arrays of int32: items[4 j ..] (16-byte aligned) are
- * item j's sequence i, its first token, rows[i] and kv_len[i]; it covers `chunk`
- * tokens from the first one on.  The items of sequence i are item_start[i] ..
- * item_start[i + 1] - 1, at least one.  max_items: most items of one sequence.
+ * Split of the cached tokens into items for kvc_kv4_attend, device arrays of
+ * int32.  items[4 j ..] (16-byte aligned): item j's sequence i, its first token
+ * (a multiple of 128), the token after its last, and rows[i].  The items of
+ * sequence i are item_start[i] .. item_start[i + 1] - 1; they follow one another
+ * and cover its kv_len[i] tokens, and there is at least one.  max_items: most
+ * items of one sequence.  block_start (n_blocks + 1): the items that block k
+ * works on are block_start[k] .. block_start[k + 1] - 1; used where
+ * kvc_kv4_attend_shape says `spanning`, else every item is a block.
  */
 typedef struct {
-  const int32_t *items, *item_start;
-  int64_t n_items;
-  int32_t chunk, max_items;
+  const int32_t *items, *item_start, *block_start;
+  int64_t n_items, n_blocks;
+  int32_t max_items;
 } kvc_kv4_split;
 
 int64_t kvc_kv4_page_bytes(int n_kv, int head_dim, int page_size, int group_size);
@@ -393,10 +396,11 @@ int kvc_kv4_read(const kvc_kv4_layout* layout, const void* pool, int64_t layer_b
  * over their sequences' pages.  causal: query i of a sequence's n sees the
  * first kv_len - n + 1 + i tokens, otherwise all kv_len.  A query that sees
  * nothing gets zeros.  Strides in elements, as for kvc_kv4_write. */
-/* For choosing the split: the blocks that work on one item of one KV head
- * (tiles) and the blocks that the current device runs at once (resident). */
+/* For choosing the split: the blocks that work on one item of one KV head, each
+ * with other columns (tiles), the blocks that the current device runs at once
+ * (resident), and whether a block may work on several items (spanning). */
 int kvc_kv4_attend_shape(const kvc_kv4_layout* layout, const kvc_kv4_step* step, int n_q, int dtype, int* tiles,
-                         int* resident);
+                         int* resident, int* spanning);
 size_t kvc_kv4_attend_workspace_bytes(const kvc_kv4_layout* layout, const kvc_kv4_step* step,
                                       const kvc_kv4_split* split, int n_q);
 int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* step, const kvc_kv4_split* split,

@@ -99,12 +99,15 @@ def _prefix(counts: np.ndarray) -> np.ndarray:
     return out
 
 
-def split_chunk(lengths: np.ndarray, copies: int, slots: int, joined: int = 0) -> int:
+_START = 192  # what a CTA's start and end cost, in tokens (about 20 ns each)
+
+
+def split_chunk(lengths: np.ndarray, copies: int, slots: int, joined: int = 0) -> tuple[int, float]:
     """Tokens of an item so that ``copies`` CTAs an item fill ``slots`` resident
-    CTAs evenly: of one to four full waves (or no split at all) the choice that
-    costs least.  In tokens of a CTA (about 20 ns each): a wave costs its item and
-    192 for a CTA's start and end, joining 200 and a token for every 100 kB of
-    partial results (``joined`` bytes an item of every sequence)."""
+    CTAs evenly, and the cost: of one to four full waves (or no split at all) the
+    choice that costs least.  In tokens of a CTA: a wave costs its item and
+    ``_START``, joining 200 and a token for every 100 kB of partial results
+    (``joined`` bytes an item of every sequence)."""
     longest = int(lengths.max(initial=1))
     total = max(1, int(lengths.sum()))
     best, cost = 0, float("inf")
@@ -115,12 +118,44 @@ def split_chunk(lengths: np.ndarray, copies: int, slots: int, joined: int = 0) -
         while waves and chunk < longest and items * copies > waves * slots:
             chunk += max(128, chunk // 64 // 128 * 128)
             items = int(np.maximum(1, -(-lengths // chunk)).sum())
-        c = -(-items * copies // slots) * (min(chunk, longest) + 192)
+        c = -(-items * copies // slots) * (min(chunk, longest) + _START)
         if items > lengths.size:
             c += 200 + joined * items / lengths.size * 1e-5
         if c < cost:
             best, cost = chunk, c
-    return best
+    return best, cost
+
+
+def split_items(lengths: np.ndarray, copies: int, slots: int, joined: int, spanning: bool):
+    """The attention's items and the blocks that work on them: ``(sequence, first
+    token, end, items of each sequence, first item of each block)``.
+
+    Equal pieces of one sequence (``split_chunk``), a block each; or, where blocks
+    may span sequences and that costs less: all tokens, in runs of 128, lie in one
+    row, which ``slots // copies`` blocks (at least two runs each) cut into equal
+    shares, and an item ends where a share or a sequence does.  That wins on
+    ragged batches, where equal pieces leave SMs idle (33 sequences of up to 8191
+    tokens: 63 against 68 us), and loses where pieces happen to fit (4 x 131072:
+    62 against 59 us), since a block with two items starts and ends twice."""
+    n = lengths.size
+    chunk, cost = split_chunk(lengths, copies, slots, joined)
+    start = _prefix(np.maximum(1, -(-lengths // 128)))
+    total = int(start[-1])
+    blocks = min(slots // copies, -(-total // (_CHUNK // 128)))
+    if spanning and blocks > 0 and n * copies < 4 * slots:
+        share = -(-total // blocks)
+        shares = np.arange(0, total, share)
+        cuts = np.unique(np.concatenate((start[:-1], shares)))  # runs at which items begin
+        block = np.append(np.searchsorted(cuts, shares), cuts.size)
+        if share * 128 + _START * int(np.diff(block).max()) + 200 + joined * cuts.size / n * 1e-5 < cost:
+            seq = np.searchsorted(start, cuts, side="right") - 1
+            end = np.minimum((np.append(cuts[1:], total) - start[seq]) * 128, lengths[seq])
+            return seq, (cuts - start[seq]) * 128, end, np.searchsorted(cuts, start), block
+    items = np.maximum(1, -(-lengths // chunk))
+    first_item = _prefix(items)
+    seq = np.repeat(np.arange(n), items)
+    first = (np.arange(int(first_item[-1])) - first_item[seq]) * chunk
+    return seq, first, np.minimum(first + chunk, lengths[seq]), first_item, np.arange(int(first_item[-1]) + 1)
 
 
 class PagedKVCache:
@@ -250,15 +285,12 @@ class PagedKVCache:
         got = step.splits.get((n_q, code))
         if got is None:
             lengths = np.array(step.lengths, dtype=np.int64)
-            tiles, resident = ops.kv4_attend_split(self._layout, step.desc, n_q, code, self.device)
-            chunk = split_chunk(lengths, self.n_kv_heads * tiles, resident, 8 * step.tokens * n_q * (self.head_dim + 2))
-            items = np.maximum(1, -(-lengths // chunk))
-            start = _prefix(items)
-            seq = np.repeat(np.arange(len(step.seqs)), items)
+            tiles, resident, spanning = ops.kv4_attend_shape(self._layout, step.desc, n_q, code, self.device)
+            joined = 8 * step.tokens * n_q * (self.head_dim + 2)
+            seq, first, end, start, blocks = split_items(lengths, self.n_kv_heads * tiles, resident, joined, spanning)
             rows = np.array([self.pages.row(s) for s in step.seqs], dtype=np.int64)
-            table = np.stack((seq, (np.arange(int(start[-1])) - start[seq]) * chunk, rows[seq], lengths[seq]), 1)
-            up = _Upload((table.reshape(-1), start), self.device)
-            split = Kv4Split(*up.at, int(start[-1]), chunk, int(items.max(initial=1)))
+            up = _Upload((np.stack((seq, first, end, rows[seq]), 1).reshape(-1), start, blocks), self.device)
+            split = Kv4Split(*up.at, seq.size, blocks.size - 1, int(np.diff(start).max(initial=1)))
             got = step.splits[n_q, code] = (split, ops.kv4_attend_workspace(self._layout, step.desc, split, n_q), up)
         got[2].use(ops._raw_stream(self.device.index))
         return got[0], got[1]

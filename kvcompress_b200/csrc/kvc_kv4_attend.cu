@@ -24,9 +24,10 @@
 // multiplies is formed from the rounded weights, so their rounding acts on
 // c' - 8 and not on c'.
 //
-// A block takes `chunk` tokens of one sequence and KV head and up to 8 NT
-// columns (a column is a query and a head of the KV head's group: all of them
-// read the same codes).  Each warp works alone on runs of 32 (64 for d = 64)
+// A block takes up to 8 NT columns (a column is a query and a head of the KV
+// head's group: all of them read the same codes) and its items, runs of tokens
+// of one sequence each: every block gets an equal share of all tokens, so one
+// may end in the middle of a sequence.  Each warp works alone on runs of 32 (64 for d = 64)
 // tokens through its own ring of bulk copies: tokens are the M rows of both
 // products, so softmax statistics stay in a lane until the end; S^T's
 // accumulators become the second product's B operand by movmatrix.  The
@@ -99,23 +100,23 @@ __device__ __forceinline__ int seq_of(const Step& S, int tok) {
   return lo;
 }
 
-// Units whose logits a thread holds at once: two give twice the independent
-// products, where the registers are there.
-constexpr int units_at_once(int nt, int ng) { return nt == 1 && ng <= 2 ? 2 : 1; }
-
 // NT tiles of 8 columns; TERMS float16 terms a query and a weight.
 template <int D, int WPG, int NT, int TERMS>
 struct Shape {
   static constexpr int NG = D / 32 / WPG;
+  // Units whose logits a thread holds at once: each brings products that do not
+  // wait for the others'.  Four units and 12 warps an SM beat two and 16 (one
+  // query of each of 4 x 131072 tokens, 4 KV heads: 58.6 against 65.3 us).
+  static constexpr int at_once = NT > 1 || NG > 2 ? 1 : D == 128 && NG == 1 && TERMS == 1 ? 4 : 2;
+  static constexpr int units = at_once == 4 ? 4 : 256 / D;  // of a stage of the ring
+  static constexpr int tokens = units * kUnit;
   // Registers a thread needs, roughly (accumulators, queries, columns' and
   // groups' statistics): with up to 128 an SM has 4 blocks of 4 warps, with up
   // to 168 three, else two.
   static constexpr int regs = 45 + D / 4 * NT + (NT * TERMS == 1 ? D / 8 : 0) + 10 * NT + 8 * NG * NT +
-                              units_at_once(NT, NG) * 4 * (NT + NG) + 35 * (TERMS - 1);
+                              at_once * 4 * (NT + NG) + 35 * (TERMS - 1);
   static constexpr int warps = 4;
-  static constexpr int blocks = regs < 145 ? 4 : regs < 180 ? 3 : 2;
-  static constexpr int units = 256 / D;  // of a stage
-  static constexpr int tokens = units * kUnit;
+  static constexpr int blocks = regs < 140 ? 4 : regs < 180 ? 3 : 2;
 };
 
 template <int D, int WPG, int NT, int TERMS>
@@ -143,45 +144,56 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
   using Sm = Smem<D, WPG, NT, TERMS>;
   constexpr int W = D / 32, NG = W / WPG, UB = unit_bytes(D, NG), WARPS = Sh::warps, STAGES = Sm::stages;
   constexpr int UNITS = Sh::units, TOKENS = Sh::tokens, COLS = 8 * NT, AHEAD = 32 / UNITS;
-  constexpr int SUB = units_at_once(NT, NG);
+  constexpr int SUB = Sh::at_once;
   constexpr bool CENTRED = TERMS == 2;
   constexpr float kCode = CENTRED ? 1.0f : 16777216.0f;  // an operand is a code / kCode
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[WARPS][STAGES];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const int item = blockIdx.x, h = blockIdx.y, col0 = blockIdx.z * COLS;
-  const int4 it = P.items[item];
-  const int b = it.x, t_begin = it.y, len = it.w;
-  const int q0 = S.q_start[b], n = S.q_start[b + 1] - q0, group = a.n_q / L.n_kv;
-  const int cols = n * group;
-  const int last = min(col0 + COLS, cols) - 1;
-  const int t_end = min(t_begin + P.chunk, visible(a.causal, len, n, max(last, 0) / group));
-  // no such columns, or nothing of this item is seen: the join knows
-  if (col0 >= cols || (t_begin > 0 && t_begin >= t_end)) {
-    grid_wait();
-    grid_go();
-    return;
-  }
-  const int t_free = visible(a.causal, len, n, col0 / group);  // below it no column masks anything
-
+  const int h = blockIdx.y, col0 = blockIdx.z * COLS, group = a.n_q / L.n_kv;
   if (lane == 0)
     for (int i = 0; i < STAGES; ++i) tc::mbar_init(&full[warp][i], UNITS);
   tc::mbar_fence_init();
   __syncwarp();
+  int stage = 0, parity = 0;  // the ring's next stage to read
+  bool dead = false, waited = false;
+  auto wait_once = [&]() {  // (what is read before is the step's own arrays and the page table)
+    if (!waited) {
+      grid_wait();
+      grid_go();
+      waited = true;
+    }
+  };
+
+  for (int item = P.block_start[blockIdx.x], end = P.block_start[blockIdx.x + 1]; item < end; ++item) {
+  const int4 it = P.items[item];
+  const int b = it.x, t_begin = it.y, len = S.kv_len[b];
+  const int q0 = S.q_start[b], n = S.q_start[b + 1] - q0, cols = n * group;
+  if (col0 >= cols) continue;
+  const int last = min(col0 + COLS, cols) - 1;
+  const int t_end = min(it.z, visible(a.causal, len, n, last / group));
+  const bool alone = P.item_start[b + 1] - P.item_start[b] == 1;
+  if (t_begin > 0 && t_begin >= t_end) {  // nothing of this item is seen
+    wait_once();
+    for (int col = col0 + threadIdx.x; col <= last; col += WARPS * 32)
+      part.ml[((int64_t)item * L.n_kv + h) * part.cols + col] = make_float2(-INFINITY, 0.0f);
+    continue;
+  }
+  const int t_free = visible(a.causal, len, n, col0 / group);  // below it no column masks anything
 
   // The warp's runs of TOKENS tokens: t_begin + (warp + i WARPS) TOKENS.
   // Lane (i % AHEAD) * UNITS + u looks up unit u's page of run i and issues its
   // copy, AHEAD runs at a time, so that no copy waits for a page lookup.
   const int runs = t_end > t_begin ? (t_end - t_begin + TOKENS - 1) / TOKENS : 0;
-  const int mine = runs > warp ? (runs - warp + WARPS - 1) / WARPS : 0;
+  const int mine = runs > warp && !dead ? (runs - warp + WARPS - 1) / WARPS : 0;
   const uint32_t ring = tc::smem_u32(smem) + warp * STAGES * Sm::stage + (lane % UNITS) * UB;
   const uint8_t* src = nullptr;
   auto look = [&](int i) {  // pages of runs i .. i + AHEAD - 1
     const int t = t_begin + (warp + (i + lane / UNITS) * WARPS) * TOKENS + (lane % UNITS) * kUnit;
     src = nullptr;
     if (t < t_end) {
-      const int64_t page = page_of(L, it.z, t, &tc::g_kvc_device_error);
+      const int64_t page = page_of(L, it.w, t, &tc::g_kvc_device_error);
       // a bad entry reads page 0: its place in the sum is wrong, but in range
       src = pool + unit_off<D>(L, page < 0 ? 0 : page, h, t);
     }
@@ -199,10 +211,8 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
     }
   };
   look(0);
-  // (what was read so far is the step's own arrays and the page table)
-  grid_wait();
-  grid_go();
-  for (int i = 0; i < STAGES && i < mine; ++i) issue(i, i);
+  wait_once();
+  for (int i = 0; i < STAGES && i < mine; ++i) issue(i, (stage + i) % STAGES);
 
   // ---- queries: lane (r, c) holds features 32 w + 8 c + 0..7 of column r of each tile
   constexpr bool QS = Sm::q_shared;
@@ -503,11 +513,12 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
   };
 
   const uint32_t stages = tc::smem_u32(smem) + warp * STAGES * Sm::stage;
-  for (int i = 0, stage = 0, parity = 0; i < mine; ++i) {
+  for (int i = 0; i < mine; ++i) {
     if (__any_sync(0xffffffffu, !tc::mbar_wait(&full[warp][stage], parity, 402))) {
-      // give up: wait (bounded) for the copies still in flight, then return
-      for (int k = i + 1; k < i + STAGES && k < mine; ++k)
-        tc::mbar_wait(&full[warp][k % STAGES], (k / STAGES) & 1, 402);
+      // give up: wait (bounded) for the copies still in flight, then do nothing more
+      for (int k = 1; k < STAGES && i + k < mine; ++k)
+        tc::mbar_wait(&full[warp][(stage + k) % STAGES], parity ^ (stage + k >= STAGES), 402);
+      dead = true;
       break;
     }
     const int t0 = t_begin + (warp + i * WARPS) * TOKENS;
@@ -551,7 +562,6 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
     }
   }
   __syncthreads();
-  const bool alone = P.item_start[b + 1] - P.item_start[b] == 1;
   for (int i = threadIdx.x; i < COLS * (D / 4); i += WARPS * 32) {
     const int col = i / (D / 4), x = i % (D / 4) * 4, cj = col0 + col;
     if (cj >= cols) break;
@@ -583,6 +593,11 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
       if (x == 0) part.ml[at] = make_float2(top, sum);
     }
   }
+  // the next item's copies go where the results were
+  tc::fence_async_smem();
+  __syncthreads();
+  }
+  wait_once();
 }
 
 // Joins the items of the sequences that have several.  D / 4 threads, a float4
@@ -601,10 +616,8 @@ __global__ void __launch_bounds__(128) attend_join_kernel(Layout L, Step S, Spli
   const int tok = (int)(id / a.n_q), head = (int)(id % a.n_q);
   const int b = seq_of(S, tok), i0 = P.item_start[b], i1 = P.item_start[b + 1];
   if (i1 - i0 == 1) return grid_wait();
-  const int q0 = S.q_start[b], n = S.q_start[b + 1] - q0, j = tok - q0, group = a.n_q / L.n_kv;
-  const int vis = visible(a.causal, S.kv_len[b], n, j), h = head / group;
-  // items past what the query sees hold nothing of it; the first always holds something
-  const int items = max(1, min(i1 - i0, (vis + P.chunk - 1) / P.chunk));
+  const int j = tok - S.q_start[b], group = a.n_q / L.n_kv;
+  const int h = head / group, items = i1 - i0;
   const int64_t at0 = ((int64_t)i0 * L.n_kv + h) * part.cols + j * group + head % group, step = L.n_kv * part.cols;
   grid_wait();
   float top = -INFINITY;
@@ -673,27 +686,27 @@ int tiles_of(int cols) { return cols <= 8 ? 1 : 2; }
 
 template <int D, int WPG, int NT, int TERMS>
 int launch(const Layout& L, const Step& S, const Split& P, const void* pool, const Qkv& a, const Partial& part,
-           int64_t n_items, int col_tiles, cudaStream_t st) {
+           int64_t n_blocks, int col_tiles, cudaStream_t st) {
   using Sm = Smem<D, WPG, NT, TERMS>;
   auto kernel = attend_kernel<D, WPG, NT, TERMS>;
   static std::atomic<uint64_t> done{0};
   if (int rc = allow_shared("attend_kernel", kernel, Sm::bytes, done)) return rc;
-  const dim3 grid((unsigned)n_items, (unsigned)L.n_kv, (unsigned)col_tiles);
+  const dim3 grid((unsigned)n_blocks, (unsigned)L.n_kv, (unsigned)col_tiles);
   return launch_after("attend_kernel", kernel, grid, Shape<D, WPG, NT, TERMS>::warps * 32, Sm::bytes, st, L, S, P,
                       static_cast<const uint8_t*>(pool), a, part);
 }
 
 template <int D, int WPG>
 int launch_tiles(const Layout& L, const Step& S, const Split& P, const void* pool, const Qkv& a, const Partial& part,
-                 int64_t n_items, int cols, cudaStream_t st) {
+                 int64_t n_blocks, int cols, cudaStream_t st) {
   const int terms = a.dtype == KVC_F32 ? 2 : 1, nt = tiles_of(cols);
   const int tiles = (int)ceil_div(cols, 8 * nt);
   if (tiles > 65535 || L.n_kv > 65535) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: too many queries or KV heads");
   if (terms == 2)
-    return nt == 1 ? launch<D, WPG, 1, 2>(L, S, P, pool, a, part, n_items, tiles, st)
-                   : launch<D, WPG, 2, 2>(L, S, P, pool, a, part, n_items, tiles, st);
-  return nt == 1 ? launch<D, WPG, 1, 1>(L, S, P, pool, a, part, n_items, tiles, st)
-                 : launch<D, WPG, 2, 1>(L, S, P, pool, a, part, n_items, tiles, st);
+    return nt == 1 ? launch<D, WPG, 1, 2>(L, S, P, pool, a, part, n_blocks, tiles, st)
+                   : launch<D, WPG, 2, 2>(L, S, P, pool, a, part, n_blocks, tiles, st);
+  return nt == 1 ? launch<D, WPG, 1, 1>(L, S, P, pool, a, part, n_blocks, tiles, st)
+                 : launch<D, WPG, 2, 1>(L, S, P, pool, a, part, n_blocks, tiles, st);
 }
 
 }  // namespace
@@ -704,15 +717,16 @@ using namespace kvc;
 using namespace kvc::kv4;
 
 extern "C" int kvc_kv4_attend_shape(const kvc_kv4_layout* layout, const kvc_kv4_step* step, int n_q, int dtype,
-                                    int* tiles, int* resident) {
+                                    int* tiles, int* resident, int* spanning) {
   if (int rc = check_layout(layout, "kvc_kv4_attend_shape")) return rc;
-  if (!step || !tiles || !resident) return fail(KVC_ERR_ARG, "kvc_kv4_attend_shape: NULL pointer");
+  if (!step || !tiles || !resident || !spanning) return fail(KVC_ERR_ARG, "kvc_kv4_attend_shape: NULL pointer");
   if (n_q < 1 || n_q % layout->n_kv) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend_shape: n_q must be a multiple of n_kv");
   const int64_t cols = std::max<int64_t>(1, (int64_t)step->max_new * (n_q / layout->n_kv));
   if (cols > INT32_MAX / 2) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend_shape: too many queries");
   if (many(cols, dtype)) {
     *tiles = (int)prefill_tiles(cols);
     *resident = num_sms();
+    *spanning = 0;
     return KVC_OK;
   }
   const int terms = dtype == KVC_F32 ? 2 : 1, nt = tiles_of((int)cols);
@@ -724,6 +738,7 @@ extern "C" int kvc_kv4_attend_shape(const kvc_kv4_layout* layout, const kvc_kv4_
   KVC_KV4_DISPATCH(layout, KVC_F);
 #undef KVC_F
   *resident = blocks * num_sms();
+  *spanning = 1;
   return KVC_OK;
 }
 
@@ -744,9 +759,11 @@ extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* 
   if (!aligned16(pool)) return fail(KVC_ERR_ALIGN, "kvc_kv4_attend: pool not 16-byte aligned");
   if (n_q < 1 || n_q > 65535 || n_q % layout->n_kv) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: n_q must be a multiple of n_kv");
   if (step->n_tokens == 0 || split->n_items == 0) return KVC_OK;
+  if (!split->item_start || (!many((int64_t)step->max_new * (n_q / layout->n_kv), dtype) && !split->block_start))
+    return fail(KVC_ERR_ARG, "kvc_kv4_attend: NULL split");
   if (!split->items || !aligned16(split->items)) return fail(KVC_ERR_ALIGN, "kvc_kv4_attend: items not 16-byte aligned");
   if (step->n_tokens < 0 || step->n_tokens > INT32_MAX || step->max_new < 1 || split->n_items < 0 ||
-      split->n_items > INT32_MAX || split->chunk < 128 || split->chunk % 128)
+      split->n_items > INT32_MAX || split->n_blocks < 0 || split->n_blocks > INT32_MAX)
     return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: bad step or split sizes");
   const int64_t cols = (int64_t)step->max_new * (n_q / layout->n_kv);
   if (cols > INT32_MAX / 2) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: too many queries");
@@ -754,7 +771,7 @@ extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* 
   if (need && (!workspace || ws_bytes < need || !aligned16(workspace)))
     return fail(KVC_ERR_WORKSPACE, "kvc_kv4_attend: workspace too small or not 16-byte aligned");
   const Step s{step->n_seqs, step->rows, step->kv_len, step->q_start};
-  const Split p{reinterpret_cast<const int4*>(split->items), split->item_start, split->chunk, split->max_items};
+  const Split p{reinterpret_cast<const int4*>(split->items), split->item_start, split->block_start, split->max_items};
   const Qkv a{q, out, q_seq_stride, q_token_stride, q_head_stride, o_seq_stride, o_token_stride, o_head_stride,
               packed, dtype, n_q, causal, scale};
   Partial part{static_cast<float*>(workspace), nullptr, cols};
@@ -765,7 +782,7 @@ extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* 
   if (many(cols, dtype)) {
     rc = launch_prefill(layout, s, p, static_cast<const uint8_t*>(pool), a, part, split->n_items, st);
   } else {
-#define KVC_F(D, WPG) rc = launch_tiles<D, WPG>(L, s, p, pool, a, part, split->n_items, (int)cols, st)
+#define KVC_F(D, WPG) rc = launch_tiles<D, WPG>(L, s, p, pool, a, part, split->n_blocks, (int)cols, st)
     KVC_KV4_DISPATCH(layout, KVC_F);
 #undef KVC_F
   }

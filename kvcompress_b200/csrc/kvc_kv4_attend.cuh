@@ -19,9 +19,10 @@ struct Qkv {
 };
 
 struct Split {
-  const int4* items;  // sequence, first token, table row, cached tokens
-  const int32_t* item_start;
-  int chunk, max_items;
+  const int4* items;          // sequence, first and last + 1 token, table row
+  const int32_t *item_start;  // of each sequence
+  const int32_t *block_start; // items of each block (kernel for few columns)
+  int max_items;
 };
 
 // Partial results of an item: o (unnormalised) and (m, l) of each of its

@@ -147,16 +147,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int W = C::W, NG = C::NG;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int4 it = P.items[blockIdx.z];
-  const int b = it.x, t_begin = it.y, len = it.w, h = blockIdx.y;
+  const int b = it.x, t_begin = it.y, len = S.kv_len[it.x], h = blockIdx.y;
   const int q0 = S.q_start[b], n = S.q_start[b + 1] - q0, group = a.n_q / L.n_kv, rows = n * group;
   // late rows see the most tokens: they go first
   const int tiles = (rows + 2 * kTile - 1) / (2 * kTile), tile = tiles - 1 - (int)blockIdx.x;
   const int row0 = tile * 2 * kTile, last = min(row0 + 2 * kTile, rows) - 1;
-  const int t_end = min(t_begin + P.chunk, visible(a.causal, len, n, max(last, 0) / group));
-  // no such rows, or nothing of this item is seen: the join knows
+  const int t_end = min(it.z, visible(a.causal, len, n, max(last, 0) / group));
+  // no such rows, or nothing of this item is seen
   if (tile < 0 || (t_begin > 0 && t_begin >= t_end)) {
     grid_wait();
     grid_go();
+    for (int row = row0 + threadIdx.x; tile >= 0 && row <= last; row += kThreads)
+      part.ml[((int64_t)blockIdx.z * L.n_kv + h) * part.cols + row] = make_float2(-INFINITY, 0.0f);
     return;
   }
   const int steps = t_end > t_begin ? (t_end - t_begin + kTile - 1) / kTile : 0;
@@ -568,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto page = [&](int step) -> const uint8_t* {
         const int t = t_begin + step * kTile + lane * kUnit;
         if (lane >= C::UNITS || step >= steps || t >= t_end) return nullptr;
-        const int64_t p = page_of(L, it.z, t, &g_kvc_device_error);
+        const int64_t p = page_of(L, it.w, t, &g_kvc_device_error);
         return pool + unit_off<D>(L, p < 0 ? 0 : p, h, t);  // a bad entry reads page 0: wrong, but in range
       };
       const uint8_t* src = page(0);

@@ -769,13 +769,14 @@ def kv4_attend(layout, step, split, pool: int, query: torch.Tensor, *, causal: b
     return out
 
 
-def kv4_attend_split(layout, step, n_q: int, code: int, device: torch.device) -> tuple[int, int]:
-    """Blocks an item of one KV head is worked on by, and blocks the device runs at once."""
-    tiles, resident = ctypes.c_int(0), ctypes.c_int(0)
+def kv4_attend_shape(layout, step, n_q: int, code: int, device: torch.device) -> tuple[int, int, bool]:
+    """Blocks an item of one KV head is worked on by, blocks the device runs at
+    once, and whether a block may work on several items."""
+    out = [ctypes.c_int(0) for _ in range(3)]
     with _on(device):
-        check(lib().kvc_kv4_attend_shape(layout, step, n_q, code, ctypes.byref(tiles), ctypes.byref(resident)),
+        check(lib().kvc_kv4_attend_shape(layout, step, n_q, code, *(ctypes.byref(x) for x in out)),
               "kvc_kv4_attend_shape")
-    return tiles.value, resident.value
+    return out[0].value, out[1].value, bool(out[2].value)
 
 
 def kv4_attend_workspace(layout, step, split, n_q: int) -> int:

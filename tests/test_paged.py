@@ -12,7 +12,7 @@ import torch
 from kvcompress_b200 import PagedKVCache, ops
 from kvcompress_b200._native import KVC, Kv4Layout, Kv4Split, Kv4Step, lib
 from kvcompress_b200.cache.pages import PageTable
-from kvcompress_b200.cache.paged import split_chunk
+from kvcompress_b200.cache.paged import split_chunk, split_items
 
 
 def _check(t: PageTable, tokens: dict, content: dict) -> None:
@@ -139,8 +139,26 @@ def test_page_table_refusals():
 def test_split_chunk_covers_and_bounds():
     for lens, copies in (([1], 1), ([0, 0], 8), ([17], 4), ([32768] * 8, 8), ([131072] * 4, 4), ([5] * 999, 64),
                          ([2 ** 31 - 300], 1), (list(range(0, 8191, 253)), 8)):
-        chunk = split_chunk(np.array(lens, dtype=np.int64), copies, 296)
+        chunk, _ = split_chunk(np.array(lens, dtype=np.int64), copies, 296)
         assert chunk % 128 == 0 and 128 <= chunk < 2 ** 31
+
+
+@pytest.mark.parametrize("spanning", [True, False])
+@pytest.mark.parametrize("lens, copies", [([1], 1), ([0, 0], 8), ([17], 4), ([32768] * 8, 8), ([131072] * 4, 4), ([5] * 999, 64),
+                                          ([2 ** 31 - 300], 1), (list(range(0, 8191, 253)), 8), ([0, 700, 0, 1], 2),
+                                          ([128] * 7 + [100000], 3), ([300] * 50, 500)])
+def test_items_cover_every_sequence_once(lens, copies, spanning):
+    n = np.array(lens, dtype=np.int64)
+    seq, first, end, start, blocks = split_items(n, copies, 444, 1000, spanning)
+    assert start[0] == 0 and start[-1] == seq.size and blocks[0] == 0 and blocks[-1] == seq.size
+    assert (np.diff(blocks) >= 1).all() and blocks.size - 1 <= max(444, seq.size)
+    for i, m in enumerate(lens):
+        at = 0
+        assert start[i + 1] > start[i]
+        for j in range(start[i], start[i + 1]):
+            assert seq[j] == i and first[j] == at and first[j] % 128 == 0 and end[j] <= m
+            at = end[j]
+        assert at == m
 
 
 @pytest.mark.parametrize("kw, err", [
@@ -167,7 +185,7 @@ def _abi():
     table = (1 << 20)  # an address that no refused call reads
     layout = Kv4Layout(table, 4, 8, 2, 128, 16, 128)
     step = Kv4Step(table, table, table, table, table, 1, 1, 1, 1)
-    split = Kv4Split(table, table, 1, 256, 1)
+    split = Kv4Split(table, table, table, 1, 1, 1)
     return layout, step, split, table
 
 

@@ -15,7 +15,8 @@
 // With float32 queries the codes are centred instead (c - 8 as float16 from
 // 1024 + c, one more instruction a register): 8 s sum(q) and 8 s' are large
 // against a logit and an average over many tokens, and the accumulators' own
-// rounding would show (7e-6 of the result instead of 1e-6).
+// rounding would show (7e-6 of the result instead of 1e-6).  For the same
+// reason they hold 16 tokens or features at most, and float32 additions join them.
 //
 // What the kernel rounds: queries of 16 bits not at all (float16 with a power
 // of two per row), float32 ones to two float16 terms (22 bits); p s' to
@@ -355,10 +356,15 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
             const uint32_t a0 = codes_lo<CENTRED>(x0), a1 = codes_lo<CENTRED>(x1), a2 = codes_hi<CENTRED>(x0),
                            a3 = codes_hi<CENTRED>(x1);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
+              float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-              for (int term = 0; term < TERMS; ++term)
-                mma16816(acc[nt], a0, a1, a2, a3, qw[term][nt][i2], qw[term][nt][i2 + 1]);
+              for (int term = TERMS - 1; term >= 0; --term)
+                mma16816(CENTRED ? part : acc[nt], a0, a1, a2, a3, qw[term][nt][i2], qw[term][nt][i2 + 1]);
+              if constexpr (CENTRED)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[nt][e] += part[e];
+            }
             x0 >>= 8;
             x1 >>= 8;
           }
@@ -501,10 +507,16 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
           const uint32_t a0 = codes_lo<CENTRED>(y0), a1 = codes_hi<CENTRED>(y0), a2 = codes_lo<CENTRED>(y1),
                          a3 = codes_hi<CENTRED>(y1);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt) {
+            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int term = 0; term < TERMS; ++term)
-              mma16816(o[nt][2 * w + i2], a0, a1, a2, a3, pf[term][nt][w / WPG][0], pf[term][nt][w / WPG][1]);
+            for (int term = TERMS - 1; term >= 0; --term)
+              mma16816(CENTRED ? part : o[nt][2 * w + i2], a0, a1, a2, a3, pf[term][nt][w / WPG][0],
+                       pf[term][nt][w / WPG][1]);
+            if constexpr (CENTRED)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[nt][2 * w + i2][e] += part[e];
+          }
           y0 >>= 8;
           y1 >>= 8;
         }

@@ -830,12 +830,12 @@ def copy_pages(pools, src: Sequence[int], dst: Sequence[int]) -> None:
     if n == 0 or not ptrs:
         return
     a, b = (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst)
-    to = set(b)
+    of, to = set(src), set(dst)
     if len(to) != n:
         raise ValueError("copy_pages: a page is written twice")
-    if not to.isdisjoint(a):
+    if not to.isdisjoint(of):
         raise ValueError("copy_pages: a page is both read and written")
-    if min(min(a), min(b)) < 0 or max(max(a), max(b)) >= n_pages:
+    if min(min(of), min(to)) < 0 or max(max(of), max(to)) >= n_pages:
         raise ValueError(f"copy_pages: page out of range (pool of {n_pages})")
     page_bytes = elems // n_pages * size
     for i in range(0, len(ptrs), KVC.MAX_CELLS):

@@ -365,15 +365,17 @@ typedef struct {
  * int32.  items[4 j ..] (16-byte aligned): item j's sequence i, its first token
  * (a multiple of 128), the token after its last, and rows[i].  The items of
  * sequence i are item_start[i] .. item_start[i + 1] - 1; they follow one another
- * and cover its kv_len[i] tokens, and there is at least one.  max_items: most
- * items of one sequence.  block_start (n_blocks + 1): the items that block k
+ * and cover its kv_len[i] tokens.  A sequence with queries and no items is left
+ * to another call on the same step with another split, so that the many queries
+ * of one sequence and the few of others can run as each runs best.  max_items and
+ * max_new: most items and most queries of one of the split's sequences.  block_start (n_blocks + 1): the items that block k
  * works on are block_start[k] .. block_start[k + 1] - 1; used where
  * kvc_kv4_attend_shape says `spanning`, else every item is a block.
  */
 typedef struct {
   const int32_t *items, *item_start, *block_start;
   int64_t n_items, n_blocks;
-  int32_t max_items;
+  int32_t max_items, max_new;
 } kvc_kv4_split;
 
 int64_t kvc_kv4_page_bytes(int n_kv, int head_dim, int page_size, int group_size);
@@ -399,10 +401,9 @@ int kvc_kv4_read(const kvc_kv4_layout* layout, const void* pool, int64_t layer_b
 /* For choosing the split: the blocks that work on one item of one KV head, each
  * with other columns (tiles), the blocks that the current device runs at once
  * (resident), and whether a block may work on several items (spanning). */
-int kvc_kv4_attend_shape(const kvc_kv4_layout* layout, const kvc_kv4_step* step, int n_q, int dtype, int* tiles,
-                         int* resident, int* spanning);
-size_t kvc_kv4_attend_workspace_bytes(const kvc_kv4_layout* layout, const kvc_kv4_step* step,
-                                      const kvc_kv4_split* split, int n_q);
+int kvc_kv4_attend_shape(const kvc_kv4_layout* layout, int max_new, int n_q, int dtype, int* tiles, int* resident,
+                         int* spanning);
+size_t kvc_kv4_attend_workspace_bytes(const kvc_kv4_layout* layout, const kvc_kv4_split* split, int n_q);
 int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* step, const kvc_kv4_split* split,
                    const void* pool, int n_q, const void* q, int64_t q_seq_stride, int64_t q_token_stride,
                    int64_t q_head_stride, void* out, int64_t o_seq_stride, int64_t o_token_stride,

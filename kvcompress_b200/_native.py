@@ -59,7 +59,7 @@ class Kv4Split(ctypes.Structure):
     """``kvc_kv4_split``."""
 
     _fields_ = [("items", P), ("item_start", P), ("block_start", P), ("n_items", I64), ("n_blocks", I64),
-                ("max_items", ctypes.c_int32)]
+                ("max_items", ctypes.c_int32), ("max_new", ctypes.c_int32)]
 
 
 _LAYOUT, _STEP, _SPLIT = (ctypes.POINTER(t) for t in (Kv4Layout, Kv4Step, Kv4Split))
@@ -101,8 +101,8 @@ _SIGNATURES = {
     "kvc_kv4_page_bytes": (I64, [I, I, I, I]),
     "kvc_kv4_write": (I, [_LAYOUT, _STEP, P, P, P, I, I64, I64, I64, I, P]),
     "kvc_kv4_read": (I, [_LAYOUT, P, I64, I, I, I64, I64, I, P, P, P]),
-    "kvc_kv4_attend_shape": (I, [_LAYOUT, _STEP, I, I, *[ctypes.POINTER(I)] * 3]),
-    "kvc_kv4_attend_workspace_bytes": (SZ, [_LAYOUT, _STEP, _SPLIT, I]),
+    "kvc_kv4_attend_shape": (I, [_LAYOUT, I, I, I, *[ctypes.POINTER(I)] * 3]),
+    "kvc_kv4_attend_workspace_bytes": (SZ, [_LAYOUT, _SPLIT, I]),
     "kvc_kv4_attend": (I, [_LAYOUT, _STEP, _SPLIT, P, I, P, I64, I64, I64, P, I64, I64, I64, I, I, I,
                            ctypes.c_float, P, SZ, P]),
     "kvc_copy_pages": (I, [I, PP, I64, I64, I64, P, P, P]),

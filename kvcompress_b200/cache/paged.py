@@ -40,6 +40,9 @@ class _Upload:
     __slots__ = ("buf", "at", "streams", "event")
 
     def __init__(self, arrays: Sequence[np.ndarray], device: torch.device) -> None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("PagedKVCache: a step is planned on its first use, which cannot be captured into a CUDA "
+                               "graph; use the step once before")
         host = torch.empty(max(1, sum(a.size for a in arrays)), dtype=torch.int32, pin_memory=True)
         view, n, offsets = host.numpy(), 0, []
         for a in arrays:
@@ -86,7 +89,7 @@ class CacheStep:
     cache: Any = field(repr=False)
     meta: _Upload = field(repr=False)  # the arrays that ``desc`` points into
     desc: Kv4Step = field(repr=False)
-    splits: dict[tuple[int, int], tuple[Kv4Split, int, _Upload]] = field(default_factory=dict, repr=False)
+    splits: dict[tuple[int, int], list] = field(default_factory=dict, repr=False)
 
     @property
     def tokens(self) -> int:
@@ -281,19 +284,40 @@ class PagedKVCache:
                        int(q_start[-1]))
         return CacheStep(seqs, counts, lengths.tolist(), writable, self.pages.epoch, self, meta, desc)
 
-    def _split(self, step: CacheStep, n_q: int, code: int) -> tuple[Kv4Split, int]:
+    def _split(self, step: CacheStep, n_q: int, code: int) -> list[tuple[Kv4Split, int]]:
         got = step.splits.get((n_q, code))
         if got is None:
-            lengths = np.array(step.lengths, dtype=np.int64)
-            tiles, resident, spanning = ops.kv4_attend_shape(self._layout, step.desc, n_q, code, self.device)
-            joined = 8 * step.tokens * n_q * (self.head_dim + 2)
-            seq, first, end, start, blocks = split_items(lengths, self.n_kv_heads * tiles, resident, joined, spanning)
-            rows = np.array([self.pages.row(s) for s in step.seqs], dtype=np.int64)
-            up = _Upload((np.stack((seq, first, end, rows[seq]), 1).reshape(-1), start, blocks), self.device)
-            split = Kv4Split(*up.at, seq.size, blocks.size - 1, int(np.diff(start).max(initial=1)))
-            got = step.splits[n_q, code] = (split, ops.kv4_attend_workspace(self._layout, step.desc, split, n_q), up)
-        got[2].use(ops._raw_stream(self.device.index))
-        return got[0], got[1]
+            got = step.splits[n_q, code] = self._plan(step, n_q, code)
+        stream = ops._raw_stream(self.device.index)
+        for _, up in got:
+            up.use(stream)
+        return [split for split, _ in got]
+
+    def _plan(self, step: CacheStep, n_q: int, code: int) -> list[tuple[tuple[Kv4Split, int], _Upload]]:
+        """The step's launches: one, or two where some sequences have many queries
+        and others few, which different kernels are for."""
+        lengths = np.array(step.lengths, dtype=np.int64)
+        counts = np.array(step.counts, dtype=np.int64)
+        rows = np.array([self.pages.row(s) for s in step.seqs], dtype=np.int64)
+        shape = lambda n: ops.kv4_attend_shape(self._layout, int(n), n_q, code, self.device)  # noqa: E731
+        spans = {int(n): shape(n)[2] for n in np.unique(counts) if n}
+        plans = []
+        for spanning in (False, True):
+            mine = np.array([n > 0 and spans[int(n)] == spanning for n in counts], dtype=bool)
+            if not mine.any():
+                continue
+            at = np.nonzero(mine)[0]
+            most = int(counts[at].max())
+            tiles, resident, _ = shape(most)
+            joined = 8 * int(counts[at].sum()) * n_q * (self.head_dim + 2)
+            seq, first, end, start, blocks = split_items(lengths[at], self.n_kv_heads * tiles, resident, joined, spanning)
+            items = np.zeros_like(lengths)
+            items[at] = np.diff(start)
+            table = np.stack((at[seq], first, end, rows[at][seq]), 1)
+            up = _Upload((table.reshape(-1), _prefix(items), blocks), self.device)
+            split = Kv4Split(*up.at, seq.size, blocks.size - 1, int(items.max()), most)
+            plans.append(((split, ops.kv4_attend_workspace(self._layout, split, n_q)), up))
+        return plans
 
     def _check(self, what: str, layer: int, step: CacheStep) -> int:
         if step.cache is not self:
@@ -360,6 +384,8 @@ class PagedKVCache:
         dirty = self.pages.dirty
         if not dirty:
             return
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("PagedKVCache: the page table has changed and cannot be updated inside a CUDA graph")
         width = self.pages.max_pages
         at = np.unique(np.concatenate([np.arange(r * width + a, r * width + b) for r, a, b in dirty]))
         host = torch.empty(2, at.size, dtype=torch.int64, pin_memory=True)

@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(128) attend_join_kernel(Layout L, Step S, Spli
   if (id >= rows) return grid_wait();
   const int tok = (int)(id / a.n_q), head = (int)(id % a.n_q);
   const int b = seq_of(S, tok), i0 = P.item_start[b], i1 = P.item_start[b + 1];
-  if (i1 - i0 == 1) return grid_wait();
+  if (i1 - i0 <= 1) return grid_wait();
   const int j = tok - S.q_start[b], group = a.n_q / L.n_kv;
   const int h = head / group, items = i1 - i0;
   const int64_t at0 = ((int64_t)i0 * L.n_kv + h) * part.cols + j * group + head % group, step = L.n_kv * part.cols;
@@ -728,12 +728,12 @@ int launch_tiles(const Layout& L, const Step& S, const Split& P, const void* poo
 using namespace kvc;
 using namespace kvc::kv4;
 
-extern "C" int kvc_kv4_attend_shape(const kvc_kv4_layout* layout, const kvc_kv4_step* step, int n_q, int dtype,
-                                    int* tiles, int* resident, int* spanning) {
+extern "C" int kvc_kv4_attend_shape(const kvc_kv4_layout* layout, int max_new, int n_q, int dtype, int* tiles,
+                                    int* resident, int* spanning) {
   if (int rc = check_layout(layout, "kvc_kv4_attend_shape")) return rc;
-  if (!step || !tiles || !resident || !spanning) return fail(KVC_ERR_ARG, "kvc_kv4_attend_shape: NULL pointer");
+  if (!tiles || !resident || !spanning) return fail(KVC_ERR_ARG, "kvc_kv4_attend_shape: NULL pointer");
   if (n_q < 1 || n_q % layout->n_kv) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend_shape: n_q must be a multiple of n_kv");
-  const int64_t cols = std::max<int64_t>(1, (int64_t)step->max_new * (n_q / layout->n_kv));
+  const int64_t cols = std::max<int64_t>(1, (int64_t)max_new * (n_q / layout->n_kv));
   if (cols > INT32_MAX / 2) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend_shape: too many queries");
   if (many(cols, dtype)) {
     *tiles = (int)prefill_tiles(cols);
@@ -754,10 +754,9 @@ extern "C" int kvc_kv4_attend_shape(const kvc_kv4_layout* layout, const kvc_kv4_
   return KVC_OK;
 }
 
-extern "C" size_t kvc_kv4_attend_workspace_bytes(const kvc_kv4_layout* layout, const kvc_kv4_step* step,
-                                                 const kvc_kv4_split* split, int n_q) {
-  if (!layout || !step || !split || split->max_items <= 1) return 0;
-  return (size_t)split->n_items * n_q * step->max_new * (layout->head_dim + 2) * sizeof(float);
+extern "C" size_t kvc_kv4_attend_workspace_bytes(const kvc_kv4_layout* layout, const kvc_kv4_split* split, int n_q) {
+  if (!layout || !split || split->max_items <= 1 || split->n_items < 0 || split->max_new < 0 || n_q < 0) return 0;
+  return (size_t)split->n_items * n_q * split->max_new * (layout->head_dim + 2) * sizeof(float);
 }
 
 extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* step, const kvc_kv4_split* split,
@@ -771,15 +770,15 @@ extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* 
   if (!aligned16(pool)) return fail(KVC_ERR_ALIGN, "kvc_kv4_attend: pool not 16-byte aligned");
   if (n_q < 1 || n_q > 65535 || n_q % layout->n_kv) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: n_q must be a multiple of n_kv");
   if (step->n_tokens == 0 || split->n_items == 0) return KVC_OK;
-  if (!split->item_start || (!many((int64_t)step->max_new * (n_q / layout->n_kv), dtype) && !split->block_start))
+  if (!split->item_start || (!many((int64_t)split->max_new * (n_q / layout->n_kv), dtype) && !split->block_start))
     return fail(KVC_ERR_ARG, "kvc_kv4_attend: NULL split");
   if (!split->items || !aligned16(split->items)) return fail(KVC_ERR_ALIGN, "kvc_kv4_attend: items not 16-byte aligned");
-  if (step->n_tokens < 0 || step->n_tokens > INT32_MAX || step->max_new < 1 || split->n_items < 0 ||
+  if (step->n_tokens < 0 || step->n_tokens > INT32_MAX || split->max_new < 1 || split->n_items < 0 ||
       split->n_items > INT32_MAX || split->n_blocks < 0 || split->n_blocks > INT32_MAX)
     return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: bad step or split sizes");
-  const int64_t cols = (int64_t)step->max_new * (n_q / layout->n_kv);
+  const int64_t cols = (int64_t)split->max_new * (n_q / layout->n_kv);
   if (cols > INT32_MAX / 2) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: too many queries");
-  const size_t need = kvc_kv4_attend_workspace_bytes(layout, step, split, n_q);
+  const size_t need = kvc_kv4_attend_workspace_bytes(layout, split, n_q);
   if (need && (!workspace || ws_bytes < need || !aligned16(workspace)))
     return fail(KVC_ERR_WORKSPACE, "kvc_kv4_attend: workspace too small or not 16-byte aligned");
   const Step s{step->n_seqs, step->rows, step->kv_len, step->q_start};
@@ -787,7 +786,7 @@ extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* 
   const Qkv a{q, out, q_seq_stride, q_token_stride, q_head_stride, o_seq_stride, o_token_stride, o_head_stride,
               packed, dtype, n_q, causal, scale};
   Partial part{static_cast<float*>(workspace), nullptr, cols};
-  if (need) part.ml = reinterpret_cast<float2*>(part.o + (size_t)split->n_items * n_q * step->max_new * layout->head_dim);
+  if (need) part.ml = reinterpret_cast<float2*>(part.o + (size_t)split->n_items * n_q * split->max_new * layout->head_dim);
   const Layout L = to_layout(layout);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc = KVC_OK;

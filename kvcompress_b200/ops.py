@@ -748,8 +748,9 @@ def kv4_write(layout, step, pool: int, key: torch.Tensor, value: torch.Tensor, d
 def kv4_attend(layout, step, split, pool: int, query: torch.Tensor, *, causal: bool, scale: float,
                device: torch.device) -> torch.Tensor:
     """Attention of a step's queries over the pages of the layer at address
-    ``pool`` (``kvc_kv4_attend``).  ``split(n_q, code)`` gives the split of the
-    cached tokens for ``n_q`` query heads of dtype ``code``, and the workspace's bytes."""
+    ``pool`` (``kvc_kv4_attend``).  ``split(n_q, code)`` gives the splits of the
+    cached tokens for ``n_q`` query heads of dtype ``code`` (a launch each) and
+    their workspaces' bytes."""
     code = _kv4_code(query.dtype)
     sb, st, sh, packed = _kv4_tokens(query, step, "kv4_attend", None, layout, device)
     n_q = query.shape[1]
@@ -759,29 +760,29 @@ def kv4_attend(layout, step, split, pool: int, query: torch.Tensor, *, causal: b
     if step.n_tokens == 0:
         return out
     o = out.stride()
-    sp, ws_n = split(n_q, code)
-    # a buffer of this call's own: a captured graph keeps the one it was captured
-    # with, and no other graph or stream writes to it
-    ws = torch.empty(ws_n, dtype=torch.uint8, device=device) if ws_n else None
-    _call("kv4_attend", device, 2 * query.numel() * query.element_size(), lib().kvc_kv4_attend, layout, step, sp, pool,
-          n_q, query.data_ptr(), sb, st, sh, out.data_ptr(), 0 if packed else o[0], o[0] if packed else o[2], o[1],
-          packed, code, causal, scale, ws.data_ptr() if ws_n else None, ws_n)
+    for sp, ws_n in split(n_q, code):
+        # a buffer of this call's own: a captured graph keeps the one it was captured
+        # with, and no other graph or stream writes to it
+        ws = torch.empty(ws_n, dtype=torch.uint8, device=device) if ws_n else None
+        _call("kv4_attend", device, 2 * query.numel() * query.element_size(), lib().kvc_kv4_attend, layout, step, sp,
+              pool, n_q, query.data_ptr(), sb, st, sh, out.data_ptr(), 0 if packed else o[0], o[0] if packed else o[2],
+              o[1], packed, code, causal, scale, ws.data_ptr() if ws_n else None, ws_n)
     return out
 
 
-def kv4_attend_shape(layout, step, n_q: int, code: int, device: torch.device) -> tuple[int, int, bool]:
+def kv4_attend_shape(layout, max_new: int, n_q: int, code: int, device: torch.device) -> tuple[int, int, bool]:
     """Blocks an item of one KV head is worked on by, blocks the device runs at
     once, and whether a block may work on several items."""
     out = [ctypes.c_int(0) for _ in range(3)]
     with _on(device):
-        check(lib().kvc_kv4_attend_shape(layout, step, n_q, code, *(ctypes.byref(x) for x in out)),
+        check(lib().kvc_kv4_attend_shape(layout, max_new, n_q, code, *(ctypes.byref(x) for x in out)),
               "kvc_kv4_attend_shape")
     return out[0].value, out[1].value, bool(out[2].value)
 
 
-def kv4_attend_workspace(layout, step, split, n_q: int) -> int:
+def kv4_attend_workspace(layout, split, n_q: int) -> int:
     """Bytes of ``kvc_kv4_attend``'s workspace."""
-    return int(lib().kvc_kv4_attend_workspace_bytes(layout, step, split, n_q))
+    return int(lib().kvc_kv4_attend_workspace_bytes(layout, split, n_q))
 
 
 def kv4_read(layout, pool: int, layer_bytes: int, n_layers: int, row: int, t0: int, t1: int, dtype: torch.dtype,

@@ -561,6 +561,39 @@ def test_captured_steps_replay():
             check_attend(c, q, step, kv, layer=layer)
 
 
+def test_a_new_step_is_not_planned_inside_a_graph():
+    c = make(2, 128)
+    s = c.add()
+    k, v = cells(40, 2, 128, BF16)
+    q = queries(1, 4, 128, BF16)
+    c.write(0, k, v, c.extend([s], [40]))
+    step = c.view([s], [1])
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(RuntimeError, match="use the step once before"):
+            c.attend(0, q, step)
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            c.view([s], [1])
+        q.add_(0)
+    check_attend(c, q, step, [(k, v)])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("counts", [[1, 300, 1, 0, 40, 1, 2], [2000, 1, 1, 1, 1, 1, 1]])
+def test_prompts_and_single_tokens_in_one_step(dtype, counts):
+    lens = [9000, 310, 1, 50, 700, 5000, 20]
+    lens[0] = max(lens[0], counts[0])
+    c = make(2, 128, 128, 64, 16384, 7, pages=400)
+    seqs = [c.add() for _ in lens]
+    k, v = cells(sum(lens), 2, 128, dtype)
+    c.write(0, k, v, c.extend(seqs, lens))
+    kv = list(zip(k.split(lens), v.split(lens)))
+    q = queries(sum(counts), 8, 128, dtype, size=0.1)
+    for causal in (True, False):
+        check_attend(c, q, c.view(seqs, counts), kv, causal)
+
+
 def test_another_stream():
     c = make(2, 128, 128, 16, 4096, 2)
     s = c.add()

@@ -185,7 +185,7 @@ def _abi():
     table = (1 << 20)  # an address that no refused call reads
     layout = Kv4Layout(table, 4, 8, 2, 128, 16, 128)
     step = Kv4Step(table, table, table, table, table, 1, 1, 1, 1)
-    split = Kv4Split(table, table, table, 1, 1, 1)
+    split = Kv4Split(table, table, table, 1, 1, 1, 1)
     return layout, step, split, table
 
 

@@ -89,7 +89,7 @@ class CacheStep:
     cache: Any = field(repr=False)
     meta: _Upload = field(repr=False)  # the arrays that ``desc`` points into
     desc: Kv4Step = field(repr=False)
-    splits: dict[tuple[int, int], list] = field(default_factory=dict, repr=False)
+    splits: dict[tuple[int, int], tuple[list, list]] = field(default_factory=dict, repr=False)
 
     @property
     def tokens(self) -> int:
@@ -209,6 +209,7 @@ class PagedKVCache:
         # zeros: a page's bytes are defined before its first tokens are written
         self.pool = torch.zeros(self.n_layers, self.pages.n_pages, self.page_bytes, dtype=torch.uint8, device=device)
         self.table = torch.zeros(self.pages.table.shape, dtype=torch.int32, device=device)
+        self._byte = torch.zeros(1, dtype=torch.uint8, device=device)  # workspaces are empty_like its expansions
         self._layers = [self.pool.data_ptr() + i * self.pool.stride(0) for i in range(self.n_layers)]
         self._layout = Kv4Layout(self.table.data_ptr(), self.table.stride(0), self.pages.n_pages, self.n_kv_heads,
                                  self.head_dim, self.page_size, self.group_size)
@@ -284,16 +285,17 @@ class PagedKVCache:
                        int(q_start[-1]))
         return CacheStep(seqs, counts, lengths.tolist(), writable, self.pages.epoch, self, meta, desc)
 
-    def _split(self, step: CacheStep, n_q: int, code: int) -> list[tuple[Kv4Split, int]]:
+    def _split(self, step: CacheStep, n_q: int, code: int) -> list[tuple[Kv4Split, int, torch.Tensor | None]]:
         got = step.splits.get((n_q, code))
         if got is None:
-            got = step.splits[n_q, code] = self._plan(step, n_q, code)
+            plans = self._plan(step, n_q, code)
+            got = step.splits[n_q, code] = [p[:3] for p in plans], [p[3] for p in plans]
         stream = ops._raw_stream(self.device.index)
-        for _, up in got:
+        for up in got[1]:
             up.use(stream)
-        return [split for split, _ in got]
+        return got[0]
 
-    def _plan(self, step: CacheStep, n_q: int, code: int) -> list[tuple[tuple[Kv4Split, int], _Upload]]:
+    def _plan(self, step: CacheStep, n_q: int, code: int) -> list[tuple]:
         """The step's launches: one, or two where some sequences have many queries
         and others few, which different kernels are for."""
         lengths = np.array(step.lengths, dtype=np.int64)
@@ -316,7 +318,8 @@ class PagedKVCache:
             table = np.stack((at[seq], first, end, rows[at][seq]), 1)
             up = _Upload((table.reshape(-1), _prefix(items), blocks), self.device)
             split = Kv4Split(*up.at, seq.size, blocks.size - 1, int(items.max()), most)
-            plans.append(((split, ops.kv4_attend_workspace(self._layout, split, n_q)), up))
+            nbytes = ops.kv4_attend_workspace(self._layout, split, n_q)
+            plans.append((split, nbytes, self._byte.expand(nbytes) if nbytes else None, up))
         return plans
 
     def _check(self, what: str, layer: int, step: CacheStep) -> int:

@@ -749,24 +749,25 @@ def kv4_attend(layout, step, split, pool: int, query: torch.Tensor, *, causal: b
                device: torch.device) -> torch.Tensor:
     """Attention of a step's queries over the pages of the layer at address
     ``pool`` (``kvc_kv4_attend``).  ``split(n_q, code)`` gives the splits of the
-    cached tokens for ``n_q`` query heads of dtype ``code`` (a launch each) and
-    their workspaces' bytes."""
+    cached tokens for ``n_q`` query heads of dtype ``code`` (a launch each), with
+    a tensor of the workspace's type and size for each that needs one."""
     code = _kv4_code(query.dtype)
     sb, st, sh, packed = _kv4_tokens(query, step, "kv4_attend", None, layout, device)
     n_q = query.shape[1]
     if n_q % layout.n_kv or n_q == 0:
         raise ValueError(f"kv4_attend: {n_q} query heads are no multiple of {layout.n_kv} KV heads")
-    out = torch.empty(query.shape, dtype=query.dtype, device=device)
+    out = torch.empty_like(query)  # (features stay contiguous)
     if step.n_tokens == 0:
         return out
-    o = out.stride()
-    for sp, ws_n in split(n_q, code):
+    o, nbytes = out.stride(), 2 * query.numel() * query.element_size()
+    o = (0, o[0], o[1]) if packed else (o[0], o[2], o[1])
+    q, to, fn = query.data_ptr(), out.data_ptr(), lib().kvc_kv4_attend
+    for sp, ws_n, like in split(n_q, code):
         # a buffer of this call's own: a captured graph keeps the one it was captured
         # with, and no other graph or stream writes to it
-        ws = torch.empty(ws_n, dtype=torch.uint8, device=device) if ws_n else None
-        _call("kv4_attend", device, 2 * query.numel() * query.element_size(), lib().kvc_kv4_attend, layout, step, sp,
-              pool, n_q, query.data_ptr(), sb, st, sh, out.data_ptr(), 0 if packed else o[0], o[0] if packed else o[2],
-              o[1], packed, code, causal, scale, ws.data_ptr() if ws_n else None, ws_n)
+        ws = None if like is None else torch.empty_like(like)
+        _call("kv4_attend", device, nbytes, fn, layout, step, sp, pool, n_q, q, sb, st, sh, to, *o, packed, code, causal,
+              scale, None if ws is None else ws.data_ptr(), ws_n)
     return out
 
 

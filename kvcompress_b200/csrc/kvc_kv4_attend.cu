@@ -32,7 +32,7 @@
 // tokens through its own ring of bulk copies: tokens are the M rows of both
 // products, so softmax statistics stay in a lane until the end; S^T's
 // accumulators become the second product's B operand by movmatrix.  The
-// running maximum is raised only when a logit exceeds it by 2^4, which is
+// running maximum is raised only when a logit exceeds it by 2^8, which is
 // rare, so the loop holds one vote and no reductions.  The warps' partial
 // results are joined through shared memory, the blocks' of a sequence by
 // attend_join_kernel in a fixed order.
@@ -57,7 +57,7 @@ int kv4_attend_read_device_error(int* out) {
 namespace kv4 {
 namespace {
 
-constexpr float kTop = 2048.0f;  // weights p s' are held as (p s' / cap) * kTop <= 2^4 * 2^11 < 65504
+constexpr float kTop = 128.0f;  // weights p s' are held as (p s' / cap) * kTop <= 2^8 * 2^7 < 65504
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {

@@ -20,9 +20,9 @@
 // put into the same order.
 //
 // The running maximum is a reference that is only raised when a row's logits
-// exceed it by 2^4; only then O (in TMEM) is rescaled, by the softmax threads.
-// Weights are held 2^7 fold in float16, which leaves 2^-21 of a row's largest
-// for normal numbers.  A masked token's weight is 0, but its value may be NaN:
+// exceed it by 2^8; only then O (in TMEM) is rescaled, by the softmax threads.
+// Weights are held 2^7 fold in float16, so that those down to 2^-21 of the
+// reference are normal numbers.  A masked token's weight is 0, but its value may be NaN:
 // such values are written as 0 and their tokens flagged, and a row that does see
 // a flagged token gets NaN in that group at the end.
 #include "kvc_kv4_attend.cuh"

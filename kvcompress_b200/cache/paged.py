@@ -79,7 +79,7 @@ class CacheStep:
 
     ``counts[i]`` tokens belong to ``seqs[i]``, the last ones of its
     ``lengths[i]`` cached tokens.  A step is good until a fork, free, truncate
-    or compact changes the cache."""
+    or compact changes the cache.  Its arrays go to the device on its first use."""
 
     seqs: list[int]
     counts: list[int]
@@ -87,13 +87,13 @@ class CacheStep:
     writable: bool
     epoch: int
     cache: Any = field(repr=False)
-    meta: _Upload = field(repr=False)  # the arrays that ``desc`` points into
-    desc: Kv4Step = field(repr=False)
+    meta: _Upload | None = field(default=None, repr=False)  # the arrays that ``desc`` points into
+    desc: Kv4Step | None = field(default=None, repr=False)
     splits: dict[tuple[int, int], tuple[list, list]] = field(default_factory=dict, repr=False)
 
     @property
     def tokens(self) -> int:
-        return int(self.desc.n_tokens)
+        return sum(self.counts)
 
 
 def _prefix(counts: np.ndarray) -> np.ndarray:
@@ -119,7 +119,7 @@ def split_chunk(lengths: np.ndarray, copies: int, slots: int, joined: int = 0) -
         chunk = -(-chunk // 128) * 128
         items = int(np.maximum(1, -(-lengths // chunk)).sum())
         while waves and chunk < longest and items * copies > waves * slots:
-            chunk += max(128, chunk // 64 // 128 * 128)
+            chunk += max(128, chunk // 32 // 128 * 128)
             items = int(np.maximum(1, -(-lengths // chunk)).sum())
         c = -(-items * copies // slots) * (min(chunk, longest) + _START)
         if items > lengths.size:
@@ -177,8 +177,9 @@ class PagedKVCache:
             out = cache.attend(layer, q, step)
 
     Launches go to the current stream; use a cache from one stream at a time.
-    ``write`` and ``attend`` may be captured into a CUDA graph (not ``extend``,
-    ``view``, ``fork``, ``compact``), which then repeats that step.  There is no
+    ``write`` and ``attend`` may be captured into a CUDA graph once the step has been
+    used outside one (not ``extend``, ``view``, ``fork``, ``compact``); the graph then
+    repeats that step.  There is no
     gradient through a cache in 4 bits.
     """
 
@@ -209,6 +210,7 @@ class PagedKVCache:
         # zeros: a page's bytes are defined before its first tokens are written
         self.pool = torch.zeros(self.n_layers, self.pages.n_pages, self.page_bytes, dtype=torch.uint8, device=device)
         self.table = torch.zeros(self.pages.table.shape, dtype=torch.int32, device=device)
+        self._shapes: dict[tuple[int, int, int], tuple[int, int, bool]] = {}
         self._byte = torch.zeros(1, dtype=torch.uint8, device=device)  # workspaces are empty_like its expansions
         self._layers = [self.pool.data_ptr() + i * self.pool.stride(0) for i in range(self.n_layers)]
         self._layout = Kv4Layout(self.table.data_ptr(), self.table.stride(0), self.pages.n_pages, self.n_kv_heads,
@@ -269,21 +271,22 @@ class PagedKVCache:
         return self._step(seqs, counts, False)
 
     def _step(self, seqs: list[int], counts: list[int], writable: bool) -> CacheStep:
-        self._sync()
-        n = np.array(counts, dtype=np.int64)
-        lengths = np.array([self.pages.length(s) for s in seqs], dtype=np.int64)
-        rows = np.array([self.pages.row(s) for s in seqs], dtype=np.int64)
-        if int(n.sum()) > 2 ** 31 - 1:
+        if sum(counts) > 2 ** 31 - 1:
             raise ValueError("PagedKVCache: too many tokens in one step")
+        return CacheStep(seqs, counts, [self.pages.length(s) for s in seqs], writable, self.pages.epoch, self)
+
+    def _prepare(self, step: CacheStep) -> None:
+        """Put the step's arrays on the device."""
+        self._sync()
+        n, lengths = np.array(step.counts, dtype=np.int64), np.array(step.lengths, dtype=np.int64)
+        rows = np.array([self.pages.row(s) for s in step.seqs], dtype=np.int64)
         halves = np.zeros_like(n)
-        if writable:  # aligned runs of 8 tokens that the new ones touch
+        if step.writable:  # aligned runs of 8 tokens that the new ones touch
             halves = np.where(n > 0, (lengths - 1) // 8 - (lengths - n) // 8 + 1, 0)
         q_start, half_start = _prefix(n), _prefix(halves)
-        half_seq = np.repeat(np.arange(len(seqs)), halves)
-        meta = _Upload((rows, lengths, q_start, half_seq, half_start), self.device)
-        desc = Kv4Step(*meta.at, int(half_start[-1]), len(seqs), int(n.max(initial=0)),
-                       int(q_start[-1]))
-        return CacheStep(seqs, counts, lengths.tolist(), writable, self.pages.epoch, self, meta, desc)
+        half_seq = np.repeat(np.arange(n.size), halves)
+        step.meta = _Upload((rows, lengths, q_start, half_seq, half_start), self.device)
+        step.desc = Kv4Step(*step.meta.at, int(half_start[-1]), n.size, int(n.max(initial=0)), int(q_start[-1]))
 
     def _split(self, step: CacheStep, n_q: int, code: int) -> list[tuple[Kv4Split, int, torch.Tensor | None]]:
         got = step.splits.get((n_q, code))
@@ -301,16 +304,14 @@ class PagedKVCache:
         lengths = np.array(step.lengths, dtype=np.int64)
         counts = np.array(step.counts, dtype=np.int64)
         rows = np.array([self.pages.row(s) for s in step.seqs], dtype=np.int64)
-        shape = lambda n: ops.kv4_attend_shape(self._layout, int(n), n_q, code, self.device)  # noqa: E731
-        spans = {int(n): shape(n)[2] for n in np.unique(counts) if n}
+        spans = {n: self._shape(n, n_q, code)[2] for n in set(step.counts) if n}
         plans = []
         for spanning in (False, True):
-            mine = np.array([n > 0 and spans[int(n)] == spanning for n in counts], dtype=bool)
-            if not mine.any():
+            if spanning not in spans.values():
                 continue
-            at = np.nonzero(mine)[0]
+            at = np.array([i for i, n in enumerate(step.counts) if n and spans[n] == spanning], dtype=np.int64)
             most = int(counts[at].max())
-            tiles, resident, _ = shape(most)
+            tiles, resident, _ = self._shape(most, n_q, code)
             joined = 8 * int(counts[at].sum()) * n_q * (self.head_dim + 2)
             seq, first, end, start, blocks = split_items(lengths[at], self.n_kv_heads * tiles, resident, joined, spanning)
             items = np.zeros_like(lengths)
@@ -322,6 +323,12 @@ class PagedKVCache:
             plans.append((split, nbytes, self._byte.expand(nbytes) if nbytes else None, up))
         return plans
 
+    def _shape(self, max_new: int, n_q: int, code: int) -> tuple[int, int, bool]:
+        got = self._shapes.get((max_new, n_q, code))
+        if got is None:
+            got = self._shapes[max_new, n_q, code] = ops.kv4_attend_shape(self._layout, max_new, n_q, code, self.device)
+        return got
+
     def _check(self, what: str, layer: int, step: CacheStep) -> int:
         if step.cache is not self:
             raise ValueError(f"PagedKVCache.{what}: the step belongs to another cache")
@@ -330,6 +337,8 @@ class PagedKVCache:
                                "step was made; make it again")
         if not 0 <= layer < self.n_layers:
             raise IndexError(f"PagedKVCache.{what}: layer {layer} of {self.n_layers}")
+        if step.meta is None:
+            self._prepare(step)
         step.meta.use(ops._raw_stream(self.device.index))
         return self._layers[layer]
 
@@ -390,7 +399,9 @@ class PagedKVCache:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("PagedKVCache: the page table has changed and cannot be updated inside a CUDA graph")
         width = self.pages.max_pages
-        at = np.unique(np.concatenate([np.arange(r * width + a, r * width + b) for r, a, b in dirty]))
+        at = np.concatenate([np.arange(r * width + a, r * width + b) for r, a, b in dirty])
+        if len(dirty) > 1 and at.size > len(dirty):  # (the same entry twice gets the same page twice)
+            at = np.unique(at)
         host = torch.empty(2, at.size, dtype=torch.int64, pin_memory=True)
         host[0] = torch.from_numpy(at)
         host[1] = torch.from_numpy(self.pages.table.reshape(-1)[at].astype(np.int64))

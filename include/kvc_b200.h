@@ -368,9 +368,10 @@ typedef struct {
  * and cover its kv_len[i] tokens.  A sequence with queries and no items is left
  * to another call on the same step with another split, so that the many queries
  * of one sequence and the few of others can run as each runs best.  max_items and
- * max_new: most items and most queries of one of the split's sequences.  block_start (n_blocks + 1): the items that block k
- * works on are block_start[k] .. block_start[k + 1] - 1; used where
- * kvc_kv4_attend_shape says `spanning`, else every item is a block.
+ * max_new: most items and most queries of one of the split's sequences.
+ * block_start (n_blocks + 1): the items that block k works on are block_start[k] ..
+ * block_start[k + 1] - 1; used where kvc_kv4_attend_shape says `spanning`, else
+ * every item is a block.
  */
 typedef struct {
   const int32_t *items, *item_start, *block_start;
@@ -394,15 +395,16 @@ int kvc_kv4_write(const kvc_kv4_layout* layout, const kvc_kv4_step* step, void* 
 int kvc_kv4_read(const kvc_kv4_layout* layout, const void* pool, int64_t layer_bytes, int n_layers, int row,
                  int64_t t0, int64_t t1, int dtype, void* k_out, void* v_out, void* stream);
 
-/* softmax(scale q k^T) v of the step's queries (n_q heads, a multiple of n_kv)
- * over their sequences' pages.  causal: query i of a sequence's n sees the
- * first kv_len - n + 1 + i tokens, otherwise all kv_len.  A query that sees
- * nothing gets zeros.  Strides in elements, as for kvc_kv4_write. */
 /* For choosing the split: the blocks that work on one item of one KV head, each
  * with other columns (tiles), the blocks that the current device runs at once
  * (resident), and whether a block may work on several items (spanning). */
 int kvc_kv4_attend_shape(const kvc_kv4_layout* layout, int max_new, int n_q, int dtype, int* tiles, int* resident,
                          int* spanning);
+
+/* softmax(scale q k^T) v of the step's queries (n_q heads, a multiple of n_kv)
+ * over their sequences' pages.  causal: query i of a sequence's n sees the
+ * first kv_len - n + 1 + i tokens, otherwise all kv_len.  A query that sees
+ * nothing gets zeros.  Strides in elements, as for kvc_kv4_write. */
 size_t kvc_kv4_attend_workspace_bytes(const kvc_kv4_layout* layout, const kvc_kv4_split* split, int n_q);
 int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* step, const kvc_kv4_split* split,
                    const void* pool, int n_q, const void* q, int64_t q_seq_stride, int64_t q_token_stride,

@@ -30,17 +30,59 @@ __all__ = ["CacheStep", "PagedKVCache"]
 _CHUNK = 256  # tokens of the smallest item of the attention's split
 
 
-class _Upload:
+def _capturing(device: torch.device) -> bool:
+    if device.index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
+class _Fence:
+    """What the cache itself has put on a stream (a table's update, page copies, a
+    step's arrays), for the other streams that use it."""
+
+    __slots__ = ("device", "event", "streams", "buf")
+
+    def __init__(self, device: torch.device, buf: torch.Tensor | None = None) -> None:
+        self.device, self.buf = device, buf  # ``buf``: not to be reused before its uses are done
+        with torch.cuda.device(device):
+            self.event = torch.cuda.Event()
+        self.mark()
+
+    def mark(self) -> None:
+        """The work ends here, on the device's current stream."""
+        with torch.cuda.device(self.device):
+            self.event.record()
+        self.streams = {ops._raw_stream(self.device.index)}  # streams that are behind it
+
+    def use(self, stream: int) -> None:
+        """Put the raw ``stream``, the device's current one, behind the work."""
+        if stream not in self.streams:
+            self._join(stream)
+
+    def _join(self, stream: int) -> None:
+        # a stream under capture cannot wait for one outside; its graph runs after
+        # whatever the program made sure was done before
+        if _capturing(self.device):
+            return
+        cur = torch.cuda.current_stream(self.device)
+        cur.wait_event(self.event)
+        if self.buf is not None:
+            self.buf.record_stream(cur)
+        self.streams.add(stream)
+
+
+class _Upload(_Fence):
     """int32 arrays in one device buffer, copied from pinned memory on the
     current stream (torch keeps that until the copy is done).
 
     Kernels index with these arrays, so on whatever stream one is launched, it
     has to come after the copy, and the buffer must not be reused before it."""
 
-    __slots__ = ("buf", "at", "streams", "event")
+    __slots__ = ("at",)
 
     def __init__(self, arrays: Sequence[np.ndarray], device: torch.device) -> None:
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing(device):
             raise RuntimeError("PagedKVCache: a step is planned on its first use, which cannot be captured into a CUDA "
                                "graph; use the step once before")
         host = torch.empty(max(1, sum(a.size for a in arrays)), dtype=torch.int32, pin_memory=True)
@@ -49,27 +91,8 @@ class _Upload:
             view[n:n + a.size] = a
             offsets.append(n)
             n += a.size
-        with torch.cuda.device(device):
-            self.buf = host.to(device, non_blocking=True)
-            self.event = torch.cuda.Event()
-            self.event.record()
+        super().__init__(device, host.to(device, non_blocking=True))
         self.at = [self.buf.data_ptr() + 4 * o for o in offsets]  # the arrays' addresses
-        self.streams = {ops._raw_stream(device.index)}  # streams that are behind the copy
-
-    def use(self, stream: int) -> None:
-        """Put the raw ``stream``, the device's current one, behind the copy."""
-        if stream not in self.streams:
-            self._join(stream)
-
-    def _join(self, stream: int) -> None:
-        # a stream under capture cannot wait for one outside; its graph runs after
-        # whatever the program made sure was done before
-        if torch.cuda.is_current_stream_capturing():
-            return
-        cur = torch.cuda.current_stream(self.buf.device)
-        cur.wait_event(self.event)
-        self.buf.record_stream(cur)
-        self.streams.add(stream)
 
 
 @dataclass
@@ -176,11 +199,13 @@ class PagedKVCache:
             cache.write(layer, k, v, step)
             out = cache.attend(layer, q, step)
 
-    Launches go to the current stream; use a cache from one stream at a time.
-    ``write`` and ``attend`` may be captured into a CUDA graph once the step has been
-    used outside one (not ``extend``, ``view``, ``fork``, ``compact``); the graph then
-    repeats that step.  There is no
-    gradient through a cache in 4 bits.
+    Launches go to the current stream; use a cache from one stream at a time (what
+    it puts on the device by itself is ordered across streams, ``write`` and
+    ``attend`` are not).  ``write`` and ``attend`` may be captured into a CUDA graph
+    once the step has been used outside one; the graph then repeats that step, and
+    must not outlive the cache, which keeps the captured steps' arrays.  ``extend``,
+    ``compact`` and a step's first use cannot be captured.  There is no gradient
+    through a cache in 4 bits.
     """
 
     def __init__(self, *, n_layers: int, n_pages: int, n_kv_heads: int, head_dim: int, page_size: int = 64,
@@ -212,6 +237,8 @@ class PagedKVCache:
         self.table = torch.zeros(self.pages.table.shape, dtype=torch.int32, device=device)
         self._shapes: dict[tuple[int, int, int], tuple[int, int, bool]] = {}
         self._byte = torch.zeros(1, dtype=torch.uint8, device=device)  # workspaces are empty_like its expansions
+        self._fence = _Fence(device)
+        self._captured: dict[int, CacheStep] = {}  # steps in graphs, whose arrays have to stay
         self._layers = [self.pool.data_ptr() + i * self.pool.stride(0) for i in range(self.n_layers)]
         self._layout = Kv4Layout(self.table.data_ptr(), self.table.stride(0), self.pages.n_pages, self.n_kv_heads,
                                  self.head_dim, self.page_size, self.group_size)
@@ -241,6 +268,7 @@ class PagedKVCache:
 
     def compact(self) -> int:
         """Move the used pages to the pool's start; returns the number of moved pages."""
+        self._no_capture("compact")
         moves = self.pages.compact()
         self._copy(moves)
         self._sync()
@@ -255,6 +283,7 @@ class PagedKVCache:
     def extend(self, seqs: Sequence[int], counts: Sequence[int]) -> CacheStep:
         """Room for ``counts[i]`` new tokens of ``seqs[i]`` (``RuntimeError`` without
         enough free pages, nothing changed then); the step to write and attend them with."""
+        self._no_capture("extend")
         seqs, counts = [int(s) for s in seqs], [int(n) for n in counts]
         self._copy(self.pages.extend(seqs, counts))
         return self._step(seqs, counts, True)
@@ -339,7 +368,11 @@ class PagedKVCache:
             raise IndexError(f"PagedKVCache.{what}: layer {layer} of {self.n_layers}")
         if step.meta is None:
             self._prepare(step)
-        step.meta.use(ops._raw_stream(self.device.index))
+        stream = ops._raw_stream(self.device.index)
+        self._fence.use(stream)
+        step.meta.use(stream)
+        if stream and _capturing(self.device):  # (the default stream, 0, is never captured)
+            self._captured[id(step)] = step
         return self._layers[layer]
 
     # ---- data ---------------------------------------------------------------
@@ -387,17 +420,23 @@ class PagedKVCache:
 
     # ---- internals ---------------------------------------------------------
 
+    def _no_capture(self, what: str) -> None:
+        if _capturing(self.device):
+            raise RuntimeError(f"PagedKVCache.{what}: not possible inside a CUDA graph")
+
     def _copy(self, pairs: list[tuple[int, int]]) -> None:
         if pairs:
+            self._fence.use(ops._raw_stream(self.device.index))
             ops.copy_pages(self.pool, [s for s, _ in pairs], [d for _, d in pairs])
+            self._fence.mark()
 
     def _sync(self) -> None:
         """Bring the device's page table up to the host's."""
+        self._fence.use(ops._raw_stream(self.device.index))
         dirty = self.pages.dirty
         if not dirty:
             return
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("PagedKVCache: the page table has changed and cannot be updated inside a CUDA graph")
+        self._no_capture("read, write or attend after the page table has changed")
         width = self.pages.max_pages
         at = np.concatenate([np.arange(r * width + a, r * width + b) for r, a, b in dirty])
         if len(dirty) > 1 and at.size > len(dirty):  # (the same entry twice gets the same page twice)
@@ -408,3 +447,4 @@ class PagedKVCache:
         dev = host.to(self.device, non_blocking=True)
         self.table.view(-1).index_copy_(0, dev[0], dev[1].to(torch.int32))
         dirty.clear()
+        self._fence.mark()

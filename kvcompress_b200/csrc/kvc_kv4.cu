@@ -1,6 +1,7 @@
 // Writing, reading and moving the pages of the 4-bit KV cache.
 //
-// All three are bound by memory.  A warp of the write and read kernels takes 8
+// Write and read do enough arithmetic to be bound by instruction issue almost as
+// much as by memory, copies by memory alone.  A warp of the write and read kernels takes 8
 // tokens of one head's K and V, 4 lanes a token: lane c of a token holds the
 // features 32 w + 8 c + 0..7, which is both a 16-byte load of a 16-bit input
 // (4 lanes: 64 contiguous bytes) and word w of K's chunk c, so K's codes need
@@ -453,7 +454,8 @@ extern "C" int kvc_kv4_write(const kvc_kv4_layout* layout, const kvc_kv4_step* s
   if (!aligned16(pool)) return fail(KVC_ERR_ALIGN, "kvc_kv4_write: pool not 16-byte aligned");
   if (step->n_halves < 0 || step->n_seqs < 0) return fail(KVC_ERR_SHAPE, "kvc_kv4_write: negative size");
   if (step->n_halves == 0) return KVC_OK;
-  if (!k || !v) return fail(KVC_ERR_ARG, "kvc_kv4_write: NULL pointer");
+  if (!k || !v || !step->rows || !step->kv_len || !step->q_start || !step->half_seq || !step->half_start)
+    return fail(KVC_ERR_ARG, "kvc_kv4_write: NULL pointer");
   if (step->n_halves > INT32_MAX / 4 || layout->n_kv > 65535)
     return fail(KVC_ERR_SHAPE, "kvc_kv4_write: too many tokens or KV heads in one call");
   const dim3 grid((unsigned)ceil_div(step->n_halves, 4), (unsigned)layout->n_kv);

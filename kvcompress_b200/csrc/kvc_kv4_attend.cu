@@ -770,6 +770,7 @@ extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* 
   if (!aligned16(pool)) return fail(KVC_ERR_ALIGN, "kvc_kv4_attend: pool not 16-byte aligned");
   if (n_q < 1 || n_q > 65535 || n_q % layout->n_kv) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: n_q must be a multiple of n_kv");
   if (step->n_tokens == 0 || split->n_items == 0) return KVC_OK;
+  if (!step->rows || !step->kv_len || !step->q_start) return fail(KVC_ERR_ARG, "kvc_kv4_attend: NULL step");
   if (!split->item_start || (!many((int64_t)split->max_new * (n_q / layout->n_kv), dtype) && !split->block_start))
     return fail(KVC_ERR_ARG, "kvc_kv4_attend: NULL split");
   if (!split->items || !aligned16(split->items)) return fail(KVC_ERR_ALIGN, "kvc_kv4_attend: items not 16-byte aligned");

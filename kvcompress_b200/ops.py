@@ -9,6 +9,7 @@ K and V, or many layers): one launch covers the whole batch.
 from __future__ import annotations
 
 import ctypes
+from operator import index
 from typing import Sequence
 
 import torch
@@ -756,7 +757,9 @@ def kv4_attend(layout, step, split, pool: int, query: torch.Tensor, *, causal: b
     n_q = query.shape[1]
     if n_q % layout.n_kv or n_q == 0:
         raise ValueError(f"kv4_attend: {n_q} query heads are no multiple of {layout.n_kv} KV heads")
-    out = torch.empty_like(query)  # (features stay contiguous)
+    out = torch.empty_like(query)
+    if out.stride(-1) != 1:  # (of a query whose strides overlap)
+        out = torch.empty(query.shape, dtype=query.dtype, device=device)
     if step.n_tokens == 0:
         return out
     o, nbytes = out.stride(), 2 * query.numel() * query.element_size()
@@ -831,7 +834,7 @@ def copy_pages(pools, src: Sequence[int], dst: Sequence[int]) -> None:
         raise ValueError(f"copy_pages: {n} sources but {len(dst)} destinations")
     if n == 0 or not ptrs:
         return
-    a, b = (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst)
+    src, dst = list(map(index, src)), list(map(index, dst))  # (tensors on the host have no equality to rely on)
     of, to = set(src), set(dst)
     if len(to) != n:
         raise ValueError("copy_pages: a page is written twice")
@@ -839,6 +842,7 @@ def copy_pages(pools, src: Sequence[int], dst: Sequence[int]) -> None:
         raise ValueError("copy_pages: a page is both read and written")
     if min(min(of), min(to)) < 0 or max(max(of), max(to)) >= n_pages:
         raise ValueError(f"copy_pages: page out of range (pool of {n_pages})")
+    a, b = (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst)
     page_bytes = elems // n_pages * size
     for i in range(0, len(ptrs), KVC.MAX_CELLS):
         part = ptrs[i:i + KVC.MAX_CELLS]

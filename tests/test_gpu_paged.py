@@ -7,8 +7,10 @@ values in float64 under the bound of ``bound``.
 
 from __future__ import annotations
 
+import gc
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -435,6 +437,11 @@ def test_copy_pages(dtype, inner):
     assert torch.equal(pool.view(torch.uint8), raw)
     ops.copy_pages(pool, [], [])
     ops.copy_pages([], [], [])
+    for twice in (torch.tensor([2, 2]), [torch.tensor(2), torch.tensor(2)], np.array([2, 2])):
+        with pytest.raises(ValueError, match="written twice"):
+            ops.copy_pages(pool, [0, 1], twice)
+    with pytest.raises(TypeError):
+        ops.copy_pages(pool, [0.0], [1])
     for bad in (([0], [50]), ([-1], [0]), ([0, 1], [2, 2]), ([0, 1], [1, 2]), ([0], [])):
         with pytest.raises(ValueError):
             ops.copy_pages(pool, *bad)
@@ -578,6 +585,69 @@ def test_a_new_step_is_not_planned_inside_a_graph():
         q.add_(0)
     c.truncate(s, 40)
     check_attend(c, q, c.view([s], [1]), [(k, v)])
+
+
+def test_a_captured_step_may_be_dropped():
+    """The graph's step arrays stay, whatever the allocator hands out afterwards."""
+    c = make(2, 128, 128, 64, 20000, 2, pages=400)
+    s = c.add()
+    k, v = cells(9000, 2, 128, BF16)
+    q = queries(3, 4, 128, BF16)
+    c.write(0, k, v, c.extend([s], [9000]))
+    step = c.view([s], [3])
+    want = c.attend(0, q, step)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = c.attend(0, q, step)
+        with pytest.raises(RuntimeError, match="inside a CUDA graph"):
+            c.extend([s], [1])
+        with pytest.raises(RuntimeError, match="inside a CUDA graph"):
+            c.compact()
+    assert c.length(s) == 9000
+    del step
+    gc.collect()
+    torch.cuda.synchronize()
+    # in range whatever the old arrays' bytes become: all zeros
+    junk = [torch.zeros(n, dtype=torch.int32, device="cuda") for n in (1, 8, 64, 128, 512, 1024) for _ in range(40)]
+    for _ in range(2):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    assert len(junk) == 240 and ops.device_error() == 0
+
+
+def test_page_copies_are_ordered_before_another_streams_use():
+    """extend's copy of a shared page waits on a busy stream; the step is used on another one."""
+    c = make(2, 128, 128, 64, 256, 2)
+    s = c.add()
+    k, v = cells(100, 2, 128, BF16)
+    c.write(0, k[:99], v[:99], c.extend([s], [99]))
+    f = c.fork(s)
+    q = queries(1, 4, 128, BF16)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    torch.cuda._sleep(20_000_000)  # about 10 ms on the current stream
+    step = c.extend([f], [1])
+    with torch.cuda.stream(side):
+        c.write(0, k[99:], v[99:], step)
+        out = c.attend(0, q, step)
+    torch.cuda.synchronize()
+    assert torch.equal(out, c.attend(0, q, step))
+    check_attend(c, q, step, [(k, v)])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("n", [6, 50])
+def test_queries_whose_strides_overlap(dtype, n):
+    c = make(2, 128, 128, 64, 1024, 2)
+    s = c.add()
+    k, v = cells(500, 2, 128, dtype)
+    c.write(0, k, v, c.extend([s], [500]))
+    base = queries(n + 4, 1, 128, dtype).flatten()
+    for q in (base.as_strided((n, 4, 128), (1, 64, 1)), base[:128].expand(n, 4, 128), base.as_strided((n, 4, 128), (2, 2, 1))):
+        out = check_attend(c, q, c.view([s], [n]), [(k, v)])
+        assert torch.equal(out, c.attend(0, q.contiguous(), c.view([s], [n])))
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])

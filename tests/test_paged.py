@@ -202,6 +202,17 @@ def test_abi_refuses_bad_layouts(field, value):
     assert L.kvc_last_error()
 
 
+@pytest.mark.parametrize("field", ["rows", "kv_len", "q_start", "half_seq", "half_start"])
+def test_abi_refuses_missing_step_arrays(field):
+    layout, step, split, p = _abi()
+    setattr(step, field, None)
+    L = lib()
+    assert L.kvc_kv4_write(layout, step, p, p, p, KVC.BF16, 0, 256, 128, 1, None) == KVC.ERR_ARG
+    if not field.startswith("half"):
+        assert L.kvc_kv4_attend(layout, step, split, p, 2, p, 0, 256, 128, p, 0, 256, 128, 1, KVC.BF16, 1, 1.0, None, 0,
+                                None) == KVC.ERR_ARG
+
+
 def test_abi_refuses_bad_arguments():
     layout, step, split, p = _abi()
     L = lib()

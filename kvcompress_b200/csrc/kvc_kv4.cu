@@ -1,7 +1,11 @@
 // Writing, reading and moving the pages of the 4-bit KV cache.
 //
-// Write and read do enough arithmetic to be bound by instruction issue almost as
-// much as by memory, copies by memory alone.  A warp of the write and read kernels takes 8
+// Figures are for one layer of 32768 tokens, 8 heads of 128, bf16, one group a
+// head: 134 MB dense and 36 MB packed, 26 us at the copy peak of 6.55 TB/s.  The
+// write takes 50 us (3.4 TB/s), bound by instruction issue (61% of the slots over
+// the whole launch): it forms 268M exactly rounded codes and moves 1 GB through
+// registers as float32.  The read takes 27 us (6.3 TB/s), bound by memory; page
+// copies reach 96% of the copy peak.  A warp of the write and read kernels takes 8
 // tokens of one head's K and V, 4 lanes a token: lane c of a token holds the
 // features 32 w + 8 c + 0..7, which is both a 16-byte load of a 16-bit input
 // (4 lanes: 64 contiguous bytes) and word w of K's chunk c, so K's codes need
@@ -246,7 +250,8 @@ __device__ __forceinline__ void store_words(uint8_t* dst, const uint32_t (&word)
   else *reinterpret_cast<uint2*>(dst) = make_uint2(word[0], word[1]);
 }
 
-// W = D / 32 words a lane; WPG words a quantisation group.
+// W = D / 32 words a lane; WPG words a quantisation group.  K and V of a token
+// share a warp: twice the loads in flight (a warp each: 62 us instead of 50).
 template <typename T, int D, int WPG>
 __global__ void __launch_bounds__(128) kv4_write_kernel(Layout L, Step S, uint8_t* pool, KvIn in, int n_halves,
                                                         const int32_t* __restrict__ half_seq,
@@ -391,6 +396,8 @@ struct CopyPairs {
   int32_t src[N], dst[N];
 };
 
+// Bound by memory: four 16-byte loads in flight a thread, 16 KB a block; 300
+// pages of 32 KB in each of 32 pools take 100 us (6.3 TB/s read and written).
 template <typename V, int N>
 __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CellPtrsMut pools,
                                                          const __grid_constant__ CopyPairs<N> pairs, int64_t page_bytes,

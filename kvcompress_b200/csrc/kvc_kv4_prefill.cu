@@ -25,6 +25,21 @@
 // reference are normal numbers.  A masked token's weight is 0, but its value may be NaN:
 // such values are written as 0 and their tokens flagged, and a row that does see
 // a flagged token gets NaN in that group at the end.
+//
+// Roundings to 16 bits: K and V (zero + scale q has up to 16 bits) and the
+// weights to float16, half a step of 2^-11 each, which is below bfloat16 queries'
+// own resolution and as large as float16's: 7e-4 of the result of float16 queries
+// over 1500 tokens, where an attention that keeps K and V in float32 is off by 2e-4.
+// Exact values would take a second term of each, and half again to twice the
+// products.  Bfloat16 queries are held in float16 under a power of two a row.
+//
+// Measured: 2048 queries of 32 heads over 8192 tokens (8 KV heads of 128,
+// bfloat16) 308 us, 780 TFLOP/s, 46% of the GEMM peak; 1001 queries of each of 2
+// sequences over 1500 tokens (12 heads of 64, each its own K and V) 31 us.  Bound by latency along one row
+// tile's chain: a step of 128 tokens takes about 4200 clocks, of which the
+// products are 2048 (tensor pipe 45%), the exponentials of both tiles 2048 (41%),
+// and one tile's softmax 2500 from its logits' arrival to its last weights.  One
+// block an SM: 227 KB of shared memory and all of TMEM.
 #include "kvc_kv4_attend.cuh"
 
 namespace kvc {

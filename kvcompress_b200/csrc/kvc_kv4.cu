@@ -2,7 +2,7 @@
 //
 // Figures are for one layer of 32768 tokens, 8 heads of 128, bf16, one group a
 // head: 134 MB dense and 36 MB packed, 26 us at the copy peak of 6.55 TB/s.  The
-// write takes 50 us (3.4 TB/s), bound by instruction issue (61% of the slots over
+// write takes 47.5 us (3.6 TB/s), bound by instruction issue (61% of the slots over
 // the whole launch): it forms 268M exactly rounded codes and moves 1 GB through
 // registers as float32.  The read takes 27 us (6.3 TB/s), bound by memory; page
 // copies reach 96% of the copy peak.  A warp of the write and read kernels takes 8
@@ -251,9 +251,10 @@ __device__ __forceinline__ void store_words(uint8_t* dst, const uint32_t (&word)
 }
 
 // W = D / 32 words a lane; WPG words a quantisation group.  K and V of a token
-// share a warp: twice the loads in flight (a warp each: 62 us instead of 50).
+// share a warp: twice the loads in flight (a warp each: 62 us instead of 50).  Seven
+// blocks an SM where a lane's inputs are 16-bit (72 registers): 50 -> 47.5 us.
 template <typename T, int D, int WPG>
-__global__ void __launch_bounds__(128) kv4_write_kernel(Layout L, Step S, uint8_t* pool, KvIn in, int n_halves,
+__global__ void __launch_bounds__(128, sizeof(T) == 2 ? 7 : 1) kv4_write_kernel(Layout L, Step S, uint8_t* pool, KvIn in, int n_halves,
                                                         const int32_t* __restrict__ half_seq,
                                                         const int32_t* __restrict__ half_start) {
   constexpr int W = D / 32, NG = W / WPG;

@@ -550,7 +550,10 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
       for (int u = 0; u < UNITS; u += SUB) absorb(stages + stage * Sm::stage + u * UB, t0 + u * kUnit, std::true_type{});
     }
     __syncwarp();  // every lane has read the stage
-    if (i + STAGES < mine) issue(i + STAGES, stage);
+    if (i + STAGES < mine) {
+      tc::fence_async_smem();  // the copy's writes come after those reads
+      issue(i + STAGES, stage);
+    }
     if (++stage == STAGES) stage = 0, parity ^= 1;
   }
 

@@ -594,6 +594,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int rs = step % C::RAWS;
         if (step >= C::RAWS) ok = mbar_wait(&bars[C::raw_empty + rs], (step / C::RAWS + 1) & 1, 440);
         if (!__all_sync(0xffffffffu, ok)) break;
+        fence_async_smem();  // the copies' writes come after the reads that freed the place
         if (lane < C::UNITS) {
           if (src) {
             mbar_expect_tx(&bars[C::raw_full + rs], C::UB);

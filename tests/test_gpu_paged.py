@@ -361,6 +361,21 @@ def test_long_caches_are_split_and_joined(lens, nq, hkv):
         assert torch.equal(out, c.attend(0, q, step))  # the joining order is fixed
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("d, group", SHAPES)
+@pytest.mark.parametrize("nq, lens", [(1, [6000, 5000, 17]), (4, [3000, 2999]), (200, [4000])])
+def test_repeated_calls_give_the_same_bits(dtype, d, group, nq, lens):
+    """Rings of codes are refilled while they are read: a call that read too late would differ."""
+    c = make(4, d, group, 32, 8192, len(lens), pages=500)
+    seqs = [c.add() for _ in lens]
+    k, v = cells(sum(lens), 4, d, dtype)
+    c.write(0, k, v, c.extend(seqs, lens))
+    step = c.view(seqs, [nq] * len(lens))
+    q = queries(nq * len(lens), 16, d, dtype)
+    out = c.attend(0, q, step)
+    assert not torch.stack([(c.attend(0, q, step) != out).any() for _ in range(40)]).any()
+
+
 def test_offsets_beyond_32_bits():
     """Pages past 4 GiB of the pool and past 2^31 elements of the output."""
     page, h = 256, 8

@@ -105,7 +105,7 @@ _SIGNATURES = {
     "kvc_kv4_attend_workspace_bytes": (SZ, [_LAYOUT, _SPLIT, I]),
     "kvc_kv4_attend": (I, [_LAYOUT, _STEP, _SPLIT, P, I, P, I64, I64, I64, P, I64, I64, I64, I, I, I,
                            ctypes.c_float, P, SZ, P]),
-    "kvc_copy_pages": (I, [I, PP, I64, I64, I64, P, P, P]),
+    "kvc_copy_pages": (I, [I, P, I64, I64, I64, P, P, P]),
 }
 
 

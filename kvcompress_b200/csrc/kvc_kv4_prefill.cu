@@ -4,8 +4,8 @@
 // A block takes up to 256 rows of one sequence and KV head (a row is a query
 // and a head of the KV head's group: they share K and V) as two tiles of 128,
 // and the tokens of one item in tiles of 128.  With many rows to a token it
-// pays to dequantise once into shared memory, K and V rounded to float16 (their
-// values are at most 65119), and to feed both products from there:
+// pays to dequantise once into shared memory, K and V in float16 (their values are
+// at most 65119), and to feed both products from there:
 //   S = Q K^T    A, B in shared memory, M = N = 128, K = d
 //   O += P V     A = P in TMEM (over the first half of S), B = V^T, N = d
 // Roles: warps 0-3 and 4-7 hold the softmax of one row tile each (a thread a
@@ -26,20 +26,23 @@
 // such values are written as 0 and their tokens flagged, and a row that does see
 // a flagged token gets NaN in that group at the end.
 //
-// Roundings to 16 bits: K and V (zero + scale q has up to 16 bits) and the
-// weights to float16, half a step of 2^-11 each, which is below bfloat16 queries'
-// own resolution and as large as float16's: 7e-4 of the result of float16 queries
-// over 1500 tokens, where an attention that keeps K and V in float32 is off by 2e-4.
-// Exact values would take a second term of each, and half again to twice the
-// products.  Bfloat16 queries are held in float16 under a power of two a row.
+// Roundings to 16 bits: weights to float16, half a step of 2^-11, and K and V
+// (zero + scale q has up to 16 bits) likewise, which bfloat16 queries' own output
+// hides.  Float16 queries would show it (7e-4 of the result over 1500 tokens with
+// loud channels in K, 2e-4 with exact values), so where the tiles fit, for d = 64, K
+// and V are held in two terms, which costs time (1001 queries of each of 2
+// sequences over 1500 tokens, 12 heads of 64: 31 -> 41 us); for d = 128 the second
+// terms would leave one buffer each (306 -> 634 us with K's alone).  Queries are
+// held in float16 under a power of two a row.
 //
 // Measured: 2048 queries of 32 heads over 8192 tokens (8 KV heads of 128,
-// bfloat16) 308 us, 780 TFLOP/s, 46% of the GEMM peak; 1001 queries of each of 2
-// sequences over 1500 tokens (12 heads of 64, each its own K and V) 31 us.  Bound by latency along one row
-// tile's chain: a step of 128 tokens takes about 4200 clocks, of which the
+// bfloat16) 304 us, 790 TFLOP/s, 47% of the GEMM peak; the float16 case above 41
+// us.  Bound by latency along one row tile's chain: a step of 128 tokens takes about 4200 clocks, of which the
 // products are 2048 (tensor pipe 45%), the exponentials of both tiles 2048 (41%),
 // and one tile's softmax 2500 from its logits' arrival to its last weights.  One
 // block an SM: 227 KB of shared memory and all of TMEM.
+#include <type_traits>
+
 #include "kvc_kv4_attend.cuh"
 
 namespace kvc {
@@ -64,14 +67,16 @@ constexpr int kTile = 128;      // rows of a row tile, tokens of a token tile
 constexpr int kThreads = 16 * 32;
 constexpr float kShift = 7.0f;  // weights are 2^7 fold
 
-template <int D, int WPG>
+// TERMS: float16 terms of a value of K and V.
+template <int D, int WPG, int TERMS>
 struct Pre {
   static constexpr int W = D / 32, NG = W / WPG, UB = unit_bytes(D, NG), UNITS = kTile / kUnit;
-  static constexpr int TILE = kTile * D * 2;  // bytes of a Q, K or V tile
+  static constexpr int TILE = kTile * D * 2;  // bytes of a Q tile
   static constexpr int RAW = UNITS * UB;
-  static constexpr int RAWS = 6 * TILE + 2 * RAW + 1024 <= 227 * 1024 ? 2 : 1;  // tiles of codes in flight
+  static constexpr int KV = TERMS * TILE;  // bytes of a K or V tile, its terms one after the other
+  static constexpr int RAWS = 2 * TILE + 4 * KV + 2 * RAW + 1024 <= 227 * 1024 ? 2 : 1;  // tiles of codes in flight
   static constexpr int FLAGS = 4;  // a tile's flags outlive its codes until both softmax tiles are past it
-  static constexpr int q = 0, k = 2 * TILE, v = 4 * TILE, raw = 6 * TILE, flags = raw + RAWS * RAW;
+  static constexpr int q = 0, k = 2 * TILE, v = k + 2 * KV, raw = v + 2 * KV, flags = raw + RAWS * RAW;
   static constexpr int bars = flags + FLAGS * NG * 16;
   // barriers
   static constexpr int q_full = 0, raw_full = 2, raw_empty = raw_full + RAWS, k_full = raw_empty + RAWS,
@@ -155,10 +160,26 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// z + s q, formed in float32, as two float16 terms.
+__device__ __forceinline__ void two_terms(__half2 q, __half2 s, __half2 z, __half2& hi, __half2& lo) {
+  const float2 qf = __half22float2(q), sf = __half22float2(s), zf = __half22float2(z);
+  const float x = fmaf(qf.x, sf.x, zf.x), y = fmaf(qf.y, sf.y, zf.y);
+  hi = __floats2half2_rn(x, y);
+  const float2 h = __half22float2(hi);
+  lo = __floats2half2_rn(x - h.x, y - h.y);
+}
+
+// Two terms where the queries can tell and the tiles fit.
+template <typename T, int D>
+constexpr int terms_of() {
+  return std::is_same<T, __half>::value && D == 64 ? 2 : 1;
+}
+
 template <typename T, int D, int WPG>
 __global__ void __launch_bounds__(kThreads, 1)
     prefill_kernel(Layout L, Step S, Split P, const uint8_t* __restrict__ pool, Qkv a, Partial part, int q_vec, int o_vec) {
-  using C = Pre<D, WPG>;
+  constexpr int TERMS = terms_of<T, D>();
+  using C = Pre<D, WPG, TERMS>;
   constexpr int W = C::W, NG = C::NG;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int4 it = P.items[blockIdx.z];
@@ -420,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool dirty = false;
       if (it < steps) {
         const int step = it, rs = step % C::RAWS, buf = step & 1, t0 = t_begin + step * kTile;
-        const uint32_t raw = rs * C::RAW, tile_at = buf * C::TILE;
+        const uint32_t raw = rs * C::RAW, tile_at = buf * C::KV;
         ok = mbar_wait(&bars[C::raw_full + rs], (step / C::RAWS) & 1, 420);
         if (ok && step >= 2) ok = mbar_wait(&bars[C::k_empty + buf], ((step >> 1) + 1) & 1, 421);
         if (!__all_sync(0xffffffffu, ok)) break;
@@ -439,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + C::flags + ((step % C::FLAGS) * NG + g) * 16 + k * 4), "r"(fl)
                            : "memory");
           }
-#pragma unroll
+#pragma unroll 1  // (unrolled, its loads spill: 2048 queries over 8192 tokens 314 -> 320 us)
         for (int rep = 0; rep < 4; ++rep) {
           uint32_t x[W];
           lds_words<W>(k_src + raw + rep * 2 * C::UB, x);
@@ -450,10 +471,16 @@ __global__ void __launch_bounds__(kThreads, 1)
               const __half2 sz = half2_of(lds32(kp_src + raw + rep * 2 * C::UB + w / WPG * 4));
               s2 = __low2half2(sz), z2 = __high2half2(sz);
             }
-            const uint32_t y = x[w] >> 8;
-            sts128(k_dst[w & 1] + tile_at + (w >> 1) * (kTile * 128) + rep * 4096, bits(__hfma2(centred_lo(x[w]), s2, z2)),
-                   bits(__hfma2(centred_hi(x[w]), s2, z2)), bits(__hfma2(centred_lo(y), s2, z2)),
-                   bits(__hfma2(centred_hi(y), s2, z2)));
+            const uint32_t y = x[w] >> 8, at = k_dst[w & 1] + tile_at + (w >> 1) * (kTile * 128) + rep * 4096;
+            const __half2 q[4] = {centred_lo(x[w]), centred_hi(x[w]), centred_lo(y), centred_hi(y)};
+            __half2 hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (TERMS == 2) two_terms(q[e], s2, z2, hi[e], lo[e]);
+              else hi[e] = __hfma2(q[e], s2, z2);
+            }
+            sts128(at, bits(hi[0]), bits(hi[1]), bits(hi[2]), bits(hi[3]));
+            if constexpr (TERMS == 2) sts128(at + C::TILE, bits(lo[0]), bits(lo[1]), bits(lo[2]), bits(lo[3]));
           }
         }
         fence_async_smem();
@@ -462,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int step = it - (C::RAWS - 1);
       if (step >= 0) {
         const int rs = step % C::RAWS, buf = step & 1, t0 = t_begin + step * kTile;
-        const uint32_t raw = rs * C::RAW, tile_at = buf * C::TILE;
+        const uint32_t raw = rs * C::RAW, tile_at = buf * C::KV;
         const bool check = C::RAWS > 1 ? dirty_before : dirty;
         if (step >= 2) ok = mbar_wait(&bars[C::v_empty + buf], ((step >> 1) + 1) & 1, 422);
         if (!__all_sync(0xffffffffu, ok)) break;
@@ -498,17 +525,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           // nibbles 0..3 are features 1, 0, 3, 2
-          uint32_t o[4][4];
+          uint32_t o[TERMS][4][4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t y = x[k][u] >> 8;
-            o[1][k] = bits(__hfma2(centred_lo(x[k][u]), s2[k], z2[k]));
-            o[0][k] = bits(__hfma2(centred_hi(x[k][u]), s2[k], z2[k]));
-            o[3][k] = bits(__hfma2(centred_lo(y), s2[k], z2[k]));
-            o[2][k] = bits(__hfma2(centred_hi(y), s2[k], z2[k]));
+            const __half2 q[4] = {centred_hi(x[k][u]), centred_lo(x[k][u]), centred_hi(y), centred_lo(y)};
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+              if constexpr (TERMS == 2) {
+                __half2 hi, lo;
+                two_terms(q[f], s2[k], z2[k], hi, lo);
+                o[0][f][k] = bits(hi), o[1][f][k] = bits(lo);
+              } else {
+                o[0][f][k] = bits(__hfma2(q[f], s2[k], z2[k]));
+              }
+            }
           }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) sts128(v_dst[k] + tile_at + u * 4096, o[k][0], o[k][1], o[k][2], o[k][3]);
+          for (int term = 0; term < TERMS; ++term)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              sts128(v_dst[k] + tile_at + term * C::TILE + u * 4096, o[term][k][0], o[term][k][1], o[term][k][2], o[term][k][3]);
         }
         mbar_arrive(&bars[C::raw_empty + rs]);
         fence_async_smem();
@@ -527,13 +564,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       bool ok = true;
       auto scores = [&](int half, int step) {
-        const uint64_t qd = q_desc + (uint32_t)half * (C::TILE >> 4), kd = k_desc + (uint32_t)(step & 1) * (C::TILE >> 4);
+        const uint64_t qd = q_desc + (uint32_t)half * (C::TILE >> 4), kd = k_desc + (uint32_t)(step & 1) * (C::KV >> 4);
         if (elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks) {
-            const uint32_t off = ((ks >> 2) * (kTile * 128) + (ks & 3) * 32) >> 4;
-            umma_f16(tm + half * kTile, qd + off, kd + off, id_s, ks ? 1u : 0u);
-          }
+          for (int term = 0; term < TERMS; ++term)
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) {
+              const uint32_t off = ((ks >> 2) * (kTile * 128) + (ks & 3) * 32) >> 4;
+              umma_f16(tm + half * kTile, qd + off, kd + term * (C::TILE >> 4) + off, id_s, ks || term ? 1u : 0u);
+            }
           umma_commit(&bars[C::s_full + half]);
         }
         __syncwarp();
@@ -551,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int step = 0; ok && step < steps; ++step) {
         ok = mbar_wait(&bars[C::v_full + (step & 1)], (step >> 1) & 1, 432);
-        const uint64_t vd = v_desc + (uint32_t)(step & 1) * (C::TILE >> 4);
+        const uint64_t vd = v_desc + (uint32_t)(step & 1) * (C::KV >> 4);
         for (int half = 0; half < halves; ++half) {
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
@@ -559,9 +598,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
             if (ok && elect_one()) {
 #pragma unroll
-              for (int ks = 0; ks < kTile / 32; ++ks)
-                umma_f16_ts(tm + 2 * kTile + half * D, tm + half * kTile + hf * 32 + ks * 8,
-                            vd + ((hf * (D * 128) + ks * 32) >> 4), id_o, step || hf || ks ? 1u : 0u);
+              for (int term = 0; term < TERMS; ++term)
+#pragma unroll
+                for (int ks = 0; ks < kTile / 32; ++ks)
+                  umma_f16_ts(tm + 2 * kTile + half * D, tm + half * kTile + hf * 32 + ks * 8,
+                              vd + ((term * C::TILE + hf * (D * 128) + ks * 32) >> 4), id_o,
+                              step || hf || ks || term ? 1u : 0u);
               if (hf == 1) umma_commit(&bars[C::o_done + half]);
             }
             __syncwarp();
@@ -616,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <typename T, int D, int WPG>
 int launch(const Layout& L, const Step& S, const Split& P, const uint8_t* pool, const Qkv& a, const Partial& part,
            const dim3& grid, cudaStream_t st) {
-  using C = Pre<D, WPG>;
+  using C = Pre<D, WPG, terms_of<T, D>()>;
   auto kernel = prefill_kernel<T, D, WPG>;
   static std::atomic<uint64_t> done{0};
   if (int rc = allow_shared("prefill_kernel", kernel, C::bytes, done)) return rc;

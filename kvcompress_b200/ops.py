@@ -9,7 +9,7 @@ K and V, or many layers): one launch covers the whole batch.
 from __future__ import annotations
 
 import ctypes
-from operator import index
+from array import array
 from typing import Sequence
 
 import torch
@@ -818,7 +818,7 @@ def copy_pages(pools, src: Sequence[int], dst: Sequence[int]) -> None:
         if not pools.is_contiguous():
             raise ValueError("copy_pages: pools must be contiguous")
         base, step, size = pools.data_ptr(), pools.stride(0) * pools.element_size(), pools.element_size()
-        ptrs, n_pages, elems, device = [base + i * step for i in range(shape[0])], shape[1], pools.stride(0), pools.device
+        ptrs, n_pages, elems, device = [base + i * step for i in range(shape[0])], shape[1], pools[:1].numel(), pools.device
     else:
         xs = list(pools)
         for i in range(0, len(xs), KVC.MAX_CELLS):
@@ -834,17 +834,20 @@ def copy_pages(pools, src: Sequence[int], dst: Sequence[int]) -> None:
         raise ValueError(f"copy_pages: {n} sources but {len(dst)} destinations")
     if n == 0 or not ptrs:
         return
-    src, dst = list(map(index, src)), list(map(index, dst))  # (tensors on the host have no equality to rely on)
-    of, to = set(src), set(dst)
+    try:
+        a, b = array("i", src), array("i", dst)
+    except OverflowError:
+        raise ValueError(f"copy_pages: page out of range (pool of {n_pages})") from None
+    of, to = set(a), set(b)
     if len(to) != n:
         raise ValueError("copy_pages: a page is written twice")
     if not to.isdisjoint(of):
         raise ValueError("copy_pages: a page is both read and written")
     if min(min(of), min(to)) < 0 or max(max(of), max(to)) >= n_pages:
         raise ValueError(f"copy_pages: page out of range (pool of {n_pages})")
-    a, b = (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst)
     page_bytes = elems // n_pages * size
     for i in range(0, len(ptrs), KVC.MAX_CELLS):
-        part = ptrs[i:i + KVC.MAX_CELLS]
+        part = array("Q", ptrs[i:i + KVC.MAX_CELLS])
         _call("copy_pages", device, 2 * n * page_bytes * len(part), lib().kvc_copy_pages, len(part),
-              (ctypes.c_void_p * len(part))(*part), n_pages, page_bytes, n, a, b)
+              part.buffer_info()[0], n_pages, page_bytes, n, a.buffer_info()[0],
+              b.buffer_info()[0])

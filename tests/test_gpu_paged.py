@@ -452,6 +452,11 @@ def test_copy_pages(dtype, inner):
     assert torch.equal(pool.view(torch.uint8), raw)
     ops.copy_pages(pool, [], [])
     ops.copy_pages([], [], [])
+    ops.copy_pages(torch.empty(3, 5, 0, device="cuda"), [0], [1])
+    ops.copy_pages(torch.empty(0, 5, 2, device="cuda"), [0], [1])
+    for far in (1 << 31, -(1 << 40)):
+        with pytest.raises(ValueError, match="out of range"):
+            ops.copy_pages(pool, [0], [far])
     for twice in (torch.tensor([2, 2]), [torch.tensor(2), torch.tensor(2)], np.array([2, 2])):
         with pytest.raises(ValueError, match="written twice"):
             ops.copy_pages(pool, [0, 1], twice)

@@ -199,7 +199,8 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
   const uint32_t ring = tc::smem_u32(smem) + warp * STAGES * Sm::stage + (lane % UNITS) * UB;
   const uint8_t* src = nullptr;
   auto look = [&](int i) {  // pages of runs i .. i + AHEAD - 1
-    const int t = t_begin + (warp + (i + lane / UNITS) * WARPS) * TOKENS + (lane % UNITS) * kUnit;
+    const int run = i + lane / UNITS;  // (the position of one past the last may not fit in 32 bits)
+    const int t = run < mine ? t_begin + (warp + run * WARPS) * TOKENS + (lane % UNITS) * kUnit : t_end;
     src = nullptr;
     if (t < t_end) {
       const int64_t page = page_of(L, it.w, t, &tc::g_kvc_device_error);

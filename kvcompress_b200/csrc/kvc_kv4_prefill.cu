@@ -625,8 +625,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---- bring the codes: lane u copies unit u of each tile
       bool ok = true;
       auto page = [&](int step) -> const uint8_t* {
+        if (lane >= C::UNITS || step >= steps) return nullptr;  // (the position may not fit in 32 bits)
         const int t = t_begin + step * kTile + lane * kUnit;
-        if (lane >= C::UNITS || step >= steps || t >= t_end) return nullptr;
+        if (t >= t_end) return nullptr;
         const int64_t p = page_of(L, it.w, t, &g_kvc_device_error);
         return pool + unit_off<D>(L, p < 0 ? 0 : p, h, t);  // a bad entry reads page 0: wrong, but in range
       };

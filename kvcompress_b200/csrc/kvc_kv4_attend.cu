@@ -21,9 +21,13 @@
 // What the kernel rounds: queries of 16 bits not at all (float16 with a power
 // of two per row), float32 ones to two float16 terms (22 bits); p s' to
 // float16 under a power of two that keeps its maximum near the top of the
-// range (two terms for float32 queries).  The sum that the constant 8 s'
-// multiplies is formed from the rounded weights, so their rounding acts on
-// c' - 8 and not on c'.
+// range (two terms for float32 queries, the second under 2^11 more).  That power
+// is each column's and group's own and goes by the tokens that the column sees, so
+// that a quiet group beside a loud one, or queries before a loud token, keep their
+// bits.  What remains: where p s' is below 2^-21 of its group's largest s' (p = 1 at
+// the running maximum) it is rounded to steps of 2^-31 of that (2^-42 with two
+// terms).  The sum that the constant 8 s' multiplies is formed from the rounded
+// weights, so their rounding acts on c' - 8 and not on c'.
 //
 // A block takes up to 8 NT columns (a column is a query and a head of the KV
 // head's group: all of them read the same codes) and its items, runs of tokens
@@ -65,7 +69,9 @@ int kv4_attend_read_device_error(int* out) {
 namespace kv4 {
 namespace {
 
-constexpr float kTop = 128.0f;  // weights p s' are held as (p s' / cap) * kTop <= 2^8 * 2^7 < 65504
+constexpr float kTop = 128.0f;  // weights p s' are held as p s' hold <= 2^8 * 2^7 < 65504
+constexpr uint32_t kUnheld = 127 + 100;  // exponent of 2^100: any value scale asks for less
+constexpr float kLow = 2048.0f;  // a weight's second term is held so many fold, which keeps it a normal number as long as the first
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -80,6 +86,27 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+
+// 1 / x of a power of two within 2^-126 .. 2^126.
+__device__ __forceinline__ float pow2_inverse(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
+
+// Powers of two, one for each of two columns and NG groups, as the bytes of their exponents.
+template <int NG>
+struct Pow2 {
+  uint32_t word[NG == 4 ? 2 : 1];
+  __device__ __forceinline__ void fill(uint32_t exponent) {
+#pragma unroll
+    for (uint32_t& w : word) w = exponent * 0x01010101u;
+  }
+  __device__ __forceinline__ float get(int j, int g) const {
+    const int at = j * NG + g;
+    return __uint_as_float((word[at / 4] >> (8 * (at % 4)) & 0xFFu) << 23);
+  }
+  __device__ __forceinline__ void set(int j, int g, float x) {
+    const int at = j * NG + g, shift = 8 * (at % 4);
+    word[at / 4] = (word[at / 4] & ~(0xFFu << shift)) | __float_as_uint(x) >> 23 << shift;
+  }
+};
 
 // Two codes of a word as a float16 operand: nibble 0 (lo) or 1 (hi, 16 fold) of
 // each half; plain codes are 2^-24 fold, centred ones c - 8.
@@ -303,9 +330,12 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
   // Logits are kept in raw units (fac times them is log2 units).  A column's
   // reference mf (log2 units) is raised when a logit exceeds mt.
   float o[NT][2 * W][4], mf[NT][2], mt[NT][2], l[NT][2], z[NT][2][NG], zc[NT][NG][4];
-  float cap = 0.0f, hold = 0.0f;  // value scales are at most cap; hold = kTop / cap
+  // Each column's and group's own: kTop over a power of two that the value scales
+  // it has seen stay below (kUnheld: none yet).
+  Pow2<NG> hold[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
+    hold[nt].fill(kUnheld);
 #pragma unroll
     for (int i = 0; i < 2 * W; ++i)
 #pragma unroll
@@ -404,8 +434,16 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
     }
 
     // value parameters; raise the references where they have to be
+    // (all columns' value scales are the same until some are masked)
+    constexpr int HN = MASKED ? NT : 1, HJ = MASKED ? 2 : 1;
     float2 vp[SUB][2][NG];
-    float vtop = 0.0f;
+    float vtop[HN][HJ][NG];
+#pragma unroll
+    for (int nt = 0; nt < HN; ++nt)
+#pragma unroll
+      for (int j = 0; j < HJ; ++j)
+#pragma unroll
+        for (int g = 0; g < NG; ++g) vtop[nt][j][g] = 0.0f;
 #pragma unroll
     for (int u = 0; u < SUB; ++u)
 #pragma unroll
@@ -414,30 +452,38 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
         lds_words<NG>(sub + u * UB + vp_base(D, NG) + (r + 8 * i2) * NG * 4, words);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          float2 p = unpack_half2(words[g]);
-          if (MASKED && ts + u * kUnit + r + 8 * i2 >= t_end) p = make_float2(0.0f, 0.0f);
+          const float2 p = unpack_half2(words[g]);
           vp[u][i2][g] = p;
-          vtop = fmaxf(vtop, p.x);
+#pragma unroll
+          for (int nt = 0; nt < HN; ++nt)
+#pragma unroll
+            for (int j = 0; j < HJ; ++j)
+              vtop[nt][j][g] = fmaxf(vtop[nt][j][g], MASKED && s[u][nt][2 * i2 + j] == -INFINITY ? 0.0f : p.x);
         }
       }
-    bool raise = vtop > cap;
+    bool raise = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) raise |= top[nt][0] > mt[nt][0] || top[nt][1] > mt[nt][1];
+#pragma unroll
+    for (int nt = 0; nt < HN; ++nt)
+#pragma unroll
+      for (int j = 0; j < HJ; ++j)
+#pragma unroll
+        for (int g = 0; g < NG; ++g) raise |= vtop[nt][j][g] * hold[nt].get(j, g) > kTop;
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int k = 4; k <= 16; k <<= 1) {
-        vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, k));
+#pragma unroll
+        for (int nt = 0; nt < HN; ++nt)
+#pragma unroll
+          for (int j = 0; j < HJ; ++j)
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+              vtop[nt][j][g] = fmaxf(vtop[nt][j][g], __shfl_xor_sync(0xffffffffu, vtop[nt][j][g], k));
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) top[nt][j] = fmaxf(top[nt][j], __shfl_xor_sync(0xffffffffu, top[nt][j], k));
-      }
-      float fcap = 1.0f;
-      if (vtop > cap) {  // the next power of two above it
-        const float up = 2.0f * __uint_as_float(__float_as_uint(vtop) & 0x7F800000u);
-        fcap = cap / up;
-        cap = up;
-        hold = kTop / up;
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -452,12 +498,19 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
           }
           l[nt][j] *= f;
 #pragma unroll
-          for (int g = 0; g < NG; ++g) z[nt][j][g] *= f;
-          f *= fcap;
+          for (int g = 0; g < NG; ++g) {
+            z[nt][j][g] *= f;
+            const float most = vtop[MASKED ? nt : 0][MASKED ? j : 0][g];
+            float fg = f;
+            if (const float was = hold[nt].get(j, g); most * was > kTop) {  // the next power of two above it
+              const float h = kTop * 0.5f * pow2_inverse(__uint_as_float(__float_as_uint(most) & 0x7F800000u));
+              fg *= h * pow2_inverse(was);
+              hold[nt].set(j, g, h);
+            }
 #pragma unroll
-          for (int i2 = 0; i2 < 2 * W; ++i2) o[nt][i2][j] *= f, o[nt][i2][j + 2] *= f;
-#pragma unroll
-          for (int g = 0; g < NG; ++g) zc[nt][g][j] *= f;
+            for (int i2 = 2 * g * WPG; i2 < 2 * (g + 1) * WPG; ++i2) o[nt][i2][j] *= fg, o[nt][i2][j + 2] *= fg;
+            zc[nt][g][j] *= fg;
+          }
         }
     }
 
@@ -483,8 +536,8 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
 #pragma unroll
           for (int i2 = 0; i2 < 2; ++i2) {
             const float2 vs = vp[u][i2][g];
-            const float held = vs.x * hold;
-            float w0 = p[2 * i2] * held, w1 = p[2 * i2 + 1] * held;
+            float w0 = p[2 * i2] * (vs.x * hold[MASKED ? nt : 0].get(0, g));
+            float w1 = p[2 * i2 + 1] * (vs.x * hold[MASKED ? nt : 0].get(MASKED ? 1 : 0, g));
             if constexpr (MASKED) {  // a token that a column does not see may hold NaN
               const bool n0 = s[u][nt][2 * i2] == -INFINITY, n1 = s[u][nt][2 * i2 + 1] == -INFINITY;
               w0 = n0 ? 0.0f : w0;
@@ -499,7 +552,7 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
             pf[0][nt][g][i2] = transpose8x8(hi);
             if constexpr (TERMS == 2) {
               const float2 got = unpack_half2(hi);
-              pf[1][nt][g][i2] = transpose8x8(pack_half2(w0 - got.x, w1 - got.y));
+              pf[1][nt][g][i2] = transpose8x8(pack_half2((w0 - got.x) * kLow, (w1 - got.y) * kLow));
             }
           }
         if constexpr (!CENTRED) {  // the rounded weights' sums: a product with ones
@@ -517,14 +570,14 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
                          a3 = codes_hi<CENTRED>(y1);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float part[TERMS][4] = {};
 #pragma unroll
-            for (int term = TERMS - 1; term >= 0; --term)
-              mma16816(CENTRED ? part : o[nt][2 * w + i2], a0, a1, a2, a3, pf[term][nt][w / WPG][0],
+            for (int term = 0; term < TERMS; ++term)
+              mma16816(CENTRED ? part[term] : o[nt][2 * w + i2], a0, a1, a2, a3, pf[term][nt][w / WPG][0],
                        pf[term][nt][w / WPG][1]);
             if constexpr (CENTRED)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[nt][2 * w + i2][e] += part[e];
+              for (int e = 0; e < 4; ++e) o[nt][2 * w + i2][e] += fmaf(part[1][e], 1.0f / kLow, part[0][e]);
           }
           y0 >>= 8;
           y1 >>= 8;
@@ -573,10 +626,10 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
 #pragma unroll
         for (int g = 0; g < NG; ++g) z[nt][j][g] += __shfl_xor_sync(0xffffffffu, z[nt][j][g], k);
       }
-      const float unhold = cap * (1.0f / kTop), f0 = unhold * kCode, f1 = f0 * 0.0625f;
       float* dst = so + (warp * COLS + col) * Sm::o_stride + 4 * r;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
+        const float unhold = pow2_inverse(hold[nt].get(j, w / WPG)), f0 = unhold * kCode, f1 = f0 * 0.0625f;
         const float zg = CENTRED ? z[nt][j][w / WPG] : fmaf(-8.0f * unhold, zc[nt][w / WPG][j], z[nt][j][w / WPG]);
         *reinterpret_cast<float4*>(dst + 32 * w) =
             make_float4(fmaf(o[nt][2 * w][j + 2], f1, zg), fmaf(o[nt][2 * w][j], f0, zg),

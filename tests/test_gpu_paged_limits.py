@@ -5,7 +5,7 @@ from __future__ import annotations
 
 import pytest
 import torch
-from test_gpu_paged import BF16, FP32, attention, cells, held, make, queries
+from test_gpu_paged import BF16, FP16, FP32, attention, cells, held, make, queries
 
 from kvcompress_b200 import ops
 
@@ -39,3 +39,73 @@ def test_the_longest_sequence(dtype, nq):
     tol = (5.4e-2 if nq == 16 else 7e-3) + torch.finfo(dtype).eps / 2
     assert (got - want).abs().max() <= tol * v.abs().max()
     assert ops.device_error() == 0
+
+
+# ---- value scales that lie far apart -----------------------------------------
+
+# How far a group of an output may be off, relative to that group's own norm over all rows.  16-bit outputs: half a step of
+# their type (bf16 3.9e-3, fp16 4.9e-4), which over many elements averages below its maximum, and the weights' float16
+# half step (4.9e-4), which independent weights average too: their maxima together for bf16, 6e-4 for fp16 (the mean of the two
+# squared is 3.4e-4).  float32: logits of sum |q k| <= 5 or so from two-term queries (22 bits) and float32 sums,
+# 5 (2^-22 + 2^-21) = 3.6e-6, two-term weights 2^-22.
+GROUP_TOL = {BF16: 4.4e-3, FP16: 6e-4, FP32: 4e-6}
+
+
+def group_errors(c, q, s, k, v, rows=slice(None)):
+    got = c.attend(0, q, c.view([s], [q.shape[0]]))
+    want, _ = attention(q, held(k, c.group_size), held(v, c.group_size), True, c.head_dim ** -0.5)
+    got, want = (x.double()[rows].unflatten(-1, (-1, c.group_size)) for x in (got, want))
+    return ((got - want) ** 2).sum((0, 1, 3)).sqrt() / (want ** 2).sum((0, 1, 3)).sqrt()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("d, group", [(64, 32), (128, 64), (128, 32)])
+@pytest.mark.parametrize("nq", [1, 7, 40])
+@pytest.mark.parametrize("far", [12, 20])
+def test_quiet_groups_beside_loud_ones(dtype, d, group, nq, far):
+    """Every second group's values are 2^12 or 2^20 times as large as the others'."""
+    c = make(1, d, group, 64, 2048, 1)
+    s = c.add()
+    k, v = cells(2000, 1, d, FP32)
+    up = 13 if far == 20 else 6
+    v = v * torch.where(torch.arange(d, device="cuda") // group % 2 == 0, 2.0 ** up, 2.0 ** (up - far))
+    k, v = k.to(dtype), v.to(dtype)
+    c.write(0, k, v, c.extend([s], [2000]))
+    off = group_errors(c, queries(nq, 4, d, dtype, size=0.5), s, k, v)
+    assert (off <= GROUP_TOL[dtype]).all(), off
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("d, group", [(64, 64), (128, 128), (128, 64), (128, 32)])
+@pytest.mark.parametrize("heads", [1, 2, 3])
+def test_loud_tokens_that_only_later_queries_see(dtype, d, group, heads):
+    """The last four tokens' values are 2^20 times as large: the first four queries' results must not know."""
+    c = make(1, d, group, 64, 2048, 1)
+    s = c.add()
+    k, v = cells(1500, 1, d, FP32)
+    v[:-4] *= 2.0 ** -7
+    v[-4:] *= 2.0 ** 13
+    k, v = k.to(dtype), v.to(dtype)
+    c.write(0, k, v, c.extend([s], [1500]))
+    q = queries(8, heads, d, dtype, size=0.5)
+    for rows in (slice(0, 4), slice(4, 8)):
+        off = group_errors(c, q, s, k, v, rows)
+        assert (off <= GROUP_TOL[dtype]).all(), (rows, off)
+
+
+@pytest.mark.parametrize("d, group", [(64, 64), (128, 128), (128, 32)])
+@pytest.mark.parametrize("nq", [1, 6])
+def test_a_loud_token_of_next_to_no_weight(d, group, nq):
+    """One token's values are 2^18 times as large, and its weight e^-25: the others' weights keep their bits."""
+    c = make(1, d, group, 64, 2048, 1)
+    s = c.add()
+    k, v = cells(1500, 1, d, FP32)
+    v = v * 2.0 ** -8
+    q = queries(nq, 4, d, FP32, size=0.02)
+    q[..., -1] = 4.0
+    k[..., -1] = 0.0
+    k[100, 0, -1] = -6.25 * d ** 0.5
+    v[100] *= 2.0 ** 18
+    c.write(0, k, v, c.extend([s], [1500]))
+    off = group_errors(c, q, s, k, v)
+    assert (off <= GROUP_TOL[FP32]).all(), off

@@ -175,7 +175,7 @@ struct Smem {
 
 template <int D, int WPG, int NT, int TERMS>
 __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D, WPG, NT, TERMS>::blocks)
-    attend_kernel(Layout L, Step S, Split P, const uint8_t* __restrict__ pool, Qkv a, Partial part) {
+    attend_kernel(Layout L, Step S, Split P, const uint8_t* __restrict__ pool, Qkv a, Partial part, int tile0) {
   using Sh = Shape<D, WPG, NT, TERMS>;
   using Sm = Smem<D, WPG, NT, TERMS>;
   constexpr int W = D / 32, NG = W / WPG, UB = unit_bytes(D, NG), WARPS = Sh::warps, STAGES = Sm::stages;
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(Shape<D, WPG, NT, TERMS>::warps * 32, Shape<D,
   __shared__ uint64_t full[WARPS][STAGES];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const int h = blockIdx.y, col0 = blockIdx.z * COLS, group = a.n_q / L.n_kv;
+  const int h = blockIdx.y, col0 = (tile0 + (int)blockIdx.z) * COLS, group = a.n_q / L.n_kv;
   if (lane == 0)
     for (int i = 0; i < STAGES; ++i) tc::mbar_init(&full[warp][i], UNITS);
   tc::mbar_fence_init();
@@ -769,9 +769,13 @@ int launch(const Layout& L, const Step& S, const Split& P, const void* pool, con
   auto kernel = attend_kernel<D, WPG, NT, TERMS>;
   static std::atomic<uint64_t> done{0};
   if (int rc = allow_shared("attend_kernel", kernel, Sm::bytes, done)) return rc;
-  const dim3 grid((unsigned)n_blocks, (unsigned)L.n_kv, (unsigned)col_tiles);
-  return launch_after("attend_kernel", kernel, grid, Shape<D, WPG, NT, TERMS>::warps * 32, Sm::bytes, st, L, S, P,
-                      static_cast<const uint8_t*>(pool), a, part);
+  for (int tile0 = 0; tile0 < col_tiles; tile0 += kGridZ) {
+    const dim3 grid((unsigned)n_blocks, (unsigned)L.n_kv, (unsigned)std::min(kGridZ, col_tiles - tile0));
+    if (int rc = launch_after("attend_kernel", kernel, grid, Shape<D, WPG, NT, TERMS>::warps * 32, Sm::bytes, st, L, S, P,
+                              static_cast<const uint8_t*>(pool), a, part, tile0))
+      return rc;
+  }
+  return KVC_OK;
 }
 
 template <int D, int WPG>
@@ -779,7 +783,7 @@ int launch_tiles(const Layout& L, const Step& S, const Split& P, const void* poo
                  int64_t n_blocks, int cols, cudaStream_t st) {
   const int terms = a.dtype == KVC_F32 ? 2 : 1, nt = tiles_of(cols);
   const int tiles = (int)ceil_div(cols, 8 * nt);
-  if (tiles > 65535 || L.n_kv > 65535) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: too many queries or KV heads");
+  if (L.n_kv > 65535) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: too many KV heads");
   if (terms == 2)
     return nt == 1 ? launch<D, WPG, 1, 2>(L, S, P, pool, a, part, n_blocks, tiles, st)
                    : launch<D, WPG, 2, 2>(L, S, P, pool, a, part, n_blocks, tiles, st);

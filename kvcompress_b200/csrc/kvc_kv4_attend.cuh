@@ -7,6 +7,7 @@
 namespace kvc {
 namespace kv4 {
 
+constexpr int kGridZ = 65535;  // a grid's largest extent in z: more column tiles or items are several launches
 constexpr float kLog2e = 1.4426950408889634f;
 // log2 units a logit may exceed its row's reference by: raising costs a pass over
 // the accumulators, and float16 weights have room for 2^15 (4 instead of 8: 5% more

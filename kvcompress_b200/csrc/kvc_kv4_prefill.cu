@@ -41,6 +41,7 @@
 // products are 2048 (tensor pipe 45%), the exponentials of both tiles 2048 (41%),
 // and one tile's softmax 2500 from its logits' arrival to its last weights.  One
 // block an SM: 227 KB of shared memory and all of TMEM.
+#include <algorithm>
 #include <type_traits>
 
 #include "kvc_kv4_attend.cuh"
@@ -177,12 +178,14 @@ constexpr int terms_of() {
 
 template <typename T, int D, int WPG>
 __global__ void __launch_bounds__(kThreads, 1)
-    prefill_kernel(Layout L, Step S, Split P, const uint8_t* __restrict__ pool, Qkv a, Partial part, int q_vec, int o_vec) {
+    prefill_kernel(Layout L, Step S, Split P, const uint8_t* __restrict__ pool, Qkv a, Partial part, int q_vec, int o_vec,
+                   int item0) {
   constexpr int TERMS = terms_of<T, D>();
   using C = Pre<D, WPG, TERMS>;
   constexpr int W = C::W, NG = C::NG;
   extern __shared__ __align__(1024) uint8_t smem[];
-  const int4 it = P.items[blockIdx.z];
+  const int item = item0 + (int)blockIdx.z;
+  const int4 it = P.items[item];
   const int b = it.x, t_begin = it.y, len = S.kv_len[it.x], h = blockIdx.y;
   const int q0 = S.q_start[b], n = S.q_start[b + 1] - q0, group = a.n_q / L.n_kv, rows = n * group;
   // late rows see the most tokens: they go first
@@ -194,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     grid_wait();
     grid_go();
     for (int row = row0 + threadIdx.x; tile >= 0 && row <= last; row += kThreads)
-      part.ml[((int64_t)blockIdx.z * L.n_kv + h) * part.cols + row] = make_float2(-INFINITY, 0.0f);
+      part.ml[((int64_t)item * L.n_kv + h) * part.cols + row] = make_float2(-INFINITY, 0.0f);
     return;
   }
   const int steps = t_end > t_begin ? (t_end - t_begin + kTile - 1) / kTile : 0;
@@ -380,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool alone = P.item_start[b + 1] - P.item_start[b] == 1;
       const float inv = l == 0.0f ? 0.0f : alone ? 1.0f / l : 1.0f;
       const int64_t at = alone ? (a.packed ? (int64_t)(q0 + j) * a.o_st : b * a.o_sb + j * a.o_st) + (int64_t)(h * group + g0) * a.o_sh
-                               : (((int64_t)blockIdx.z * L.n_kv + h) * part.cols + row) * D;
+                               : (((int64_t)item * L.n_kv + h) * part.cols + row) * D;
 #pragma unroll
       for (int ch = 0; ch < D / 32; ++ch) {
         float o[32];
@@ -658,14 +661,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <typename T, int D, int WPG>
 int launch(const Layout& L, const Step& S, const Split& P, const uint8_t* pool, const Qkv& a, const Partial& part,
-           const dim3& grid, cudaStream_t st) {
+           int64_t tiles, int64_t n_items, cudaStream_t st) {
   using C = Pre<D, WPG, terms_of<T, D>()>;
   auto kernel = prefill_kernel<T, D, WPG>;
   static std::atomic<uint64_t> done{0};
   if (int rc = allow_shared("prefill_kernel", kernel, C::bytes, done)) return rc;
   const int q_vec = aligned16(a.q) && ((a.q_sb | a.q_st | a.q_sh) & 7) == 0;
   const int o_vec = aligned16(a.out) && ((a.o_sb | a.o_st | a.o_sh) & 7) == 0;
-  return launch_after("prefill_kernel", kernel, grid, kThreads, C::bytes, st, L, S, P, pool, a, part, q_vec, o_vec);
+  for (int64_t item0 = 0; item0 < n_items; item0 += kGridZ) {
+    const dim3 grid((unsigned)tiles, (unsigned)L.n_kv, (unsigned)std::min<int64_t>(kGridZ, n_items - item0));
+    if (int rc = launch_after("prefill_kernel", kernel, grid, kThreads, C::bytes, st, L, S, P, pool, a, part, q_vec, o_vec,
+                              (int)item0))
+      return rc;
+  }
+  return KVC_OK;
 }
 
 }  // namespace
@@ -674,13 +683,11 @@ int launch_prefill(const kvc_kv4_layout* l, const Step& S, const Split& P, const
                    const Partial& part, int64_t n_items, cudaStream_t st) {
   const Layout L = to_layout(l);
   const int64_t tiles = prefill_tiles(part.cols);
-  if (n_items > 65535 || L.n_kv > 65535 || tiles > INT32_MAX)
-    return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: too many queries, items or KV heads");
-  const dim3 grid((unsigned)tiles, (unsigned)L.n_kv, (unsigned)n_items);
+  if (L.n_kv > 65535) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: too many KV heads");
   int rc = KVC_OK;
 #define KVC_F(D, WPG)                                                                             \
-  rc = a.dtype == KVC_F16 ? launch<__half, D, WPG>(L, S, P, pool, a, part, grid, st)              \
-                          : launch<__nv_bfloat16, D, WPG>(L, S, P, pool, a, part, grid, st)
+  rc = a.dtype == KVC_F16 ? launch<__half, D, WPG>(L, S, P, pool, a, part, tiles, n_items, st)              \
+                          : launch<__nv_bfloat16, D, WPG>(L, S, P, pool, a, part, tiles, n_items, st)
   KVC_KV4_DISPATCH(l, KVC_F);
 #undef KVC_F
   return rc;

@@ -109,3 +109,37 @@ def test_a_loud_token_of_next_to_no_weight(d, group, nq):
     c.write(0, k, v, c.extend([s], [1500]))
     off = group_errors(c, q, s, k, v)
     assert (off <= GROUP_TOL[FP32]).all(), off
+
+
+# ---- more columns or items than a grid's third extent ---------------------------
+
+
+def same_for_all(q, k, v, group):
+    """Each query (n, H, d) over all of k and v (T, 1, d), in float64."""
+    k, v = held(k, group)[:, 0], held(v, group)[:, 0]
+    return torch.softmax(q.double() @ k.T * q.shape[-1] ** -0.5, -1) @ v
+
+
+def test_more_than_65535_tiles_of_float32_columns():
+    c = make(1, 64, 64, 16, 64, 1)
+    s = c.add()
+    k, v = cells(40, 1, 64, FP32)
+    c.write(0, k, v, c.extend([s], [40]))
+    q = queries(1025, 1024, 64, FP32)  # 1049600 columns in tiles of 16
+    got = c.attend(0, q, c.view([s], [1025]), causal=False)
+    want = same_for_all(q, k, v, 64)
+    assert (got - want).norm() <= 1e-5 * want.norm()
+    assert (got - want).abs().max() <= 1e-4 * v.abs().max()
+
+
+def test_more_than_65535_items_of_many_columns():
+    c = make(1, 64, 64, 16, 64, 1)
+    s = c.add()
+    k, v = cells(20, 1, 64, BF16)
+    c.write(0, k, v, c.extend([s], [20]))
+    n = 65600
+    q = queries(n, 40, 64, BF16)  # 40 columns each: the kernel for many queries
+    got = c.attend(0, q, c.view([s] * n, [1] * n))
+    want = same_for_all(q, k, v, 64)
+    assert (got - want).norm() <= 5e-3 * want.norm()
+    assert (got - want).abs().max() <= 2 ** -7 * v.abs().max()

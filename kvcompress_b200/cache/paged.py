@@ -232,11 +232,13 @@ class PagedKVCache:
         self.device = device
         self._scale = self.head_dim ** -0.5
         self.page_bytes = ops.kv4_page_bytes(self.n_kv_heads, self.head_dim, self.page_size, self.group_size)
-        # zeros: a page's bytes are defined before its first tokens are written
-        self.pool = torch.zeros(self.n_layers, self.pages.n_pages, self.page_bytes, dtype=torch.uint8, device=device)
-        self.table = torch.zeros(self.pages.table.shape, dtype=torch.int32, device=device)
+        # (no inference tensors: a cache made in inference mode is updated outside it too)
+        with torch.inference_mode(False):
+            # zeros: a page's bytes are defined before its first tokens are written
+            self.pool = torch.zeros(self.n_layers, self.pages.n_pages, self.page_bytes, dtype=torch.uint8, device=device)
+            self.table = torch.zeros(self.pages.table.shape, dtype=torch.int32, device=device)
+            self._byte = torch.zeros(1, dtype=torch.uint8, device=device)  # workspaces are empty_like its expansions
         self._shapes: dict[tuple[int, int, int], tuple[int, int, bool]] = {}
-        self._byte = torch.zeros(1, dtype=torch.uint8, device=device)  # workspaces are empty_like its expansions
         self._fence = _Fence(device)
         self._captured: dict[int, CacheStep] = {}  # steps in graphs, whose arrays have to stay
         self._layers = [self.pool.data_ptr() + i * self.pool.stride(0) for i in range(self.n_layers)]

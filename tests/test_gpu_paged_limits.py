@@ -5,7 +5,7 @@ from __future__ import annotations
 
 import pytest
 import torch
-from test_gpu_paged import BF16, FP16, FP32, attention, cells, held, make, queries
+from test_gpu_paged import BF16, FP16, FP32, attention, cells, check_attend, held, make, queries, read_equal
 
 from kvcompress_b200 import ops
 
@@ -143,3 +143,29 @@ def test_more_than_65535_items_of_many_columns():
     want = same_for_all(q, k, v, 64)
     assert (got - want).norm() <= 5e-3 * want.norm()
     assert (got - want).abs().max() <= 2 ** -7 * v.abs().max()
+
+
+# ---- other modes of torch ----------------------------------------------------
+
+
+@pytest.mark.parametrize("made, used", [(True, False), (False, True), (True, True)])
+def test_inference_mode(made, used):
+    """A cache made in inference mode is used outside it, and the other way round."""
+    k, v = cells(70, 2, 64, BF16)
+    q = queries(3, 4, 64, BF16)
+    with torch.inference_mode(made):
+        c = make(2, 64, pages=64)
+        a = c.add()
+        c.write(0, k[:30], v[:30], c.extend([a], [30]))
+    with torch.inference_mode(used):
+        b = c.fork(a)
+        c.write(0, k[30:], v[30:], c.extend([b], [40]))
+        out = c.attend(0, q, c.view([b], [3]))
+        c.free(a)
+        c.compact()
+        assert torch.equal(out, c.attend(0, q, c.view([b], [3])))
+    with torch.inference_mode(made):
+        c.truncate(b, 50)
+        c.write(0, k[50:], v[50:], c.extend([b], [20]))
+        check_attend(c, q, c.view([b], [3]), [(k, v)])
+        read_equal(c, b, k, v)

@@ -808,7 +808,8 @@ def copy_pages(pools, src: Sequence[int], dst: Sequence[int]) -> None:
     is the page (a K or V cache of each layer, say), of any element type, or one
     tensor whose first dimension indexes the pools.  ``src`` / ``dst``: page numbers
     on the host.  A page may be copied to several places; no page may be written
-    twice, or be read and written (``ValueError``)."""
+    twice, or be read and written (``ValueError``).  Autograd sees the pools as
+    changed in place; pools that need a gradient are refused while it records."""
     if isinstance(pools, torch.Tensor):
         shape = pools.shape
         if len(shape) < 2:
@@ -819,6 +820,7 @@ def copy_pages(pools, src: Sequence[int], dst: Sequence[int]) -> None:
             raise ValueError("copy_pages: pools must be contiguous")
         base, step, size = pools.data_ptr(), pools.stride(0) * pools.element_size(), pools.element_size()
         ptrs, n_pages, elems, device = [base + i * step for i in range(shape[0])], shape[1], pools[:1].numel(), pools.device
+        xs = [pools]
     else:
         xs = list(pools)
         for i in range(0, len(xs), KVC.MAX_CELLS):
@@ -829,6 +831,8 @@ def copy_pages(pools, src: Sequence[int], dst: Sequence[int]) -> None:
             return
         ptrs, n_pages, elems, device = [x.data_ptr() for x in xs], xs[0].shape[0], xs[0].numel(), xs[0].device
         size = xs[0].element_size()
+    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+        raise RuntimeError("copy_pages: there is no gradient through copied pages; use torch.no_grad() or detach()")
     n = len(src)
     if n != len(dst):
         raise ValueError(f"copy_pages: {n} sources but {len(dst)} destinations")
@@ -851,3 +855,4 @@ def copy_pages(pools, src: Sequence[int], dst: Sequence[int]) -> None:
         _call("copy_pages", device, 2 * n * page_bytes * len(part), lib().kvc_copy_pages, len(part),
               part.buffer_info()[0], n_pages, page_bytes, n, a.buffer_info()[0],
               b.buffer_info()[0])
+    torch.autograd.graph.increment_version([x for x in xs if not x.is_inference()])

@@ -169,3 +169,30 @@ def test_inference_mode(made, used):
         c.write(0, k[50:], v[50:], c.extend([b], [20]))
         check_attend(c, q, c.view([b], [3]), [(k, v)])
         read_equal(c, b, k, v)
+
+
+def test_copied_pages_and_autograd():
+    for many in (False, True):
+        pool = torch.randn(2, 4, 8, device="cuda")
+        w = torch.ones_like(pool).requires_grad_()
+        want = pool.clone()
+        want[:, 1] = want[:, 0]
+        y = (pool * w).sum()
+        ops.copy_pages(list(pool.unbind(0)) if many else pool, [0], [1])
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        assert torch.equal(pool, want)
+        pool.requires_grad_()
+        for x in (pool, pool * 1):
+            with pytest.raises(RuntimeError, match="gradient"):
+                ops.copy_pages(list(x.unbind(0)) if many else x, [2], [3])
+        assert torch.equal(pool, want)
+        with torch.no_grad():
+            ops.copy_pages(list(pool.unbind(0)) if many else pool, [2], [3])
+            want[:, 3] = want[:, 2]
+        assert torch.equal(pool, want)
+        with torch.inference_mode():
+            x = pool * 1
+            ops.copy_pages(list(x.unbind(0)) if many else x, [0], [2])
+            want[:, 2] = want[:, 0]
+        assert torch.equal(x, want)

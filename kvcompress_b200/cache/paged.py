@@ -41,10 +41,10 @@ class _Fence:
     """What the cache itself has put on a stream (a table's update, page copies, a
     step's arrays), for the other streams that use it."""
 
-    __slots__ = ("device", "event", "streams", "buf")
+    __slots__ = ("device", "event", "streams", "bufs")
 
-    def __init__(self, device: torch.device, buf: torch.Tensor | None = None) -> None:
-        self.device, self.buf = device, buf  # ``buf``: not to be reused before its uses are done
+    def __init__(self, device: torch.device, *bufs: torch.Tensor) -> None:
+        self.device, self.bufs = device, bufs  # ``bufs``: memory not to be reused before its uses are done
         with torch.cuda.device(device):
             self.event = torch.cuda.Event()
         self.mark()
@@ -67,8 +67,8 @@ class _Fence:
             return
         cur = torch.cuda.current_stream(self.device)
         cur.wait_event(self.event)
-        if self.buf is not None:
-            self.buf.record_stream(cur)
+        for buf in self.bufs:
+            buf.record_stream(cur)
         self.streams.add(stream)
 
 
@@ -91,8 +91,9 @@ class _Upload(_Fence):
             view[n:n + a.size] = a
             offsets.append(n)
             n += a.size
-        super().__init__(device, host.to(device, non_blocking=True))
-        self.at = [self.buf.data_ptr() + 4 * o for o in offsets]  # the arrays' addresses
+        buf = host.to(device, non_blocking=True)
+        super().__init__(device, buf)
+        self.at = [buf.data_ptr() + 4 * o for o in offsets]  # the arrays' addresses
 
 
 @dataclass
@@ -239,7 +240,7 @@ class PagedKVCache:
             self.table = torch.zeros(self.pages.table.shape, dtype=torch.int32, device=device)
             self._byte = torch.zeros(1, dtype=torch.uint8, device=device)  # workspaces are empty_like its expansions
         self._shapes: dict[tuple[int, int, int], tuple[int, int, bool]] = {}
-        self._fence = _Fence(device)
+        self._fence = _Fence(device, self.pool, self.table)
         self._captured: dict[int, CacheStep] = {}  # steps in graphs, whose arrays have to stay
         self._layers = [self.pool.data_ptr() + i * self.pool.stride(0) for i in range(self.n_layers)]
         self._layout = Kv4Layout(self.table.data_ptr(), self.table.stride(0), self.pages.n_pages, self.n_kv_heads,

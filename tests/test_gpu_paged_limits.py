@@ -3,6 +3,8 @@ columns, other modes of torch, memory used on several streams."""
 
 from __future__ import annotations
 
+import gc
+
 import pytest
 import torch
 from test_gpu_paged import BF16, FP16, FP32, attention, cells, check_attend, held, make, queries, read_equal
@@ -196,3 +198,30 @@ def test_copied_pages_and_autograd():
             ops.copy_pages(list(x.unbind(0)) if many else x, [0], [2])
             want[:, 2] = want[:, 0]
         assert torch.equal(x, want)
+
+
+# ---- memory used on several streams ---------------------------------------------
+
+
+def test_a_dropped_caches_memory_is_kept_for_another_streams_work():
+    c = make(2, 64, 64, 64, 64 * 4000, 1, dirty=False)
+    s = c.add()
+    k, v = cells(3000, 2, 64, BF16)
+    q = queries(1, 4, 64, BF16)
+    c.write(0, k, v, c.extend([s], [3000]))
+    step = c.view([s], [1])
+    want = c.attend(0, q, step)
+    torch.cuda.synchronize()
+    at, shape = c.pool.data_ptr(), c.pool.shape
+    assert c.pool.numel() > 20 << 20  # a block of its own, which the allocator would hand out again at once
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(1_000_000_000)  # about half a second, longer than the collection below
+        got = c.attend(0, q, step)
+    del c, step
+    gc.collect()
+    new = torch.empty(shape, dtype=torch.uint8, device="cuda")
+    assert not side.query()
+    assert new.data_ptr() != at
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)

@@ -225,3 +225,47 @@ def test_a_dropped_caches_memory_is_kept_for_another_streams_work():
     assert new.data_ptr() != at
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+# ---- roundings -------------------------------------------------------------------
+
+
+def loud_cells(n, d, dtype, by, off):
+    """K with d / 16 channels `by` times as loud, half of them shifted by `off`."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    size, shift = torch.ones(d, device="cuda"), torch.zeros(d, device="cuda")
+    at = torch.randperm(d, generator=g, device="cuda")[:d // 16]
+    size[at] = by
+    shift[at[::2]] = off
+    k = torch.randn(n, 1, d, generator=g, device="cuda") * size + shift
+    return k.to(dtype), torch.randn(n, 1, d, generator=g, device="cuda").to(dtype)
+
+
+# (not float32 with far offsets: its own rounding of logits of hundreds dominates there)
+@pytest.mark.parametrize("dtype, by, off", [(t, by, off) for t in (BF16, FP16, FP32)
+                                            for by, off in ((8, 4), (20, 4), (8, 60), (8, 200)) if t != FP32 or off == 4])
+@pytest.mark.parametrize("d, group", [(64, 64), (64, 32), (128, 128), (128, 64), (128, 32)])
+@pytest.mark.parametrize("nq", [2, 8, 60])
+def test_roundings_are_those_that_are_stated(dtype, by, off, d, group, nq):
+    """The norm of the error over 1500 tokens, against the roundings that each path is to have.
+
+    A value rounded to m bits (half a step 2^-m of its power of two) is off by 2^-m / sqrt 3 of that power in the mean square,
+    0.72 of which is the mean relative error of evenly spread mantissas: bf16 (m = 8) 1.63e-3, float16 (m = 11) 2.0e-4.
+    Outputs, weights and values (one float16 rounding each at most) are independent: sqrt 3 2.0e-4 = 3.5e-4 for float16
+    outputs, 1.65e-3 for bf16.  Where held K is rounded to float16 (16-bit queries of more than 32 columns, but for
+    float16 at d = 64), a logit is off by 2^-11 / sqrt 3 of each |q k| at most, added as squares; an independent error
+    of the logits changes the result by as much.  float32 queries: 22-bit terms and float32 sums of logits up to 20."""
+    c = make(1, d, group, 64, 2048, 1)
+    s = c.add()
+    k, v = loud_cells(1500, d, dtype, by, off)
+    c.write(0, k, v, c.extend([s], [1500]))
+    q = queries(nq, 4, d, dtype, size=1.0)
+    got = c.attend(0, q, c.view([s], [nq]), causal=False).double()
+    kh = held(k, group)
+    want, _ = attention(q, kh, held(v, group), False, d ** -0.5)
+    tol = {BF16: 2e-3, FP16: 4e-4, FP32: 2e-6}[dtype]
+    if dtype != FP32 and nq * 4 > 32 and not (dtype == FP16 and d == 64):
+        squares = torch.einsum("nhd,td->nht", q.double() ** 2, kh[:, 0] ** 2).mean().item()
+        tol = (tol ** 2 + squares / d * 2.0 ** -22 / 3) ** 0.5
+    err = ((got - want).norm() / want.norm()).item()
+    assert err <= tol, (err, tol)

@@ -752,8 +752,15 @@ int join(const Layout& L, const Step& S, const Split& P, const Qkv& a, const Par
               : launch_after("attend_join_kernel", attend_join_kernel<D, false>, dim3((unsigned)blocks), 128, 0, st, L, S, P, a, part, rows);
 }
 
-// 16-bit queries with more columns than this go to the kernel for many queries.
-constexpr int kFewColumns = 32;
+// 16-bit queries with more columns than this go to the kernel for many queries,
+// whose time hardly depends on them up to 128 (this one's / that one's us, in a graph):
+//   columns                                      16      32      48       64       128
+//   8 x 8192 tokens, 8 KV heads of 128        36 / 89 58 / 89 77 / 92 100 / 92 199 / 99
+//   32 x 4096, the same heads                64 / 170 110 / 169 148 / 170 197 / 170 324 / 172
+//   8 x 2048, 4 KV heads of 64             11.6 / 16.4 14.5 / 16.4 16.7 / 16.7 18.1 / 16.8 24.9 / 17.4
+//   2 x 1500, 12 KV heads of 64, float16   10.6 / 14.7 11.5 / 14.8 12.9 / 14.9 14.9 / 15.1 18.2 / 15.8
+//   1 x 8192, 8 KV heads of 128            14.5 / 19.2 18.8 / 19.3 21.0 / 19.4 23.0 / 19.8 34.0 / 23.6
+constexpr int kFewColumns = 48;
 bool many(int64_t cols, int dtype) { return dtype != KVC_F32 && cols > kFewColumns; }
 
 // Tiles of 8 columns a block takes.  Four, with 8 warps an SM for their

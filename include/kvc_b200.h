@@ -333,10 +333,13 @@ int kvc_set_kernel_policy(int policy);
  * that is no page sets the device error word (401); it is never followed, and
  * what stands for its tokens is not defined.
  *
- * The table and the arrays of kvc_kv4_step and kvc_kv4_split are written by
- * copies (cudaMemcpyAsync): the kernels may read them before the kernel in
- * front of them in the stream has ended, if that one allows it (programmatic
- * dependent launch).
+ * The kernels may read the table and the arrays of kvc_kv4_step and
+ * kvc_kv4_split before the kernel in front of them in the stream has ended
+ * (programmatic dependent launch).  So these are written by copies
+ * (cudaMemcpyAsync), or by a kernel that a copy or an ordinary kernel follows
+ * before the first call here that reads what it wrote.
+ *
+ * A sequence has at most 2^31 - 257 tokens.
  */
 typedef struct {
   const int32_t* table;

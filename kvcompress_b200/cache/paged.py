@@ -205,8 +205,23 @@ class PagedKVCache:
     ``attend`` are not).  ``write`` and ``attend`` may be captured into a CUDA graph
     once the step has been used outside one; the graph then repeats that step, and
     must not outlive the cache, which keeps the captured steps' arrays.  ``extend``,
-    ``compact`` and a step's first use cannot be captured.  There is no gradient
-    through a cache in 4 bits.
+    ``compact`` and a step's first use cannot be captured: a decoding loop, whose
+    every token is a new step, runs uncaptured.  There is no gradient through a
+    cache in 4 bits.
+
+    A step's host work is paid once for all its layers: ``extend`` 13 to 174 us (1 to
+    256 sequences), the first ``write`` 75 to 115 us more than the later ones, the
+    first ``attend`` 150 to 185.  Sequences with very different numbers of
+    queries are best given steps of their own where one of them has a long context
+    (a step is split by its largest number of queries; single tokens beside prompts
+    are taken apart already).
+
+    How near 4 bits come depends on K's channels: unit normal queries over 8192
+    tokens of rotated keys with 8 of 128 channels 8 times as loud are off by 48% with
+    one group a head, 42% with groups of 64 and 32% with groups of 32 (by V alone
+    10, 9 and 8%).  An orthogonal rotation of K and of the queries before ``write``
+    and ``attend`` (a Hadamard matrix over 128 ** 0.5, say) leaves the logits alone and
+    spreads the loud channels: 26, 22 and 21%.
     """
 
     def __init__(self, *, n_layers: int, n_pages: int, n_kv_heads: int, head_dim: int, page_size: int = 64,
@@ -309,6 +324,8 @@ class PagedKVCache:
 
     def _prepare(self, step: CacheStep) -> None:
         """Put the step's arrays on the device."""
+        # The attention reads the page table before the kernel in front of it has ended,
+        # so the table's update must not be that kernel: the copy below has to follow it.
         self._sync()
         n, lengths = np.array(step.counts, dtype=np.int64), np.array(step.lengths, dtype=np.int64)
         rows = np.array([self.pages.row(s) for s in step.seqs], dtype=np.int64)

@@ -2,10 +2,10 @@
 //
 // Figures are for one layer of 32768 tokens, 8 heads of 128, bf16, one group a
 // head: 134 MB dense and 36 MB packed, 26 us at the copy peak of 6.55 TB/s.  The
-// write takes 47.5 us (3.6 TB/s), bound by instruction issue (61% of the slots over
-// the whole launch): it forms 268M exactly rounded codes and moves 1 GB through
-// registers as float32.  The read takes 27 us (6.3 TB/s), bound by memory; page
-// copies reach 96% of the copy peak.  A warp of the write and read kernels takes 8
+// write takes 47.5 us (3.6 TB/s): it forms 67M exactly rounded codes at 16
+// instructions each, which fill 65% of the issue slots over the whole launch; the
+// rest are waits for its inputs.  The read takes 27 us (6.3 TB/s), bound by memory;
+// page copies reach 96% of the copy peak.  A warp of the write and read kernels takes 8
 // tokens of one head's K and V, 4 lanes a token: lane c of a token holds the
 // features 32 w + 8 c + 0..7, which is both a 16-byte load of a 16-bit input
 // (4 lanes: 64 contiguous bytes) and word w of K's chunk c, so K's codes need

@@ -99,9 +99,12 @@ __device__ __forceinline__ __half2 centred_hi(uint32_t w) {
 // Programmatic launches: a kernel launched with launch_after may start while
 // the previous one of its stream runs; grid_wait returns when that one is
 // complete and its writes are visible.  Every thread comes by it, before it
-// ends too, so that a kernel's end is also the end of those before it.  Only a
-// step's own arrays and the page table are read earlier: they are written by
-// copies.  grid_go lets the next such kernel start (its grid_wait still waits
+// ends too, so that a kernel's end is also the end of those before it.  Only the
+// step's and the split's arrays and the page table are read earlier.  So whatever
+// writes an entry that a kernel here will read must not be the very kernel in front
+// of it: a copy, or an ordinary kernel, has to lie between them in the stream.  The
+// arrays are written by copies; the table is updated by a kernel, with the copy of a
+// step's arrays behind it.  grid_go lets the next such kernel start (its grid_wait still waits
 // for this grid's end); it comes after grid_wait, so that no more than two
 // kernels are under way.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

@@ -42,12 +42,13 @@
 // attend_join_kernel in a fixed order.
 //
 // Measured, with the write of the new token and the join: one query of 32 heads
-// over 8 x 32768 tokens (8 KV heads of 128, 285 MB) 63 us, of 16 heads over 4 x
+// over 8 x 32768 tokens (8 KV heads of 128, 285 MB) 63 us, of 28 heads over 4 x
 // 131072 (4 KV heads) also 63, 58 in a graph; 44 us at the copy peak.  The loads
 // alone (ring without arithmetic) take 50 us and the arithmetic alone as long:
 // half of the issue slots, a third of the tensor pipe's cycles.  Start, end and
-// join are 12 to 15 us of it.  Four queries of 32 heads over 8 x 8192 tokens
-// (32 columns) take 39 us, bound by the arithmetic of their columns.
+// join are 12 to 15 us of it.  Four queries of 64 heads over 8 sequences of up to
+// 8192 tokens (32 columns) take 44 us, bound by the arithmetic of their columns, and
+// one of 32 heads over 33 sequences of up to 8191 in groups of 32 66 us.
 #include <algorithm>
 #include <type_traits>
 

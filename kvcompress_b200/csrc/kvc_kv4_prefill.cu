@@ -27,18 +27,25 @@
 // a flagged token gets NaN in that group at the end.
 //
 // Roundings to 16 bits: weights to float16, half a step of 2^-11, and K and V
-// (zero + scale q has up to 16 bits) likewise, which bfloat16 queries' own output
-// hides.  Float16 queries would show it (7e-4 of the result over 1500 tokens with
-// loud channels in K, 2e-4 with exact values), so where the tiles fit, for d = 64, K
-// and V are held in two terms, which costs time (1001 queries of each of 2
-// sequences over 1500 tokens, 12 heads of 64: 31 -> 41 us); for d = 128 the second
-// terms would leave one buffer each (306 -> 634 us with K's alone).  Queries are
-// held in float16 under a power of two a row.
+// (zero + scale q has up to 16 bits) likewise, as if the cache had been decoded to
+// float16.  K's moves a logit by up to 2^-11 sum |q k|, so it grows with K's loud
+// channels (as the 4 bits' own half step does, 1/30 of a group's span: 68 times as
+// much).  Error of the result over 1500 tokens of d = 128, with exact values 2.0e-4
+// for float16 and 1.66e-3 for bfloat16 queries (the output's own rounding, which is 8
+// times coarser than K's): 6e-4 and 1.75e-3 with channels 8 times as loud, 7.5e-4 and
+// 1.85e-3 with 20 times, 1.9e-3 and 2.4e-3 with channels at 60, 3.8e-3 and 4.2e-3 at
+// 200.  The kernel for few queries has none of this (its operands are the codes).
+// For float16 queries, where it shows most, K and V are held in two terms where the
+// tiles fit, for d = 64 (2.2e-4 to 2.6e-4 on all of these), which costs time (1001
+// queries of each of 2 sequences over 1500 tokens, 12 heads of 64: 31 -> 41 us); for
+// d = 128 the second terms would leave one buffer each (306 -> 634 us with K's alone).
+// Queries are held in float16 under a power of two a row.
 //
 // Measured: 2048 queries of 32 heads over 8192 tokens (8 KV heads of 128,
-// bfloat16) 304 us, 790 TFLOP/s, 47% of the GEMM peak; the float16 case above 41
-// us.  Bound by latency along one row tile's chain: a step of 128 tokens takes about 4200 clocks, of which the
-// products are 2048 (tensor pipe 45%), the exponentials of both tiles 2048 (41%),
+// bfloat16) 310 to 325 us as the clock allows, 740 to 780 TFLOP/s, 44 to 46% of the
+// GEMM peak, and 332 with their write; the float16 case above 41 us.  Bound by latency
+// along one row tile's chain: a step of 128 tokens takes about 4200 clocks, of which the
+// products are 2048 (tensor pipe 46%), the exponentials of both tiles 2048 (42%),
 // and one tile's softmax 2500 from its logits' arrival to its last weights.  One
 // block an SM: 227 KB of shared memory and all of TMEM.
 #include <algorithm>

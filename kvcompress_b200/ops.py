@@ -808,8 +808,9 @@ def copy_pages(pools, src: Sequence[int], dst: Sequence[int]) -> None:
     is the page (a K or V cache of each layer, say), of any element type, or one
     tensor whose first dimension indexes the pools.  ``src`` / ``dst``: page numbers
     on the host.  A page may be copied to several places; no page may be written
-    twice, or be read and written (``ValueError``).  Autograd sees the pools as
-    changed in place; pools that need a gradient are refused while it records."""
+    twice, or be read and written (``ValueError``), and pools must not overlap.
+    Autograd sees them as changed in place; pools that need a gradient are refused
+    while it records."""
     if isinstance(pools, torch.Tensor):
         shape = pools.shape
         if len(shape) < 2:

@@ -755,14 +755,17 @@ int join(const Layout& L, const Step& S, const Split& P, const Qkv& a, const Par
 
 // 16-bit queries with more columns than this go to the kernel for many queries,
 // whose time hardly depends on them up to 128 (this one's / that one's us, in a graph):
-//   columns                                      16      32      48       64       128
-//   8 x 8192 tokens, 8 KV heads of 128        36 / 89 58 / 89 77 / 92 100 / 92 199 / 99
-//   32 x 4096, the same heads                64 / 170 110 / 169 148 / 170 197 / 170 324 / 172
-//   8 x 2048, 4 KV heads of 64             11.6 / 16.4 14.5 / 16.4 16.7 / 16.7 18.1 / 16.8 24.9 / 17.4
-//   2 x 1500, 12 KV heads of 64, float16   10.6 / 14.7 11.5 / 14.8 12.9 / 14.9 14.9 / 15.1 18.2 / 15.8
-//   1 x 8192, 8 KV heads of 128            14.5 / 19.2 18.8 / 19.3 21.0 / 19.4 23.0 / 19.8 34.0 / 23.6
-constexpr int kFewColumns = 48;
-bool many(int64_t cols, int dtype) { return dtype != KVC_F32 && cols > kFewColumns; }
+//   columns                               16          48           64           96          128
+//   bfloat16
+//   8 x 8192, 8 KV heads of 128      36 / 89     77 / 92     100 / 92     134 / 96     199 / 99
+//   32 x 4096, the same heads       64 / 170   148 / 170    197 / 170    274 / 171    324 / 172
+//   8 x 2048, 4 KV heads of 64     11.6 / 16.4 16.7 / 16.7 18.1 / 16.8  21.0 / 17.1  24.9 / 17.4
+//   float16, in two terms there
+//   2 x 1500, 12 KV heads of 64    10.6 / 14.7 12.9 / 14.9 14.9 / 15.1  17.0 / 15.5  18.2 / 15.8
+//   8 x 8192, 8 KV heads of 128         –       77 / 141    100 / 142    134 / 145    198 / 148
+//   32 x 4096, the same heads           –      147 / 266    196 / 266    273 / 267    324 / 268
+constexpr int few_columns(int dtype, int head_dim) { return dtype == KVC_F16 && head_dim == 128 ? 96 : 48; }
+bool many(int64_t cols, int dtype, int head_dim) { return dtype != KVC_F32 && cols > few_columns(dtype, head_dim); }
 
 // Tiles of 8 columns a block takes.  Four, with 8 warps an SM for their
 // registers, were slower than two blocks of two that read the codes twice
@@ -813,7 +816,7 @@ extern "C" int kvc_kv4_attend_shape(const kvc_kv4_layout* layout, int max_new, i
   if (n_q < 1 || n_q % layout->n_kv) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend_shape: n_q must be a multiple of n_kv");
   const int64_t cols = std::max<int64_t>(1, (int64_t)max_new * (n_q / layout->n_kv));
   if (cols > INT32_MAX / 2) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend_shape: too many queries");
-  if (many(cols, dtype)) {
+  if (many(cols, dtype, layout->head_dim)) {
     *tiles = (int)prefill_tiles(cols);
     *resident = num_sms();
     *spanning = 0;
@@ -849,7 +852,7 @@ extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* 
   if (n_q < 1 || n_q > 65535 || n_q % layout->n_kv) return fail(KVC_ERR_SHAPE, "kvc_kv4_attend: n_q must be a multiple of n_kv");
   if (step->n_tokens == 0 || split->n_items == 0) return KVC_OK;
   if (!step->rows || !step->kv_len || !step->q_start) return fail(KVC_ERR_ARG, "kvc_kv4_attend: NULL step");
-  if (!split->item_start || (!many((int64_t)split->max_new * (n_q / layout->n_kv), dtype) && !split->block_start))
+  if (!split->item_start || (!many((int64_t)split->max_new * (n_q / layout->n_kv), dtype, layout->head_dim) && !split->block_start))
     return fail(KVC_ERR_ARG, "kvc_kv4_attend: NULL split");
   if (!split->items || !aligned16(split->items)) return fail(KVC_ERR_ALIGN, "kvc_kv4_attend: items not 16-byte aligned");
   if (step->n_tokens < 0 || step->n_tokens > INT32_MAX || split->max_new < 1 || split->n_items < 0 ||
@@ -869,7 +872,7 @@ extern "C" int kvc_kv4_attend(const kvc_kv4_layout* layout, const kvc_kv4_step* 
   const Layout L = to_layout(layout);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc = KVC_OK;
-  if (many(cols, dtype)) {
+  if (many(cols, dtype, layout->head_dim)) {
     rc = launch_prefill(layout, s, p, static_cast<const uint8_t*>(pool), a, part, split->n_items, st);
   } else {
 #define KVC_F(D, WPG) rc = launch_tiles<D, WPG>(L, s, p, pool, a, part, split->n_blocks, (int)cols, st)

@@ -762,8 +762,8 @@ int join(const Layout& L, const Step& S, const Split& P, const Qkv& a, const Par
 //   8 x 2048, 4 KV heads of 64     11.6 / 16.4 16.7 / 16.7 18.1 / 16.8  21.0 / 17.1  24.9 / 17.4
 //   float16, in two terms there
 //   2 x 1500, 12 KV heads of 64    10.6 / 14.7 12.9 / 14.9 14.9 / 15.1  17.0 / 15.5  18.2 / 15.8
-//   8 x 8192, 8 KV heads of 128         –       77 / 141    100 / 142    134 / 145    198 / 148
-//   32 x 4096, the same heads           –      147 / 266    196 / 266    273 / 267    324 / 268
+//   8 x 8192, 8 KV heads of 128         -       77 / 141    100 / 142    134 / 145    198 / 148
+//   32 x 4096, the same heads           -      147 / 266    196 / 266    273 / 267    324 / 268
 constexpr int few_columns(int dtype, int head_dim) { return dtype == KVC_F16 && head_dim == 128 ? 96 : 48; }
 bool many(int64_t cols, int dtype, int head_dim) { return dtype != KVC_F32 && cols > few_columns(dtype, head_dim); }
 

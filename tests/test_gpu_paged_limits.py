@@ -14,7 +14,7 @@ from kvcompress_b200 import ops
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("dtype, nq", [(BF16, 1), (BF16, 16), (FP32, 1)])
+@pytest.mark.parametrize("dtype, nq", [(BF16, 1), (BF16, 16), (FP16, 64), (FP32, 1)])
 def test_the_longest_sequence(dtype, nq):
     """2^31 - 300 tokens (the limit is 2^31 - 257) whose table row names the same three pages over and over.  Positions of
     tokens past the last one do not fit in 32 bits: none may be looked up in the table.
@@ -38,7 +38,7 @@ def test_the_longest_sequence(dtype, nq):
     k, v = held(k, 64)[:, 0], held(v, 64)[:, 0]
     p = torch.softmax(torch.einsum("nhd,td->nht", q.double(), k) / 8 + times.log(), -1)
     want = torch.einsum("nht,td->nhd", p, v)
-    tol = (5.4e-2 if nq == 16 else 7e-3) + torch.finfo(dtype).eps / 2
+    tol = (5.4e-2 if nq >= 16 else 7e-3) + torch.finfo(dtype).eps / 2
     assert (got - want).abs().max() <= tol * v.abs().max()
     assert ops.device_error() == 0
 
@@ -299,3 +299,18 @@ def test_columns_on_both_sides_of_the_kernels_limit(dtype, d, group):
     for counts in ([16, 16, 16], [17, 17, 17], [15, 16, 17], [32, 33, 30], [1, 17, 33], [100, 33, 1]):  # of 3 columns each
         for causal in (True, False):
             check_attend(c, queries(sum(counts), 6, d, dtype), c.view(seqs, counts), kv, causal)
+
+
+@pytest.mark.parametrize("d, group", [(64, 64), (64, 32), (128, 128), (128, 64), (128, 32)])
+@pytest.mark.parametrize("nq, lens", [(26, [3000]), (200, [4000]), (150, [2500, 800, 64, 63])])
+def test_repeated_float16_calls_give_the_same_bits(d, group, nq, lens):
+    """Tiles in two terms, whose codes two sets of warps read: one that came too late or too early would show."""
+    c = make(4, d, group, 32, 4096, len(lens), pages=300)
+    seqs = [c.add() for _ in lens]
+    k, v = cells(sum(lens), 4, d, FP16)
+    c.write(0, k, v, c.extend(seqs, lens))
+    step = c.view(seqs, [nq] * len(lens))
+    q = queries(nq * len(lens), 16, d, FP16)
+    out = check_attend(c, q, step, list(zip(k.split(lens), v.split(lens))))
+    assert not torch.stack([(c.attend(0, q, step) != out).any() for _ in range(60)]).any()
+    assert ops.device_error() == 0
